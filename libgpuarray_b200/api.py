@@ -39,6 +39,10 @@ GA_ANY_ORDER, GA_C_ORDER, GA_F_ORDER = -1, 0, 1
 GA_SUM, GA_PROD, GA_MAX, GA_MIN = range(4)
 GA_COMM_ID_BYTES = 128
 
+GA_EMBED_PAD, GA_EMBED_CHECK, GA_EMBED_ACCUMULATE = 0x1, 0x2, 0x4
+GA_LOGPROBS_IGNORE, GA_LOGPROBS_CHECK = 0x1, 0x2
+GA_LOGPROBS_MAX_TOP = 32
+
 _NP2GA = {
     np.dtype(np.bool_): GA_BOOL, np.dtype(np.int8): GA_BYTE, np.dtype(np.uint8): GA_UBYTE,
     np.dtype(np.int16): GA_SHORT, np.dtype(np.uint16): GA_USHORT, np.dtype(np.int32): GA_INT,
@@ -163,6 +167,18 @@ def lib():
         ctypes.c_char_p, ci, cu, ctypes.POINTER(_ElemwiseArg), ci)
     sig("GpuMapReduction_free", None, vp)
     sig("GpuMapReduction_call", ci, vp, A, ctypes.POINTER(vp), cu, ctypes.POINTER(ci), ci)
+    cd, pA = ctypes.c_double, ctypes.POINTER(A)
+    sig("GpuArray_embed", ci, A, A, A, cd, ctypes.c_ssize_t, ci)
+    sig("GpuEmbedGrad_new", ci, ctypes.POINTER(vp), vp)
+    sig("GpuEmbedGrad_free", None, vp)
+    sig("GpuEmbedGrad_call", ci, vp, A, A, A, cd, ctypes.c_ssize_t, ci)
+    sig("GpuLogProbs_new", ci, ctypes.POINTER(vp), vp, ci, ci, cu)
+    sig("GpuLogProbs_free", None, vp)
+    sig("GpuLogProbs_call", ci, vp, A, A, A, A, A, A, A, cd, ctypes.c_ssize_t, ci)
+    sig("GpuLogProbs_grad", ci, vp, A, A, A, A, A, A, A, cd, ctypes.c_ssize_t, ci)
+    sig("GpuClipNorm_new", ci, ctypes.POINTER(vp), vp)
+    sig("GpuClipNorm_free", None, vp)
+    sig("GpuClipNorm_call", ci, vp, A, pA, pA, cu, cd, cd)
     for name in ("gpucomm_new", "gpucomm_free", "gpucomm_gen_clique_id", "gpucomm_all_reduce",
                  "gpucomm_get_count", "gpucomm_get_rank"):
         if not hasattr(L, name):
@@ -642,6 +658,142 @@ def maxandargmax(dst_max, dst_argmax, src, axes):
     _check(src.ctx.ptr, lib().GpuArray_maxandargmax(ctypes.byref(dst_max.ga),
                                                     ctypes.byref(dst_argmax.ga),
                                                     ctypes.byref(src.ga), len(axes), ax))
+
+
+def _ref(a):
+    """The C struct of an array, or NULL for None."""
+    return None if a is None else ctypes.byref(a.ga)
+
+
+def embed(out, table, ids, scale=1.0, pad=None, check=False):
+    """GpuArray_embed (include/gpuarray/embedding.h): out[t, :] = scale * table[ids[t], :],
+    rows of zeros where ids[t] == pad. check=True waits and raises for an id
+    outside the table."""
+    flags = (0 if pad is None else GA_EMBED_PAD) | (GA_EMBED_CHECK if check else 0)
+    err = lib().GpuArray_embed(_ref(out), _ref(table), _ref(ids), scale, pad or 0, flags)
+    if err:
+        _check(out.ctx.ptr, err)
+
+
+class _Operator:
+    """A C operator object made for a context and freed with this one."""
+
+    _free = None
+
+    def _made(self, ctx, new, *args):
+        self.ctx = ctx
+        self.ptr = None
+        p = ctypes.c_void_p()
+        _check(ctx.ptr, getattr(lib(), new)(ctypes.byref(p), ctx.ptr, *args))
+        self.ptr = p
+
+    def free(self):
+        if self.ptr is not None:
+            getattr(lib(), self._free)(self.ptr)
+            self.ptr = None
+
+    def __del__(self):
+        try:
+            if self.ctx.ptr is not None:
+                self.free()
+        except Exception:
+            pass
+
+
+class GpuEmbedGrad(_Operator):
+    """GpuEmbedGrad_new/_call/_free (include/gpuarray/embedding.h): the gradient
+    of embed() for the table, dtable[v, :] = scale * sum of dout[t, :] over the
+    tokens with ids[t] == v. With accumulate=True it is added to dtable and
+    only the rows that tokens name are touched."""
+
+    _free = "GpuEmbedGrad_free"
+
+    def __init__(self, ctx):
+        self._made(ctx, "GpuEmbedGrad_new")
+
+    def __call__(self, dtable, dout, ids, scale=1.0, pad=None, accumulate=False, check=False):
+        flags = ((0 if pad is None else GA_EMBED_PAD) | (GA_EMBED_CHECK if check else 0) |
+                 (GA_EMBED_ACCUMULATE if accumulate else 0))
+        err = lib().GpuEmbedGrad_call(self.ptr, _ref(dtable), _ref(dout), _ref(ids), scale,
+                                      pad or 0, flags)
+        if err:
+            _check(self.ctx.ptr, err)
+
+
+class GpuLogProbs(_Operator):
+    """GpuLogProbs_new/_call/_grad/_free (include/gpuarray/logprobs.h): log
+    probabilities of given tokens under rows of logits, the rows' entropy and
+    their `top` most likely alternatives, and the gradient of the first two.
+
+    Destinations are passed by name; those left out are not computed. `stats`
+    holds what grad() needs of the forward pass; rows whose target equals
+    `ignore` have a logp of 0 without a gradient."""
+
+    _free = "GpuLogProbs_free"
+
+    def __init__(self, ctx, dtype, id_dtype=np.int64, top=0):
+        self.top = top
+        self._made(ctx, "GpuLogProbs_new", dtype if isinstance(dtype, int) else typecode(dtype),
+                   id_dtype if isinstance(id_dtype, int) else typecode(id_dtype), top)
+
+    def __call__(self, logits, targets=None, logp=None, entropy=None, stats=None, top_logp=None,
+                 top_ids=None, scale=1.0, ignore=None, check=False):
+        flags = (0 if ignore is None else GA_LOGPROBS_IGNORE) | (GA_LOGPROBS_CHECK if check else 0)
+        err = lib().GpuLogProbs_call(self.ptr, _ref(logp), _ref(entropy), _ref(stats), _ref(top_logp),
+                                     _ref(top_ids), _ref(logits), _ref(targets), scale, ignore or 0,
+                                     flags)
+        if err:
+            _check(self.ctx.ptr, err)
+
+    def grad(self, dlogits, logits, targets, stats, dlogp, entropy=None, dentropy=None, scale=1.0,
+             ignore=None, check=False):
+        """dlogits from the gradients arriving at logp and (with the entropy that the
+        forward pass wrote) at the entropy; dlogits may be the logits."""
+        flags = (0 if ignore is None else GA_LOGPROBS_IGNORE) | (GA_LOGPROBS_CHECK if check else 0)
+        err = lib().GpuLogProbs_grad(self.ptr, _ref(dlogits), _ref(logits), _ref(targets),
+                                     _ref(stats), _ref(dlogp), _ref(entropy), _ref(dentropy), scale,
+                                     ignore or 0, flags)
+        if err:
+            _check(self.ctx.ptr, err)
+
+
+class GpuArrayList:
+    """The C form of a list of arrays (const GpuArray *const *), made once for
+    arrays that are passed together often."""
+
+    def __init__(self, arrays):
+        self.arrays = list(arrays)
+        self.ptrs = (ctypes.POINTER(_GpuArrayStruct) * max(len(self.arrays), 1))(
+            *[ctypes.pointer(a.ga) for a in self.arrays])
+
+    def __len__(self):
+        return len(self.arrays)
+
+
+class GpuClipNorm(_Operator):
+    """GpuClipNorm_new/_call/_free (include/gpuarray/clipnorm.h): the norm over
+    all arrays of `srcs` times `scale`, and dsts[i] = srcs[i] * scale *
+    min(1, limit / norm). dsts may be srcs (in place) or None (the norm alone);
+    both are GpuArrayLists or sequences of arrays."""
+
+    _free = "GpuClipNorm_free"
+
+    def __init__(self, ctx):
+        self._made(ctx, "GpuClipNorm_new")
+
+    def __call__(self, norm, dsts, srcs, limit, scale=1.0):
+        if not isinstance(srcs, GpuArrayList):
+            same = dsts is srcs
+            srcs = GpuArrayList(srcs)
+            dsts = srcs if same else dsts
+        if dsts is not None and not isinstance(dsts, GpuArrayList):
+            dsts = GpuArrayList(dsts)
+        if dsts is not None and len(dsts) != len(srcs):
+            raise ValueError("%d destinations for %d arrays" % (len(dsts), len(srcs)))
+        err = lib().GpuClipNorm_call(self.ptr, _ref(norm), None if dsts is None else dsts.ptrs,
+                                     srcs.ptrs, len(srcs), scale, limit)
+        if err:
+            _check(self.ctx.ptr, err)
 
 
 class GpuComm:

@@ -277,6 +277,7 @@ void gpucontext_deref(gpucontext *ctx) {
   ga_extcopy_cache_free(ctx);
   ga_maxandargmax_cache_free(ctx);
   ga_take1_cache_free(ctx);
+  ga_lm_cache_free(ctx);
   ga_ctx_exit(ctx);
   ga_ctx_unref(ctx);
 }

@@ -1,0 +1,285 @@
+/* Token embedding and its gradient (include/gpuarray/embedding.h; kernels in
+ * templates/ga_embed.cuh). */
+#include "private.h"
+
+typedef struct em_layout { /* the templates' ga__em_layout */
+  unsigned long long n, v;
+  unsigned int nv, chunk, chunks;
+  int has_pad;
+  long long pad;
+  double scale;
+  unsigned long long dims[GA_LM_MAXD];
+  long long i_str[GA_LM_MAXD], t_str[GA_LM_MAXD];
+  long long t_col, v_row, v_col;
+} em_layout;
+
+struct _GpuEmbedGrad {
+  gpucontext *ctx;
+  ga_workspace ws;
+};
+
+static int is_real(int tc) { return tc == GA_HALF || tc == GA_FLOAT || tc == GA_DOUBLE; }
+
+/* key: A type | O type << 8 | id type << 16 | E << 24 | ND << 32 | gradient << 40 | accumulate << 41 */
+static void emit(ga_strb *sb, uint64_t key) {
+  const int a = (int)(key & 0xff), o = (int)((key >> 8) & 0xff), i = (int)((key >> 16) & 0xff);
+  ga_strb_printf(sb,
+                 "#include \"cluda.h\"\n#define %s\n#define GA_EM_A_T %s\n#define GA_EM_O_T %s\n"
+                 "#define GA_EM_I_T %s\n#define GA_EM_F_T %s\n#define GA_EM_E %u\n"
+                 "#define GA_EM_ND %u\n#define GA_EM_ACCUMULATE %u\n#include \"ga_embed.cuh\"\n",
+                 (key >> 40) & 1 ? "GA_EM_BUILD_GRAD" : "GA_EM_BUILD_LOOKUP", ga_ctype(a), ga_ctype(o),
+                 ga_ctype(i), a == GA_DOUBLE || o == GA_DOUBLE ? "ga_double" : "ga_float",
+                 (unsigned)((key >> 24) & 0xff), (unsigned)((key >> 32) & 0xff),
+                 (unsigned)((key >> 41) & 1));
+}
+
+static int check_types(gpucontext *ctx, const GpuArray *a, const GpuArray *o, const GpuArray *ids) {
+  if (!is_real(a->typecode) || !is_real(o->typecode))
+    return ga_err_set(ctx->err, GA_UNSUPPORTED_ERROR, "Rows must be half, float or double");
+  if (!ga_lm_is_id(ids->typecode))
+    return ga_err_set(ctx->err, GA_UNSUPPORTED_ERROR, "Token ids must be 32- or 64-bit integers");
+  return GA_NO_ERROR;
+}
+
+/* `by_token`: out or dout; `by_row`: the table or dtable */
+static int check_shapes(gpucontext *ctx, const GpuArray *by_token, const char *name,
+                        const GpuArray *by_row, const GpuArray *ids) {
+  if (by_row->nd != 2)
+    return ga_err_fmt(ctx->err, GA_VALUE_ERROR, "The table has %u dimensions, expected 2", by_row->nd);
+  if (by_token->nd != ids->nd + 1 || !ga_lm_same_dims(by_token, ids, ids->nd) ||
+      by_token->dimensions[ids->nd] != by_row->dimensions[1])
+    return ga_err_fmt(ctx->err, GA_VALUE_ERROR,
+                      "%s must have the dimensions of the ids and then the table's row length", name);
+  return GA_NO_ERROR;
+}
+
+/* Elements per access: the widest for which a load is at most 16 bytes and a store 32, the rows
+ * hold a whole number of them and every row of both arrays starts on a boundary of one. */
+static unsigned vector_width(const GpuArray *in, const GpuArray *out, size_t width) {
+  const GpuArray *a[2];
+  unsigned e, i, k;
+  a[0] = in;
+  a[1] = out;
+  e = 16 / (unsigned)gpuarray_get_elsize(in->typecode);
+  while (e * gpuarray_get_elsize(out->typecode) > 32) e /= 2;
+  for (; e > 1; e /= 2) {
+    int ok = width % e == 0;
+    for (k = 0; k < 2 && ok; k++) {
+      size_t es = gpuarray_get_elsize(a[k]->typecode), b = es * e > 16 ? 16 : es * e;
+      if (a[k]->strides[a[k]->nd - 1] != (ssize_t)es) ok = 0;
+      if ((a[k]->data->ptr + a[k]->offset) % b != 0) ok = 0;
+      for (i = 0; i + 1 < a[k]->nd; i++)
+        if (a[k]->dimensions[i] > 1 && a[k]->strides[i] % (ssize_t)b != 0) ok = 0;
+    }
+    if (ok) break;
+  }
+  return e;
+}
+
+static int fill(gpucontext *ctx, em_layout *L, ga_lead *lead, const GpuArray *by_token,
+                const GpuArray *by_row, const GpuArray *ids, double scale, ssize_t pad, int flags,
+                unsigned e) {
+  const ssize_t *str[2];
+  long long out[2][GA_LM_MAXD];
+  int err;
+  memset(L, 0, sizeof(*L));
+  str[0] = ids->strides;
+  str[1] = by_token->strides;
+  err = ga_lm_lead(ctx, ids->nd, ids->dimensions, 2, str, lead, out);
+  if (err != GA_NO_ERROR) return err;
+  L->n = lead->count;
+  L->v = by_row->dimensions[0];
+  L->nv = (unsigned)(by_row->dimensions[1] / e);
+  L->has_pad = ISSET(flags, GA_EMBED_PAD);
+  L->pad = pad;
+  L->scale = scale;
+  memcpy(L->dims, lead->dims, sizeof(L->dims));
+  memcpy(L->i_str, out[0], sizeof(L->i_str));
+  memcpy(L->t_str, out[1], sizeof(L->t_str));
+  L->t_col = by_token->strides[by_token->nd - 1];
+  L->v_row = by_row->strides[0];
+  L->v_col = by_row->strides[1];
+  return GA_NO_ERROR;
+}
+
+/* what both calls refuse before anything is enqueued */
+static int check_call(gpucontext *ctx, const GpuArray *by_row, int flags, int allowed) {
+  if (flags & ~allowed) return ga_err_fmt(ctx->err, GA_INVALID_ERROR, "Unknown flags 0x%x", flags);
+  if (by_row->dimensions[0] > 0x7fffffffUL || by_row->dimensions[1] > 0x7fffffffUL)
+    return ga_err_set(ctx->err, GA_XLARGE_ERROR, "The table has more than 2^31 - 1 rows or columns");
+  if (ISSET(flags, GA_EMBED_CHECK) && ga_lm_capturing(ctx))
+    return ga_err_set(ctx->err, GA_UNSUPPORTED_ERROR,
+                      "A checked call waits and cannot be captured into a graph");
+  return GA_NO_ERROR;
+}
+
+int GpuArray_embed(GpuArray *out, const GpuArray *table, const GpuArray *ids, double scale,
+                   ssize_t pad, int flags) {
+  gpucontext *ctx;
+  const ga_function *fn;
+  em_layout L;
+  ga_lead lead;
+  CUdeviceptr p_out, p_table, p_ids, p_err;
+  void *params[5];
+  unsigned grid[3] = {1, 1, 1}, block[3], e;
+  unsigned long long blocks;
+  int err;
+
+  if (out == NULL || out->data == NULL) return GA_INVALID_ERROR;
+  ctx = GpuArray_context(out);
+  if ((err = ga_lm_check(ctx, out, "out", 1)) != GA_NO_ERROR ||
+      (err = ga_lm_check(ctx, table, "table", 0)) != GA_NO_ERROR ||
+      (err = ga_lm_check(ctx, ids, "ids", 0)) != GA_NO_ERROR ||
+      (err = check_types(ctx, table, out, ids)) != GA_NO_ERROR ||
+      (err = check_shapes(ctx, out, "out", table, ids)) != GA_NO_ERROR ||
+      (err = check_call(ctx, table, flags, GA_EMBED_PAD | GA_EMBED_CHECK)) != GA_NO_ERROR)
+    return err;
+  e = vector_width(table, out, table->dimensions[1]);
+  err = fill(ctx, &L, &lead, out, table, ids, scale, pad, flags, e);
+  if (err != GA_NO_ERROR || L.n == 0 || L.nv == 0) return err;
+  err = ga_lm_kernel(ctx, "ga_embed",
+                     (uint64_t)table->typecode | (uint64_t)out->typecode << 8 |
+                         (uint64_t)ids->typecode << 16 | (uint64_t)e << 24 | (uint64_t)lead.nd << 32,
+                     emit, &fn);
+  if (err != GA_NO_ERROR) return err;
+  ga_lm_geometry(L.nv, block, &grid[1]);
+  blocks = (L.n + block[1] * 4 - 1) / (block[1] * 4);
+  if (blocks > 0x7fffffffULL || grid[1] > 65535)
+    return ga_err_set(ctx->err, GA_XLARGE_ERROR, "Too many tokens or too long rows for one call");
+  grid[0] = (unsigned)blocks;
+  p_out = out->data->ptr + out->offset;
+  p_table = table->data->ptr + table->offset;
+  p_ids = ids->data->ptr + ids->offset;
+  p_err = ISSET(flags, GA_EMBED_CHECK) ? ga_lm_err_word(ctx) : 0;
+  params[0] = &L;
+  params[1] = &p_out;
+  params[2] = &p_table;
+  params[3] = &p_ids;
+  params[4] = &p_err;
+  err = ga_launch(ctx, fn, grid, block, 0, params);
+  if (err == GA_NO_ERROR && ISSET(flags, GA_EMBED_CHECK))
+    err = ga_lm_err_take(ctx, "A token id is outside the table");
+  return err;
+}
+
+int GpuEmbedGrad_new(GpuEmbedGrad **eg, gpucontext *ctx) {
+  GpuEmbedGrad *r;
+  if (eg == NULL) return GA_INVALID_ERROR;
+  *eg = NULL;
+  if (ctx == NULL) return ga_err_set(ga_global_err, GA_INVALID_ERROR, "GpuEmbedGrad_new: no context");
+  r = calloc(1, sizeof(*r));
+  if (r == NULL) return ga_err_sys(ctx->err, "calloc");
+  r->ctx = ctx;
+  ctx->refcnt++;
+  *eg = r;
+  return GA_NO_ERROR;
+}
+
+void GpuEmbedGrad_free(GpuEmbedGrad *eg) {
+  gpucontext *ctx;
+  if (eg == NULL) return;
+  ctx = eg->ctx;
+  ga_workspace_free(&eg->ws);
+  free(eg);
+  ga_ctx_unref(ctx);
+}
+
+#define EG_STEP 8 /* tokens a group of threads loads at once: GA_EG_U of the template */
+
+int GpuEmbedGrad_call(GpuEmbedGrad *eg, GpuArray *dtable, const GpuArray *dout, const GpuArray *ids,
+                      double scale, ssize_t pad, int flags) {
+  gpucontext *ctx;
+  const ga_function *order, *sum, *join, *zero;
+  em_layout L;
+  ga_lead lead;
+  CUdeviceptr p_dt, p_do, p_ids, p_err, p_key, p_order, p_part;
+  void *params[6];
+  unsigned grid[3] = {1, 1, 1}, block[3], one[3] = {256, 1, 1}, g1[3] = {1, 1, 1}, e, ny;
+  unsigned long long groups, per_group;
+  size_t fsize, list;
+  uint64_t key;
+  int err, accumulate;
+
+  if (eg == NULL) return GA_INVALID_ERROR;
+  ctx = eg->ctx;
+  if ((err = ga_lm_check(ctx, dtable, "dtable", 1)) != GA_NO_ERROR ||
+      (err = ga_lm_check(ctx, dout, "dout", 0)) != GA_NO_ERROR ||
+      (err = ga_lm_check(ctx, ids, "ids", 0)) != GA_NO_ERROR ||
+      (err = check_types(ctx, dout, dtable, ids)) != GA_NO_ERROR ||
+      (err = check_shapes(ctx, dout, "dout", dtable, ids)) != GA_NO_ERROR ||
+      (err = check_call(ctx, dtable, flags, GA_EMBED_PAD | GA_EMBED_CHECK | GA_EMBED_ACCUMULATE)) !=
+          GA_NO_ERROR)
+    return err;
+  accumulate = ISSET(flags, GA_EMBED_ACCUMULATE);
+  e = vector_width(dout, dtable, dtable->dimensions[1]);
+  err = fill(ctx, &L, &lead, dout, dtable, ids, scale, pad, flags, e);
+  if (err != GA_NO_ERROR || L.nv == 0) return err;
+  if (L.n > 0x7fffffffULL)
+    return ga_err_set(ctx->err, GA_XLARGE_ERROR, "More than 2^31 - 1 tokens in one call");
+
+  key = (uint64_t)dout->typecode | (uint64_t)dtable->typecode << 8 | (uint64_t)ids->typecode << 16 |
+        (uint64_t)e << 24 | (uint64_t)lead.nd << 32 | (uint64_t)1 << 40 | (uint64_t)accumulate << 41;
+  if ((err = ga_lm_kernel(ctx, "ga_eg_order", key, emit, &order)) != GA_NO_ERROR ||
+      (err = ga_lm_kernel(ctx, "ga_eg_zero", key, emit, &zero)) != GA_NO_ERROR ||
+      (err = ga_lm_kernel(ctx, "ga_eg_sum", key, emit, &sum)) != GA_NO_ERROR ||
+      (err = ga_lm_kernel(ctx, "ga_eg_join", key, emit, &join)) != GA_NO_ERROR)
+    return err;
+
+  ga_lm_geometry(L.nv, block, &ny);
+  if (ny > 65535) return ga_err_set(ctx->err, GA_XLARGE_ERROR, "Too long rows for one call");
+  grid[1] = ny;
+  /* Chunks: enough groups to fill the device about twice, none shorter than one step. */
+  per_group = (unsigned long long)block[0] * ny;
+  groups = (unsigned long long)ctx->num_sms * 4096 / per_group;
+  if (groups == 0) groups = 1;
+  L.chunk = (unsigned)((L.n + groups - 1) / groups);
+  L.chunk = (L.chunk + EG_STEP - 1) / EG_STEP * EG_STEP;
+  if (L.chunk == 0) L.chunk = EG_STEP;
+  L.chunks = (unsigned)((L.n + L.chunk - 1) / L.chunk);
+
+  fsize = dout->typecode == GA_DOUBLE || dtable->typecode == GA_DOUBLE ? 8 : 4;
+  list = ((size_t)L.n * 4 + 511) / 512 * 512;
+  err = ga_workspace_need(ctx, &eg->ws, 2 * list + 2 * (size_t)L.chunks * L.nv * e * fsize);
+  if (err != GA_NO_ERROR) return err;
+
+  p_dt = dtable->data->ptr + dtable->offset;
+  p_do = dout->data->ptr + dout->offset;
+  p_ids = ids->data->ptr + ids->offset;
+  p_err = ISSET(flags, GA_EMBED_CHECK) ? ga_lm_err_word(ctx) : 0;
+  params[0] = &L;
+  params[1] = &p_dt;
+  if (!accumulate && L.v > 0) {
+    unsigned long long rows = (L.v + block[1] - 1) / block[1], most = (unsigned long long)ctx->num_sms * 16;
+    grid[0] = (unsigned)(rows > most ? most : rows);
+    err = ga_launch(ctx, zero, grid, block, 0, params);
+    if (err != GA_NO_ERROR) return err;
+  }
+  if (L.n == 0) return GA_NO_ERROR;
+  p_key = eg->ws.cur->ptr;
+  p_order = p_key + list;
+  p_part = p_order + list;
+
+  params[1] = &p_key;
+  params[2] = &p_order;
+  params[3] = &p_ids;
+  params[4] = &p_err;
+  g1[0] = (unsigned)((L.n + 7) / 8);
+  err = ga_launch(ctx, order, g1, one, 0, params);
+  if (err != GA_NO_ERROR) return err;
+
+  grid[0] = (L.chunks + block[1] - 1) / block[1];
+  params[1] = &p_dt;
+  params[2] = &p_do;
+  params[3] = &p_key;
+  params[4] = &p_order;
+  params[5] = &p_part;
+  err = ga_launch(ctx, sum, grid, block, 0, params);
+  if (err == GA_NO_ERROR && L.chunks > 1) {
+    params[2] = &p_key;
+    params[3] = &p_part;
+    err = ga_launch(ctx, join, grid, block, 0, params);
+  }
+  if (err == GA_NO_ERROR && ISSET(flags, GA_EMBED_CHECK))
+    err = ga_lm_err_take(ctx, "A token id is outside the table");
+  return err;
+}

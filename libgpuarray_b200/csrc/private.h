@@ -11,6 +11,10 @@
  *   ga_array.c     GpuArray bookkeeping and copies
  *   ga_elemwise.c  elementwise engine
  *   ga_reduction.c reduction engine
+ *   ga_lm.c        helpers of the language-model operators
+ *   ga_embed.c     token embedding and its gradient
+ *   ga_logprobs.c  log probabilities, entropy, alternatives, their gradient
+ *   ga_clipnorm.c  norm over a list of arrays, clipping
  *   ga_comm.c      NCCL collectives
  */
 #ifndef GA_B200_PRIVATE_H
@@ -34,6 +38,9 @@
 #include <gpuarray/kernel.h>
 #include <gpuarray/elemwise.h>
 #include <gpuarray/reduction.h>
+#include <gpuarray/embedding.h>
+#include <gpuarray/logprobs.h>
+#include <gpuarray/clipnorm.h>
 #include <gpuarray/extension.h>
 #include <gpuarray/buffer_collectives.h>
 #include <gpuarray/collectives.h>
@@ -180,6 +187,7 @@ struct _gpucontext {
   /* lazily created MAXANDARGMAX operators keyed by source type (ga_reduction.c) */
   void *maxandargmax_cache;
   void *take1_cache;        /* compiled gather kernels by (types, rank): ga_array.c */
+  void *lm_cache;           /* compiled language-model kernels by variant: ga_lm.c */
   void *peer_windows;       /* exported windows of freed communicators, for reuse: ga_comm.c */
 };
 
@@ -255,6 +263,55 @@ GA_HIDDEN void ga_extcopy_cache_free(gpucontext *ctx);
 GA_HIDDEN void ga_maxandargmax_cache_free(gpucontext *ctx);
 GA_HIDDEN void ga_take1_cache_free(gpucontext *ctx);
 GA_HIDDEN void ga_peer_windows_free(gpucontext *ctx);
+
+/* ---------------------------------------- language-model operators (ga_lm.c) */
+
+#define GA_LM_MAXD 4 /* leading dimensions a kernel can walk; the templates have the same constant */
+
+/* The dimensions before the last of some arrays, collapsed together. */
+typedef struct ga_lead {
+  unsigned int nd;               /* 1 .. GA_LM_MAXD */
+  unsigned long long count;      /* product */
+  unsigned long long dims[GA_LM_MAXD];
+} ga_lead;
+
+/* Collapses nd dimensions shared by n arrays: str[k] are array k's strides (NULL: no such
+ * array), out[k] receives those left. GA_UNSUPPORTED_ERROR when too many are left. */
+GA_HIDDEN int ga_lm_lead(gpucontext *ctx, unsigned int nd, const size_t *dims, unsigned int n,
+                         const ssize_t *const *str, ga_lead *lead, long long (*out)[GA_LM_MAXD]);
+/* Context, alignment, bounds (and for a destination: writeable, no two elements in one place). */
+GA_HIDDEN int ga_lm_check(gpucontext *ctx, const GpuArray *a, const char *what, int dest);
+GA_HIDDEN int ga_lm_is_id(int typecode);
+/* a and b have the same extents in their first nd dimensions */
+GA_HIDDEN int ga_lm_same_dims(const GpuArray *a, const GpuArray *b, unsigned int nd);
+/* 1 while the context's stream is being captured into a graph */
+GA_HIDDEN int ga_lm_capturing(gpucontext *ctx);
+
+/* The kernel `fname` of a variant: `emit` writes its source for `key` the first time. The
+ * pointer stays valid as long as the context. */
+GA_HIDDEN int ga_lm_kernel(gpucontext *ctx, const char *fname, uint64_t key,
+                           void (*emit)(ga_strb *sb, uint64_t key), const ga_function **fn);
+GA_HIDDEN void ga_lm_cache_free(gpucontext *ctx);
+
+/* Device memory of an operator. It only grows, and what it had before is kept until it is
+ * freed: a captured graph may still refer to it. */
+typedef struct ga_workspace {
+  gpudata *cur;
+  size_t sz;
+  gpudata **old;
+  unsigned int nold;
+} ga_workspace;
+GA_HIDDEN int ga_workspace_need(gpucontext *ctx, ga_workspace *ws, size_t bytes);
+GA_HIDDEN void ga_workspace_free(ga_workspace *ws);
+
+/* The word of the context's error buffer in which the language-model kernels report an id out
+ * of range (the first word is GpuArray_take1's). */
+GA_HIDDEN CUdeviceptr ga_lm_err_word(gpucontext *ctx);
+/* Waits for the stream; GA_VALUE_ERROR (and the word back at zero) if it was set. */
+GA_HIDDEN int ga_lm_err_take(gpucontext *ctx, const char *what);
+/* Threads along vectors and rows of a block for rows of nv vectors: 256 threads, whole warps
+ * along the vectors where there are that many; *ny blocks cover the row. */
+GA_HIDDEN void ga_lm_geometry(unsigned long long nv, unsigned block[3], unsigned int *ny);
 
 /* Combination of per-GPU partial results through peer memory (ga_comm.c). */
 struct _gpucomm;

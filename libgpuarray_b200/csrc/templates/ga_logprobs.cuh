@@ -1,0 +1,688 @@
+/* Log probabilities of given tokens, entropy and the most likely alternatives
+ * of rows of logits, and the gradient of the first two.
+ *
+ * With x_j = scale * z_j, m = max z, S = sum_j e^(x_j - scale m):
+ *   logp    = scale (z_t - m) - ln S
+ *   entropy = ln S - (1/S) sum_j e^(x_j - scale m) (x_j - scale m)
+ *   dz_j    = scale (a (1[j = t] - p_j) - b p_j (ln p_j + entropy)),
+ *             p_j = e^(x_j - scale m - ln S), a and b the gradients arriving
+ *             at logp and entropy.
+ * One pass over a row keeps (m, S, T = sum e y) with y in powers of two and
+ * rescales S and T when m grows (Milakov and Gimelshein, online softmax).
+ * Differences to m are taken before the scale is applied, so that logits of
+ * the type's lowest value, and rows of nothing else, stay finite.
+ *   a row without a logit above -inf: logp and alternatives -inf, entropy 0,
+ *     gradient 0;   a row with a NaN or +inf: NaN everywhere.
+ *
+ * Defines needed: GA_LP_BUILD_ROWS or GA_LP_BUILD_GRAD, GA_LP_Z_T (logits),
+ * GA_LP_ZTYPE (0 half, 1 float), GA_LP_G_T and GA_LP_GTYPE (dlogits),
+ * GA_LP_I_T (token ids), GA_LP_ND (leading dimensions), GA_LP_CONTIG (elements
+ * of a row adjacent), GA_LP_ENT (entropy wanted), and for the rows kernel
+ * GA_LP_THREADS, GA_LP_GROUP (threads per row: 32 or GA_LP_THREADS),
+ * GA_LP_CLUSTER (CTAs per row), GA_LP_TOP (alternatives wanted). */
+#include "ga_lm_common.cuh"
+
+#define GA_LP_LOG2E 1.4426950408889634f
+#define GA_LP_LN2 0.6931471805599453f
+
+struct ga__lp_layout {
+  unsigned long long rows;
+  unsigned int v;   /* logits in a row, < 2^31 */
+  unsigned int top; /* alternatives */
+  float scale;
+  int has_ignore;
+  long long ignore;
+  unsigned long long dims[GA_LM_MAXD];
+  long long z_str[GA_LM_MAXD], t_str[GA_LM_MAXD];
+  long long z_col;
+  /* rows kernel: logp, entropy, stats, top values, top ids; gradient: stats, dlogp, entropy,
+   * dentropy, dlogits */
+  long long o_str[5][GA_LM_MAXD];
+  long long o_col[5];
+};
+
+#if GA_LP_CONTIG
+#define GA_LP_E (16 / (int)sizeof(GA_LP_Z_T))
+#else
+#define GA_LP_E 1
+#endif
+
+/* A row as vectors of GA_LP_E elements at 16-byte boundaries: vector w holds elements
+ * w * E - skip ... of the row, of which those below 0 and beyond v are not there. */
+struct ga__lp_row {
+  const char *z;
+  const char *base;
+  unsigned int skip, nv;
+};
+
+static __device__ __forceinline__ ga__lp_row ga__lp_open(const ga__lp_layout &L, const char *logits,
+                                                         unsigned long long row) {
+  ga__lp_row r;
+  r.z = logits + ga__lm_offset<GA_LP_ND>(row, L.dims, L.z_str);
+#if GA_LP_CONTIG
+  const unsigned int off = (unsigned int)((size_t)r.z & 15);
+  r.base = r.z - off;
+  r.skip = off / (unsigned int)sizeof(GA_LP_Z_T);
+#else
+  r.base = r.z;
+  r.skip = 0;
+#endif
+  r.nv = (L.v + r.skip + GA_LP_E - 1) / GA_LP_E;
+  return r;
+}
+
+/* one vector as 32-bit words (two halves or one float each) */
+#if GA_LP_ZTYPE == 0
+#define GA_LP_W ((GA_LP_E + 1) / 2)
+#else
+#define GA_LP_W GA_LP_E
+#endif
+struct alignas(GA_LP_CONTIG ? 16 : 4) ga__lp_words {
+  unsigned int w[GA_LP_W];
+};
+#if GA_LP_ZTYPE == 0
+#define GA_LP_MINUS_INF 0xfc00u
+#else
+#define GA_LP_MINUS_INF 0xff800000u
+#endif
+
+/* The elements that are not there read as -inf, which changes neither m nor S nor T. */
+static __device__ __forceinline__ ga__lp_words ga__lp_load_part(const ga__lp_layout &L,
+                                                                const ga__lp_row &r, unsigned int w) {
+  ga__lp_words q;
+#pragma unroll
+  for (int j = 0; j < GA_LP_W; j++)
+    q.w[j] = GA_LP_ZTYPE == 0 ? (GA_LP_MINUS_INF | GA_LP_MINUS_INF << 16) : GA_LP_MINUS_INF;
+#pragma unroll
+  for (int j = 0; j < GA_LP_E; j++) {
+    const unsigned int i = w * GA_LP_E + j - r.skip; /* wraps below the row's start */
+    if (i < L.v) {
+#if GA_LP_ZTYPE == 0
+      const unsigned int h = *reinterpret_cast<const unsigned short *>(r.z + (long long)i * L.z_col);
+      q.w[j / 2] = (j & 1) ? (q.w[j / 2] & 0xffffu) | (h << 16) : (q.w[j / 2] & 0xffff0000u) | h;
+#else
+      q.w[j] = *reinterpret_cast<const unsigned int *>(r.z + (long long)i * L.z_col);
+#endif
+    }
+  }
+  return q;
+}
+
+static __device__ __forceinline__ int ga__lp_whole(const ga__lp_layout &L, const ga__lp_row &r,
+                                                   unsigned int w) {
+  return GA_LP_CONTIG && w * GA_LP_E >= r.skip && (w + 1) * GA_LP_E - r.skip <= L.v;
+}
+
+static __device__ __forceinline__ ga__lp_words ga__lp_load(const ga__lp_layout &L, const ga__lp_row &r,
+                                                           unsigned int w) {
+  if (ga__lp_whole(L, r, w))
+    return *reinterpret_cast<const ga__lp_words *>(r.base + (size_t)w * 16);
+  return ga__lp_load_part(L, r, w);
+}
+
+static __device__ __forceinline__ float ga__lp_z(const char *p) {
+#if GA_LP_ZTYPE == 0
+  return ga_half2float(*reinterpret_cast<const ga_half *>(p));
+#else
+  return *reinterpret_cast<const float *>(p);
+#endif
+}
+
+/* pair k of the vector as two floats (the second -inf where a vector has one element) */
+#define GA_LP_PAIRS ((GA_LP_E + 1) / 2)
+static __device__ __forceinline__ void ga__lp_pair(const ga__lp_words &q, int k, float &a, float &b) {
+#if GA_LP_ZTYPE == 0
+  ga__unpack_h2(q.w[k], a, b);
+#else
+  a = __uint_as_float(q.w[2 * k]);
+  b = 2 * k + 1 < GA_LP_W ? __uint_as_float(q.w[2 * k + 1 < GA_LP_W ? 2 * k + 1 : 0])
+                          : __uint_as_float(0xff800000u);
+#endif
+}
+
+#ifdef GA_LP_BUILD_ROWS
+#define GA_LP_U 4
+#define GA_LP_CAND 512
+/* below every logit that is not -inf: the maximum of nothing (a half is never so low; a float
+ * logit of exactly this value gives the right S all the same) */
+#define GA_LP_NOTHING -3.402823466e38f
+/* 2^y is 0 from here on; keeps 0 * y finite */
+#define GA_LP_YMIN -200.0f
+
+struct ga__lp_state {
+  float m, s, t;
+};
+
+static __device__ __forceinline__ ga__lp_state ga__lp_merge(ga__lp_state a, ga__lp_state b, float c) {
+  ga__lp_state r;
+  r.m = fmaxf(a.m, b.m);
+  const float da = ga__max_nan((a.m - r.m) * c, GA_LP_YMIN), db = ga__max_nan((b.m - r.m) * c, GA_LP_YMIN);
+  const float fa = ga__ex2(da), fb = ga__ex2(db);
+  r.s = a.s * fa + b.s * fb;
+  r.t = (a.t + a.s * da) * fa + (b.t + b.s * db) * fb;
+  return r;
+}
+
+static __device__ __forceinline__ float ga__lp_max(const ga__lp_words &q) {
+#if GA_LP_ZTYPE == 0
+  unsigned int h = q.w[0];
+#pragma unroll
+  for (int j = 1; j < GA_LP_W; j++) h = ga__max_h2(h, q.w[j]);
+  float a, b;
+  ga__unpack_h2(h, a, b);
+  return fmaxf(a, b);
+#else
+  float a = __uint_as_float(q.w[0]);
+#pragma unroll
+  for (int j = 1; j < GA_LP_W; j++) a = fmaxf(a, __uint_as_float(q.w[j]));
+  return a;
+#endif
+}
+
+#if GA_LP_TOP
+/* Orders by value, NaN lowest, and among equal values the lower index higher; 0 is no element. */
+static __device__ __forceinline__ unsigned long long ga__lp_key(float z, unsigned int i) {
+  unsigned int b = __float_as_uint(z + 0.0f); /* -0 and +0 are one value */
+  b = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+  if (z != z) b = 0;
+  return ((unsigned long long)b << 32) | (0xffffffffu - i);
+}
+static __device__ __forceinline__ float ga__lp_key_value(unsigned long long k) {
+  const unsigned int b = (unsigned int)(k >> 32);
+  if (b == 0) return __uint_as_float(0x7fffffffu);
+  return __uint_as_float((b & 0x80000000u) ? (b & 0x7fffffffu) : ~b);
+}
+
+/* keys of the vector's elements that are there; absent ones 0 */
+static __device__ __forceinline__ void ga__lp_keys(const ga__lp_layout &L, const ga__lp_row &r,
+                                                   unsigned int w, unsigned long long k[2 * GA_LP_PAIRS]) {
+  const ga__lp_words q = ga__lp_load(L, r, w);
+#pragma unroll
+  for (int p = 0; p < GA_LP_PAIRS; p++) {
+    float z[2];
+    ga__lp_pair(q, p, z[0], z[1]);
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const unsigned int i = w * GA_LP_E + 2 * p + h - r.skip;
+      k[2 * p + h] = (2 * p + h < GA_LP_E && i < L.v) ? ga__lp_key(z[h], i) : 0;
+    }
+  }
+}
+
+struct ga__lp_top_smem {
+  unsigned long long cand[GA_LP_CAND];
+  unsigned long long best[GA_LP_THREADS];
+  unsigned long long out[GA_LP_CLUSTER * 32]; /* the CTAs' lists, in the first CTA of a cluster */
+  unsigned long long tau;
+  unsigned int list[GA_LP_THREADS];
+  unsigned int nlist, ncand;
+  unsigned int count;
+};
+
+/* The `top` largest keys of vectors [v0, v1) of the row, into out[0..32) of this CTA's or the
+ * cluster's first CTA's shared memory (0 where there are fewer). All threads of the CTA.
+ *
+ * `first` is the vector in which this thread's first largest element lies. The thread's largest
+ * key bounds its others, so the top-th largest of the threads' largest keys, tau, is a lower
+ * bound for the top-th largest of all, and every key above it belongs to one of the `top`
+ * threads that reach it: only their vectors are read again. Where NaNs made `first` unusable, or
+ * the keys above tau are too many to hold (a row that hides its largest elements in few threads'
+ * vectors), tau is found by halving over the whole row. */
+static __device__ void ga__lp_top(const ga__lp_layout &L, const ga__lp_row &r, unsigned int v0,
+                                  unsigned int v1, unsigned int first, int odd, ga__lp_top_smem &S) {
+  const unsigned int tid = threadIdx.x;
+  unsigned long long k[2 * GA_LP_PAIRS], mine = 0;
+  if (v0 + tid < v1) {
+    ga__lp_keys(L, r, first, k);
+#pragma unroll
+    for (int j = 0; j < 2 * GA_LP_PAIRS; j++) mine = k[j] > mine ? k[j] : mine;
+  }
+  S.best[tid] = mine;
+  if (tid == 0) {
+    S.nlist = 0;
+    S.ncand = 0;
+  }
+  __syncthreads();
+  if (tid < 32) {
+    unsigned long long b[GA_LP_THREADS / 32], lo = 0, hi = 0, low;
+#pragma unroll
+    for (int j = 0; j < GA_LP_THREADS / 32; j++) {
+      b[j] = S.best[j * 32 + tid];
+      lo = b[j] > lo ? b[j] : lo;
+    }
+    hi = low = lo;
+#pragma unroll
+    for (int d = 16; d > 0; d /= 2) { /* the lanes' largest: 32 keys, all at least `lo` */
+      const unsigned long long h = __shfl_xor_sync(0xffffffffu, hi, d), l = __shfl_xor_sync(0xffffffffu, low, d);
+      hi = h > hi ? h : hi;
+      low = l < low ? l : low;
+    }
+    lo = low;
+    hi = hi + 1;
+    /* at least `top` keys reach lo (or all there are, where a lane has none), fewer reach hi; keys
+     * differ, so halving ends with exactly `top` of them */
+    unsigned int at_lo = 0;
+    if (lo == 0) lo = 1;
+#pragma unroll
+    for (int j = 0; j < GA_LP_THREADS / 32; j++) at_lo += b[j] >= lo;
+    at_lo = ga__warp_sum_u32(at_lo);
+    while (at_lo > L.top && hi - lo > 1) {
+      const unsigned long long mid = lo + (hi - lo) / 2;
+      unsigned int c = 0;
+#pragma unroll
+      for (int j = 0; j < GA_LP_THREADS / 32; j++) c += b[j] >= mid;
+      c = ga__warp_sum_u32(c);
+      if (c >= L.top) {
+        lo = mid;
+        at_lo = c;
+      } else {
+        hi = mid;
+      }
+    }
+    if (tid == 0) S.tau = lo;
+  }
+  __syncthreads();
+  unsigned long long tau = S.tau;
+  if (!odd && mine >= tau) S.list[atomicAdd(&S.nlist, 1u)] = tid;
+  __syncthreads();
+  const unsigned int per = (v1 - v0 + GA_LP_THREADS - 1) / GA_LP_THREADS;
+  const unsigned int items = S.nlist * per;
+  for (unsigned int it = tid; it < items; it += GA_LP_THREADS) {
+    const unsigned int w = v0 + S.list[it / per] + (it % per) * GA_LP_THREADS;
+    if (w >= v1) continue;
+    ga__lp_keys(L, r, w, k);
+#pragma unroll
+    for (int j = 0; j < 2 * GA_LP_PAIRS; j++)
+      if (k[j] >= tau) {
+        const unsigned int at = atomicAdd(&S.ncand, 1u);
+        if (at < GA_LP_CAND) S.cand[at] = k[j];
+      }
+  }
+  __syncthreads();
+  if (odd || S.ncand > GA_LP_CAND) { /* the same in every thread */
+    unsigned long long lo = 1, hi = ~0ULL; /* above every key: the largest value, inf, has 0xff800000 */
+    for (int step = 0; step < 66; step++) {
+      const unsigned long long mid = step == 0 ? 1 : lo + (hi - lo) / 2;
+      unsigned int c = 0;
+      __syncthreads();
+      if (tid == 0) S.count = 0;
+      __syncthreads();
+      for (unsigned int w = v0 + tid; w < v1; w += GA_LP_THREADS) {
+        ga__lp_keys(L, r, w, k);
+#pragma unroll
+        for (int j = 0; j < 2 * GA_LP_PAIRS; j++) c += k[j] >= mid;
+      }
+      c = ga__warp_sum_u32(c);
+      if (tid % 32 == 0) atomicAdd(&S.count, c);
+      __syncthreads();
+      c = S.count;
+      if (c >= L.top || step == 0) lo = mid;
+      else hi = mid;
+      if (c <= GA_LP_CAND && (c >= L.top || step == 0)) break;
+    }
+    tau = lo;
+    if (tid == 0) S.ncand = 0;
+    __syncthreads();
+    for (unsigned int w = v0 + tid; w < v1; w += GA_LP_THREADS) {
+      ga__lp_keys(L, r, w, k);
+#pragma unroll
+      for (int j = 0; j < 2 * GA_LP_PAIRS; j++)
+        if (k[j] >= tau) {
+          const unsigned int at = atomicAdd(&S.ncand, 1u);
+          if (at < GA_LP_CAND) S.cand[at] = k[j];
+        }
+    }
+    __syncthreads();
+  }
+  /* a key's place is the number of larger ones */
+  const unsigned int n = S.ncand < GA_LP_CAND ? S.ncand : GA_LP_CAND;
+#if GA_LP_CLUSTER > 1
+  const unsigned int slot = ga__cluster_rank() * 32;
+  for (unsigned int i = tid + n; i < L.top; i += GA_LP_THREADS) ga__cluster_put(&S.out[slot + i], 0, 0);
+#else
+  for (unsigned int i = tid + n; i < L.top; i += GA_LP_THREADS) S.out[i] = 0;
+#endif
+  for (unsigned int i = tid; i < n; i += GA_LP_THREADS) {
+    const unsigned long long key = S.cand[i];
+    unsigned int place = 0;
+    for (unsigned int j = 0; j < n; j++) place += S.cand[j] > key;
+    if (place < L.top) {
+#if GA_LP_CLUSTER > 1
+      ga__cluster_put(&S.out[slot + place], 0, key);
+#else
+      S.out[place] = key;
+#endif
+    }
+  }
+}
+#endif
+
+extern "C" __global__ void __launch_bounds__(GA_LP_THREADS)
+#if GA_LP_CLUSTER > 1
+    __cluster_dims__(GA_LP_CLUSTER, 1, 1)
+#endif
+ga_lp_rows(const __grid_constant__ ga__lp_layout L, const char *logits, const char *targets,
+           char *logp, char *entropy, char *stats, char *topv, char *topi, int *err) {
+  ga__grid_dependency_sync();
+  const unsigned int lane = threadIdx.x % GA_LP_GROUP;
+#if GA_LP_CLUSTER > 1
+  const unsigned long long row = blockIdx.x / GA_LP_CLUSTER;
+  const unsigned int part = ga__cluster_rank();
+#else
+  const unsigned long long row =
+      (unsigned long long)blockIdx.x * (GA_LP_THREADS / GA_LP_GROUP) + threadIdx.x / GA_LP_GROUP;
+  const unsigned int part = 0;
+#if GA_LP_GROUP < GA_LP_THREADS
+  if (row >= L.rows) return; /* a whole warp; nothing below waits for another */
+#endif
+#endif
+#if GA_LP_CLUSTER > 1
+  ga__cluster_arrive(); /* waited for before the first store to another CTA's shared memory */
+#endif
+  const ga__lp_row r = ga__lp_open(L, logits, row);
+  const unsigned int share = (r.nv + GA_LP_CLUSTER - 1) / GA_LP_CLUSTER;
+  const unsigned int v0 = part * share < r.nv ? part * share : r.nv;
+  const unsigned int v1 = r.nv - v0 < share ? r.nv : v0 + share;
+  const float c = L.scale * GA_LP_LOG2E;
+
+  /* the target's logit is fetched while the row streams */
+  long long target = -1;
+  float zt = 0;
+  if (lane == 0 && part == 0 && logp != nullptr) {
+    target = (long long)*reinterpret_cast<const GA_LP_I_T *>(
+        targets + ga__lm_offset<GA_LP_ND>(row, L.dims, L.t_str));
+    if (target >= 0 && target < (long long)L.v) zt = ga__lp_z(r.z + target * L.z_col);
+  }
+
+  ga__lp_state st = {GA_LP_NOTHING, 0.0f, 0.0f};
+  ga__f2 s2 = ga__f2_of(0.0f, 0.0f), t2 = s2;
+  const ga__f2 c2 = ga__f2_of(c, c);
+#if GA_LP_TOP
+  unsigned int first = v0 + lane; /* the vector of this thread's first largest element */
+  float best = __uint_as_float(0xff800000u);
+#endif
+  for (unsigned int w = v0 + lane; w < v1; w += GA_LP_GROUP * GA_LP_U) {
+    ga__lp_words q[GA_LP_U];
+    float vm[GA_LP_U], top = __uint_as_float(0xff800000u);
+    if (GA_LP_CONTIG && w > 0 && w + (GA_LP_U - 1) * GA_LP_GROUP < v1 &&
+        w + (GA_LP_U - 1) * GA_LP_GROUP + 1 < r.nv) { /* neither the row's first nor its last vector */
+#pragma unroll
+      for (int u = 0; u < GA_LP_U; u++)
+        q[u] = *reinterpret_cast<const ga__lp_words *>(r.base + (size_t)(w + u * GA_LP_GROUP) * 16);
+    } else {
+#pragma unroll
+      for (int u = 0; u < GA_LP_U; u++) {
+        if (w + u * GA_LP_GROUP < v1) q[u] = ga__lp_load(L, r, w + u * GA_LP_GROUP);
+        else {
+#pragma unroll
+          for (int j = 0; j < GA_LP_W; j++)
+            q[u].w[j] = GA_LP_ZTYPE == 0 ? (GA_LP_MINUS_INF | GA_LP_MINUS_INF << 16) : GA_LP_MINUS_INF;
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < GA_LP_U; u++) {
+      vm[u] = ga__lp_max(q[u]);
+      top = fmaxf(top, vm[u]);
+    }
+#if GA_LP_TOP
+    if (top > best) {
+#pragma unroll
+      for (int u = GA_LP_U - 1; u >= 0; u--)
+        if (vm[u] == top) first = w + u * GA_LP_GROUP;
+      best = top;
+    }
+#endif
+    if (top > st.m) {
+      const float d = ga__max_nan((st.m - top) * c, GA_LP_YMIN), f = ga__ex2(d);
+      const ga__f2 f2 = ga__f2_of(f, f);
+#if GA_LP_ENT
+      t2 = ga__f2_mul(ga__f2_fma(s2, ga__f2_of(d, d), t2), f2);
+#endif
+      s2 = ga__f2_mul(s2, f2);
+      st.m = top;
+    }
+    const ga__f2 nm2 = ga__f2_of(-st.m, -st.m);
+#pragma unroll
+    for (int u = 0; u < GA_LP_U; u++)
+#pragma unroll
+      for (int k = 0; k < GA_LP_PAIRS; k++) {
+        float a, b;
+        ga__lp_pair(q[u], k, a, b);
+        ga__f2_to(ga__f2_mul(ga__f2_add(ga__f2_of(a, b), nm2), c2), a, b);
+        a = ga__max_nan(a, GA_LP_YMIN);
+        b = ga__max_nan(b, GA_LP_YMIN);
+        const ga__f2 e2 = ga__f2_of(ga__ex2(a), ga__ex2(b));
+        s2 = ga__f2_add(s2, e2);
+#if GA_LP_ENT
+        t2 = ga__f2_fma(e2, ga__f2_of(a, b), t2);
+#endif
+      }
+  }
+  {
+    float a, b;
+    ga__f2_to(s2, a, b);
+    st.s = a + b;
+    ga__f2_to(t2, a, b);
+    st.t = a + b;
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d /= 2) {
+    ga__lp_state o;
+    o.m = __shfl_xor_sync(0xffffffffu, st.m, d);
+    o.s = __shfl_xor_sync(0xffffffffu, st.s, d);
+    o.t = __shfl_xor_sync(0xffffffffu, st.t, d);
+    st = ga__lp_merge(st, o, c);
+  }
+#if GA_LP_GROUP > 32
+  __shared__ ga__lp_state warps[GA_LP_THREADS / 32];
+  if (threadIdx.x % 32 == 0) warps[threadIdx.x / 32] = st;
+  __syncthreads();
+  /* every thread merges the warps' states in the same order: the same bits everywhere */
+  st = warps[0];
+#pragma unroll 1
+  for (int i = 1; i < GA_LP_THREADS / 32; i++) st = ga__lp_merge(st, warps[i], c);
+#endif
+#if GA_LP_CLUSTER > 1
+  ga__cluster_wait(); /* every CTA of the cluster runs */
+#endif
+#if GA_LP_TOP
+  __shared__ ga__lp_top_smem tops;
+  ga__lp_top(L, r, v0, v1, first, !(st.s == st.s), tops);
+#endif
+#if GA_LP_CLUSTER > 1
+  /* the CTAs' states and lists meet in the first one */
+  __shared__ unsigned long long parts[GA_LP_CLUSTER][2];
+  if (threadIdx.x == 0) {
+    ga__cluster_put(&parts[part][0], 0, (unsigned long long)__float_as_uint(st.m) << 32 | __float_as_uint(st.s));
+    ga__cluster_put(&parts[part][1], 0, (unsigned long long)__float_as_uint(st.t));
+  }
+  ga__cluster_arrive();
+  ga__cluster_wait();
+  if (part != 0) return;
+#pragma unroll 1
+  for (int i = 0; i < GA_LP_CLUSTER; i++) {
+    ga__lp_state o;
+    o.m = __uint_as_float((unsigned int)(parts[i][0] >> 32));
+    o.s = __uint_as_float((unsigned int)parts[i][0]);
+    o.t = __uint_as_float((unsigned int)parts[i][1]);
+    st = i == 0 ? o : ga__lp_merge(st, o, c);
+  }
+#endif
+  const int empty = st.s == 0.0f;
+  const float ls = logf(st.s);
+  const float minus_inf = __uint_as_float(0xff800000u);
+  if (lane == 0) {
+    if (logp != nullptr) {
+      float p;
+      if (L.has_ignore && target == L.ignore) p = 0.0f;
+      else if (target < 0 || target >= (long long)L.v) {
+        p = __uint_as_float(0x7fffffffu);
+        if (err != nullptr) *err = -1;
+      } else p = empty ? minus_inf : (zt - st.m) * L.scale - ls;
+      *reinterpret_cast<float *>(logp + ga__lm_offset<GA_LP_ND>(row, L.dims, L.o_str[0])) = p;
+    }
+#if GA_LP_ENT
+    if (entropy != nullptr) {
+      const float h = ls - GA_LP_LN2 * (st.t / st.s);
+      *reinterpret_cast<float *>(entropy + ga__lm_offset<GA_LP_ND>(row, L.dims, L.o_str[1])) =
+          empty || h < 0.0f ? 0.0f : h;
+    }
+#endif
+    if (stats != nullptr) {
+      char *p = stats + ga__lm_offset<GA_LP_ND>(row, L.dims, L.o_str[2]);
+      *reinterpret_cast<float *>(p) = empty ? minus_inf : st.m;
+      *reinterpret_cast<float *>(p + L.o_col[2]) = ls;
+    }
+  }
+#if GA_LP_TOP
+#if GA_LP_CLUSTER > 1
+  const unsigned int n = GA_LP_CLUSTER * 32;
+#else
+  __syncthreads();
+  const unsigned int n = L.top;
+#endif
+  for (unsigned int i = threadIdx.x; i < n; i += GA_LP_THREADS) {
+#if GA_LP_CLUSTER > 1
+    if (i % 32 >= L.top) continue;
+#endif
+    const unsigned long long key = tops.out[i];
+    if (key == 0) continue;
+    unsigned int place = i;
+#if GA_LP_CLUSTER > 1
+    place = 0;
+    for (unsigned int j = 0; j < n; j++)
+      if (j % 32 < L.top) place += tops.out[j] > key;
+    if (place >= L.top) continue;
+#endif
+    if (topv != nullptr)
+      *reinterpret_cast<float *>(topv + ga__lm_offset<GA_LP_ND>(row, L.dims, L.o_str[3]) +
+                                 place * L.o_col[3]) =
+          empty ? minus_inf : (ga__lp_key_value(key) - st.m) * L.scale - ls;
+    if (topi != nullptr)
+      *reinterpret_cast<GA_LP_I_T *>(topi + ga__lm_offset<GA_LP_ND>(row, L.dims, L.o_str[4]) +
+                                     place * L.o_col[4]) =
+          (GA_LP_I_T)(0xffffffffu - (unsigned int)key);
+  }
+#endif
+}
+#endif
+
+#ifdef GA_LP_BUILD_GRAD
+#define GA_LP_U 4
+
+static __device__ __forceinline__ void ga__lp_store(char *g, long long col, unsigned int i,
+                                                    unsigned int n, const float x[2 * GA_LP_PAIRS],
+                                                    int whole) {
+  /* elements i ... of the row (a whole vector, or those of it that are there) */
+  typedef ga__lm_vec<GA_LP_G_T, GA_LP_E> vec;
+  if (whole && col == (long long)sizeof(GA_LP_G_T) &&
+      ((size_t)(g + (long long)i * col) & (alignof(vec) - 1)) == 0) {
+    vec q;
+#if GA_LP_GTYPE == 0
+    unsigned int w[GA_LP_PAIRS];
+#pragma unroll
+    for (int k = 0; k < GA_LP_PAIRS; k++) w[k] = ga__pack_h2(x[2 * k], x[2 * k + 1]);
+    memcpy(&q, w, sizeof(q));
+#else
+#pragma unroll
+    for (int j = 0; j < GA_LP_E; j++) q.v[j] = x[j];
+#endif
+    *reinterpret_cast<vec *>(g + (long long)i * col) = q;
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < GA_LP_E; j++)
+    if (i + j < n) ga__lm_put(reinterpret_cast<GA_LP_G_T *>(g + (long long)(i + j) * col), x[j]);
+}
+
+/* A thread owns up to GA_LP_U vectors of a row; the row's numbers come from the forward pass, so
+ * that the logits are read once and the gradient written once. dlogits may be the logits. */
+extern "C" __global__ void __launch_bounds__(256)
+ga_lp_grad(const __grid_constant__ ga__lp_layout L, char *dlogits, const char *logits,
+           const char *targets, const char *stats, const char *dlogp, const char *entropy,
+           const char *dentropy, int *err) {
+  ga__grid_dependency_sync();
+  const unsigned long long row = (unsigned long long)blockIdx.x * blockDim.y + threadIdx.y;
+  if (row >= L.rows) return;
+  const ga__lp_row r = ga__lp_open(L, logits, row);
+  const unsigned int w0 = blockIdx.y * blockDim.x * GA_LP_U + threadIdx.x;
+  if (w0 >= r.nv) return;
+  char *g = dlogits + ga__lm_offset<GA_LP_ND>(row, L.dims, L.o_str[4]);
+
+  long long target = (long long)*reinterpret_cast<const GA_LP_I_T *>(
+      targets + ga__lm_offset<GA_LP_ND>(row, L.dims, L.t_str));
+  const char *sp = stats + ga__lm_offset<GA_LP_ND>(row, L.dims, L.o_str[0]);
+  const float m = *reinterpret_cast<const float *>(sp);
+  const float ls = *reinterpret_cast<const float *>(sp + L.o_col[0]);
+  float a = *reinterpret_cast<const float *>(dlogp + ga__lm_offset<GA_LP_ND>(row, L.dims, L.o_str[1]));
+  int none = 0;
+  if (L.has_ignore && target == L.ignore) {
+    a = 0.0f;
+    target = -1;
+    none = !GA_LP_ENT;
+  } else if (target < 0 || target >= (long long)L.v) {
+    a = __uint_as_float(0x7fffffffu);
+    if (w0 == 0 && err != nullptr) *err = -1;
+  }
+  if (m == __uint_as_float(0xff800000u)) none = 1; /* nothing above -inf in the row */
+  const float c = L.scale * GA_LP_LOG2E;
+  /* dz = e^(...) (w0 + w1 y) with y = log2 p, plus scale a at the target */
+  float k0 = -L.scale * a, k1 = 0.0f;
+#if GA_LP_ENT
+  {
+    const float b = *reinterpret_cast<const float *>(dentropy + ga__lm_offset<GA_LP_ND>(row, L.dims, L.o_str[3]));
+    const float h = *reinterpret_cast<const float *>(entropy + ga__lm_offset<GA_LP_ND>(row, L.dims, L.o_str[2]));
+    k0 -= L.scale * b * h;
+    k1 = -L.scale * b * GA_LP_LN2;
+  }
+#endif
+  const ga__f2 nm2 = ga__f2_of(-m, -m), c2 = ga__f2_of(c, c);
+  const float l2 = -ls * GA_LP_LOG2E;
+  const ga__f2 nl2 = ga__f2_of(l2, l2), k02 = ga__f2_of(k0, k0), k12 = ga__f2_of(k1, k1);
+  ga__lp_words q[GA_LP_U];
+  if (!none) {
+#pragma unroll
+    for (int u = 0; u < GA_LP_U; u++)
+      if (w0 + u * blockDim.x < r.nv) q[u] = ga__lp_load(L, r, w0 + u * blockDim.x);
+  }
+#pragma unroll
+  for (int u = 0; u < GA_LP_U; u++) {
+    const unsigned int w = w0 + u * blockDim.x;
+    if (w >= r.nv) break;
+    float x[2 * GA_LP_PAIRS];
+    if (none) {
+#pragma unroll
+      for (int j = 0; j < 2 * GA_LP_PAIRS; j++) x[j] = 0.0f;
+    } else {
+#pragma unroll
+      for (int k = 0; k < GA_LP_PAIRS; k++) {
+        float p, s;
+        ga__lp_pair(q[u], k, p, s);
+        ga__f2_to(ga__f2_fma(ga__f2_add(ga__f2_of(p, s), nm2), c2, nl2), p, s);
+        p = ga__max_nan(p, -200.0f);
+        s = ga__max_nan(s, -200.0f);
+        const ga__f2 y = ga__f2_of(p, s);
+        const ga__f2 e = ga__f2_of(ga__ex2(p), ga__ex2(s));
+        ga__f2_to(ga__f2_mul(e, ga__f2_fma(k12, y, k02)), x[2 * k], x[2 * k + 1]);
+      }
+      const unsigned int at = (unsigned int)target + r.skip - w * GA_LP_E;
+      if (target >= 0 && at < GA_LP_E) {
+#pragma unroll
+        for (int j = 0; j < GA_LP_E; j++)
+          if (at == j) x[j] += L.scale * a;
+      }
+    }
+    const int whole = ga__lp_whole(L, r, w);
+    const unsigned int i0 = w * GA_LP_E < r.skip ? 0 : w * GA_LP_E - r.skip;
+    if (!whole && w * GA_LP_E < r.skip) { /* the row starts inside this vector */
+#pragma unroll
+      for (int j = 0; j < GA_LP_E; j++)
+        if (j >= (int)r.skip && j - r.skip < L.v)
+          ga__lm_put(reinterpret_cast<GA_LP_G_T *>(g + (long long)(j - r.skip) * L.o_col[4]), x[j]);
+    } else {
+      ga__lp_store(g, L.o_col[4], i0, L.v, x, whole);
+    }
+  }
+}
+#endif
