@@ -13,6 +13,15 @@ typedef struct em_layout { /* the templates' ga__em_layout */
   long long t_col, v_row, v_col;
 } em_layout;
 
+typedef struct eg_fill { /* the templates' ga__eg_fill */
+  CUdeviceptr p;
+  unsigned long long bytes, r0, r1;
+} eg_fill;
+
+typedef struct eg_sort { /* the templates' ga__eg_sort */
+  unsigned int n, tiles, tile, passes, pass;
+} eg_sort;
+
 struct _GpuEmbedGrad {
   gpucontext *ctx;
   ga_workspace ws;
@@ -184,19 +193,71 @@ void GpuEmbedGrad_free(GpuEmbedGrad *eg) {
   ga_ctx_unref(ctx);
 }
 
-#define EG_STEP 8 /* tokens a group of threads loads at once: GA_EG_U of the template */
+/* constants of the template */
+#define EG_STEP 8        /* GA_EG_U */
+#define EG_FEW 512       /* GA_EG_FEW */
+#define EG_TX 32         /* GA_EG_TX */
+#define EG_BITS 9        /* GA_EG_BITS */
+#define EG_THREADS 512   /* GA_EG_THREADS */
+#define EG_ROUND 2048    /* GA_EG_ROUND */
+#define EG_MAX_TILES 128 /* every sorting CTA reads all tiles' counts: 256 KiB at most */
+
+static int launch_direct(GpuEmbedGrad *eg, em_layout *L, uint64_t key, CUdeviceptr *p_dt,
+                         CUdeviceptr *p_do, CUdeviceptr *p_ids, CUdeviceptr *p_err) {
+  gpucontext *ctx = eg->ctx;
+  const ga_function *fn;
+  void *params[5];
+  unsigned grid[3] = {1, 1, 1}, block[3] = {1, 1, 1};
+  unsigned long long ctas;
+  int err = ga_lm_kernel(ctx, "ga_eg_direct", key, emit, &fn);
+  if (err != GA_NO_ERROR) return err;
+  while (block[0] < EG_TX && block[0] < L->nv) block[0] *= 2;
+  block[1] = 256 / block[0];
+  grid[1] = (L->nv + block[0] - 1) / block[0];
+  if (grid[1] > 65535) return ga_err_set(ctx->err, GA_XLARGE_ERROR, "Too long rows for one call");
+  /* the slices of all row ranges fill the device about once */
+  ctas = (unsigned long long)ctx->num_sms * 8 / grid[1];
+  if (ctas == 0) ctas = 1;
+  L->chunk = (unsigned)((L->v + ctas - 1) / ctas);
+  grid[0] = (unsigned)((L->v + L->chunk - 1) / L->chunk);
+  params[0] = L;
+  params[1] = p_dt;
+  params[2] = p_do;
+  params[3] = p_ids;
+  params[4] = p_err;
+  return ga_launch(ctx, fn, grid, block, 0, params);
+}
+
+/* The part `i` of `parts` of dtable's rows for the CTAs beside a sorting launch to write zeros to. */
+static void fill_part(eg_fill *F, const em_layout *L, CUdeviceptr p_dt, unsigned e, size_t es,
+                      int accumulate, unsigned i, unsigned parts) {
+  const unsigned long long row = (unsigned long long)L->nv * e * es, all = row * L->v;
+  memset(F, 0, sizeof(*F));
+  F->p = p_dt;
+  if (accumulate) return;
+  if (L->v_col == (long long)es && (L->v_row == (long long)row || L->v == 1) && p_dt % 16 == 0) {
+    const unsigned long long step = (all / parts + 15) / 16 * 16, lo = step * i < all ? step * i : all;
+    F->p = p_dt + lo;
+    F->bytes = i + 1 == parts || all - lo < step ? all - lo : step;
+  } else {
+    F->r0 = L->v * i / parts;
+    F->r1 = L->v * (i + 1) / parts;
+  }
+}
 
 int GpuEmbedGrad_call(GpuEmbedGrad *eg, GpuArray *dtable, const GpuArray *dout, const GpuArray *ids,
                       double scale, ssize_t pad, int flags) {
   gpucontext *ctx;
-  const ga_function *order, *sum, *join, *zero;
+  const ga_function *count, *scatter, *sum, *join;
   em_layout L;
   ga_lead lead;
-  CUdeviceptr p_dt, p_do, p_ids, p_err, p_key, p_order, p_part;
-  void *params[6];
-  unsigned grid[3] = {1, 1, 1}, block[3], one[3] = {256, 1, 1}, g1[3] = {1, 1, 1}, e, ny;
-  unsigned long long groups, per_group;
-  size_t fsize, list;
+  eg_fill F;
+  eg_sort S;
+  CUdeviceptr p_dt, p_do, p_ids, p_err, p_counts, p_key[2], p_order[2], p_part;
+  void *params[9];
+  unsigned grid[3] = {1, 1, 1}, block[3], flat[3] = {EG_THREADS, 1, 1}, g1[3] = {1, 1, 1}, e, ny, bits, last;
+  unsigned long long groups;
+  size_t fsize, list, cbytes, es;
   uint64_t key;
   int err, accumulate;
 
@@ -211,16 +272,30 @@ int GpuEmbedGrad_call(GpuEmbedGrad *eg, GpuArray *dtable, const GpuArray *dout, 
           GA_NO_ERROR)
     return err;
   accumulate = ISSET(flags, GA_EMBED_ACCUMULATE);
+  es = gpuarray_get_elsize(dtable->typecode);
   e = vector_width(dout, dtable, dtable->dimensions[1]);
   err = fill(ctx, &L, &lead, dout, dtable, ids, scale, pad, flags, e);
-  if (err != GA_NO_ERROR || L.nv == 0) return err;
+  if (err != GA_NO_ERROR) return err;
   if (L.n > 0x7fffffffULL)
     return ga_err_set(ctx->err, GA_XLARGE_ERROR, "More than 2^31 - 1 tokens in one call");
+  if (L.nv == 0 || (L.n == 0 && accumulate)) return GA_NO_ERROR;
 
   key = (uint64_t)dout->typecode | (uint64_t)dtable->typecode << 8 | (uint64_t)ids->typecode << 16 |
         (uint64_t)e << 24 | (uint64_t)lead.nd << 32 | (uint64_t)1 << 40 | (uint64_t)accumulate << 41;
-  if ((err = ga_lm_kernel(ctx, "ga_eg_order", key, emit, &order)) != GA_NO_ERROR ||
-      (err = ga_lm_kernel(ctx, "ga_eg_zero", key, emit, &zero)) != GA_NO_ERROR ||
+  p_dt = dtable->data->ptr + dtable->offset;
+  p_do = dout->data->ptr + dout->offset;
+  p_ids = ids->data->ptr + ids->offset;
+  p_err = ISSET(flags, GA_EMBED_CHECK) ? ga_lm_err_word(ctx) : 0;
+
+  if (L.n <= EG_FEW && L.v > 0) {
+    err = launch_direct(eg, &L, key, &p_dt, &p_do, &p_ids, &p_err);
+    if (err == GA_NO_ERROR && ISSET(flags, GA_EMBED_CHECK))
+      err = ga_lm_err_take(ctx, "A token id is outside the table");
+    return err;
+  }
+
+  if ((err = ga_lm_kernel(ctx, "ga_eg_count", key, emit, &count)) != GA_NO_ERROR ||
+      (err = ga_lm_kernel(ctx, "ga_eg_scatter", key, emit, &scatter)) != GA_NO_ERROR ||
       (err = ga_lm_kernel(ctx, "ga_eg_sum", key, emit, &sum)) != GA_NO_ERROR ||
       (err = ga_lm_kernel(ctx, "ga_eg_join", key, emit, &join)) != GA_NO_ERROR)
     return err;
@@ -229,53 +304,63 @@ int GpuEmbedGrad_call(GpuEmbedGrad *eg, GpuArray *dtable, const GpuArray *dout, 
   if (ny > 65535) return ga_err_set(ctx->err, GA_XLARGE_ERROR, "Too long rows for one call");
   grid[1] = ny;
   /* Chunks: enough groups to fill the device about twice, none shorter than one step. */
-  per_group = (unsigned long long)block[0] * ny;
-  groups = (unsigned long long)ctx->num_sms * 4096 / per_group;
+  groups = (unsigned long long)ctx->num_sms * 4096 / ((unsigned long long)block[0] * ny);
   if (groups == 0) groups = 1;
   L.chunk = (unsigned)((L.n + groups - 1) / groups);
   L.chunk = (L.chunk + EG_STEP - 1) / EG_STEP * EG_STEP;
-  if (L.chunk == 0) L.chunk = EG_STEP;
   L.chunks = (unsigned)((L.n + L.chunk - 1) / L.chunk);
+
+  S.n = (unsigned)L.n;
+  S.tiles = (unsigned)((L.n + EG_ROUND - 1) / EG_ROUND);
+  if (S.tiles > EG_MAX_TILES) S.tiles = EG_MAX_TILES;
+  S.tile = (unsigned)(((L.n + S.tiles - 1) / S.tiles + EG_ROUND - 1) / EG_ROUND * EG_ROUND);
+  S.tiles = (unsigned)((L.n + S.tile - 1) / S.tile);
+  for (bits = 1; bits < 32 && (L.v >> bits) != 0; bits++) {} /* keys go up to V */
+  S.passes = (bits + EG_BITS - 1) / EG_BITS;
 
   fsize = dout->typecode == GA_DOUBLE || dtable->typecode == GA_DOUBLE ? 8 : 4;
   list = ((size_t)L.n * 4 + 511) / 512 * 512;
-  err = ga_workspace_need(ctx, &eg->ws, 2 * list + 2 * (size_t)L.chunks * L.nv * e * fsize);
+  cbytes = (size_t)S.passes * EG_THREADS * S.tiles * 4;
+  err = ga_workspace_need(ctx, &eg->ws, cbytes + 4 * list + 2 * (size_t)L.chunks * L.nv * e * fsize);
   if (err != GA_NO_ERROR) return err;
+  p_counts = eg->ws.cur->ptr;
+  p_key[0] = p_counts + cbytes;
+  p_order[0] = p_key[0] + list;
+  p_key[1] = p_order[0] + list;
+  p_order[1] = p_key[1] + list;
+  p_part = p_order[1] + list;
 
-  p_dt = dtable->data->ptr + dtable->offset;
-  p_do = dout->data->ptr + dout->offset;
-  p_ids = ids->data->ptr + ids->offset;
-  p_err = ISSET(flags, GA_EMBED_CHECK) ? ga_lm_err_word(ctx) : 0;
+  /* the CTAs that write zeros: what the device holds beside the sorting ones */
+  g1[0] = S.tiles + (accumulate ? 0 : ctx->num_sms * 4 > S.tiles + ctx->num_sms ? ctx->num_sms * 4 - S.tiles : ctx->num_sms);
   params[0] = &L;
-  params[1] = &p_dt;
-  if (!accumulate && L.v > 0) {
-    unsigned long long rows = (L.v + block[1] - 1) / block[1], most = (unsigned long long)ctx->num_sms * 16;
-    grid[0] = (unsigned)(rows > most ? most : rows);
-    err = ga_launch(ctx, zero, grid, block, 0, params);
-    if (err != GA_NO_ERROR) return err;
+  params[1] = &S;
+  params[2] = &F;
+  params[3] = &p_counts;
+  params[4] = &p_ids;
+  params[5] = &p_err;
+  fill_part(&F, &L, p_dt, e, es, accumulate, 0, S.passes + 1);
+  err = ga_launch(ctx, count, g1, flat, 0, params);
+  for (S.pass = 0; S.pass < S.passes && err == GA_NO_ERROR; S.pass++) {
+    fill_part(&F, &L, p_dt, e, es, accumulate, S.pass + 1, S.passes + 1);
+    params[5] = &p_key[1 - S.pass % 2];
+    params[6] = &p_order[1 - S.pass % 2];
+    params[7] = &p_key[S.pass % 2];
+    params[8] = &p_order[S.pass % 2];
+    err = ga_launch(ctx, scatter, g1, flat, 0, params);
   }
-  if (L.n == 0) return GA_NO_ERROR;
-  p_key = eg->ws.cur->ptr;
-  p_order = p_key + list;
-  p_part = p_order + list;
+  last = (S.passes - 1) % 2;
 
-  params[1] = &p_key;
-  params[2] = &p_order;
-  params[3] = &p_ids;
-  params[4] = &p_err;
-  g1[0] = (unsigned)((L.n + 7) / 8);
-  err = ga_launch(ctx, order, g1, one, 0, params);
-  if (err != GA_NO_ERROR) return err;
-
-  grid[0] = (L.chunks + block[1] - 1) / block[1];
-  params[1] = &p_dt;
-  params[2] = &p_do;
-  params[3] = &p_key;
-  params[4] = &p_order;
-  params[5] = &p_part;
-  err = ga_launch(ctx, sum, grid, block, 0, params);
+  if (err == GA_NO_ERROR) {
+    grid[0] = (L.chunks + block[1] - 1) / block[1];
+    params[1] = &p_dt;
+    params[2] = &p_do;
+    params[3] = &p_key[last];
+    params[4] = &p_order[last];
+    params[5] = &p_part;
+    err = ga_launch(ctx, sum, grid, block, 0, params);
+  }
   if (err == GA_NO_ERROR && L.chunks > 1) {
-    params[2] = &p_key;
+    params[2] = &p_key[last];
     params[3] = &p_part;
     err = ga_launch(ctx, join, grid, block, 0, params);
   }

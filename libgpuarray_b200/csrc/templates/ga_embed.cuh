@@ -91,58 +91,31 @@ ga_embed(const __grid_constant__ ga__em_layout L, char *out, const char *table, 
 #endif
 
 #ifdef GA_EM_BUILD_GRAD
-/* The gradient is a sum over SORTED tokens: three launches that depend on
- * nothing but the ids' values, so that the result is the same bits every time.
+/* The gradient is a sum over SORTED tokens, in launches that depend on nothing
+ * but the ids' values, so that the result is the same bits every time.
  *
- * 1. ga_eg_order: order[rank] = token, key[rank] = row, by row and, within a
- *    row, by token. Tokens that contribute nothing get the key V and go last.
- * 2. ga_eg_sum: the sorted tokens are cut into equal chunks; a group of threads
- *    sums a chunk's rows, one vector position per thread. A run of equal keys
- *    that lies inside the chunk is finished and written; the parts of runs that
- *    cross a chunk's ends go to `part`, which holds two rows per chunk.
- * 3. ga_eg_join: the group of the chunk in which a crossing run starts adds its
- *    parts in order and writes the row.
- * Rows that no token names are written by ga_eg_zero before (unless the
- * gradient is accumulated). */
+ * Few tokens: ga_eg_direct. A CTA owns a range of table rows and a slice of
+ * their vectors, picks its tokens from all ids, sorts them in shared memory,
+ * writes zeros and sums.
+ *
+ * Many tokens: the tokens are sorted by row and, within a row, by token (a
+ * radix sort of GA_EG_BITS bits a pass: ga_eg_count, then ga_eg_scatter for
+ * each pass, which also counts for the next). Tokens that contribute nothing
+ * get the key V and go last. The CTAs beyond the sort's write the zeros of the
+ * rows, a part of them in each launch, so that the sort hides behind them.
+ * Then ga_eg_sum: the sorted tokens are cut into equal chunks; a group of
+ * threads sums a chunk's rows, one vector position per thread. A run of equal
+ * keys that lies inside the chunk is finished and written; the parts of runs
+ * that cross a chunk's ends are parked, two rows per chunk. ga_eg_join: the
+ * group of the chunk in which a crossing run starts adds its parts in order
+ * and writes the row. */
 
-/* The tokens' ranks by counting: a warp per token compares its key with all. */
-extern "C" __global__ void __launch_bounds__(256)
-ga_eg_order(const __grid_constant__ ga__em_layout L, unsigned int *key, unsigned int *order,
-            const char *ids, int *err) {
-  ga__grid_dependency_sync();
-  const unsigned int n = (unsigned int)L.n, lane = threadIdx.x % 32;
-  const unsigned int t = blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
-  if (t >= n) return; /* a whole warp */
-  const long long mine = ga__em_row(L, ids, t);
-  if (mine == -2 && lane == 0 && err != nullptr) *err = -1;
-  const unsigned long long k = mine < 0 ? L.v : (unsigned long long)mine;
-  unsigned int before = 0;
-  for (unsigned int i = lane; i < n; i += 32) {
-    const long long other = ga__em_row(L, ids, i);
-    const unsigned long long o = other < 0 ? L.v : (unsigned long long)other;
-    before += o < k || (o == k && i < t);
-  }
-  before = ga__warp_sum_u32(before);
-  if (lane == 0) {
-    key[before] = (unsigned int)k;
-    order[before] = t;
-  }
-}
-
-extern "C" __global__ void __launch_bounds__(256)
-ga_eg_zero(const __grid_constant__ ga__em_layout L, char *dtable) {
-  ga__grid_dependency_sync();
-  const unsigned int v = blockIdx.y * blockDim.x + threadIdx.x;
-  if (v >= L.nv) return;
-  for (unsigned long long r = (unsigned long long)blockIdx.x * blockDim.y + threadIdx.y; r < L.v;
-       r += (unsigned long long)gridDim.x * blockDim.y) {
-    ga__lm_vec<GA_EM_O_T, GA_EM_E> q;
-#pragma unroll
-    for (int j = 0; j < GA_EM_E; j++) ga__lm_put(&q.v[j], (GA_EM_F_T)0);
-    *reinterpret_cast<ga__lm_vec<GA_EM_O_T, GA_EM_E> *>(dtable + (long long)r * L.v_row +
-                                                       (long long)v * GA_EM_E * L.v_col) = q;
-  }
-}
+/* zeros for a part of dtable: flat bytes where its rows are adjacent, else row by row */
+struct ga__eg_fill {
+  char *p;
+  unsigned long long bytes; /* > 0: flat */
+  unsigned long long r0, r1; /* rows, otherwise */
+};
 
 static __device__ __forceinline__ void ga__eg_write(const ga__em_layout &L, char *dtable,
                                                     unsigned int row, unsigned int v,
@@ -162,14 +135,238 @@ static __device__ __forceinline__ void ga__eg_write(const ga__em_layout &L, char
   *reinterpret_cast<ga__lm_vec<GA_EM_O_T, GA_EM_E> *>(p) = q;
 }
 
+static __device__ __forceinline__ void ga__eg_zero_row(const ga__em_layout &L, char *dtable,
+                                                       unsigned long long row, unsigned int v) {
+  ga__lm_vec<GA_EM_O_T, GA_EM_E> q;
+#pragma unroll
+  for (int j = 0; j < GA_EM_E; j++) ga__lm_put(&q.v[j], (GA_EM_F_T)0);
+  *reinterpret_cast<ga__lm_vec<GA_EM_O_T, GA_EM_E> *>(dtable + (long long)row * L.v_row +
+                                                     (long long)v * GA_EM_E * L.v_col) = q;
+}
+
+static __device__ __forceinline__ void ga__eg_zeros(const ga__em_layout &L, const ga__eg_fill &F,
+                                                    unsigned int cta, unsigned int ctas) {
+  if (F.bytes > 0) {
+    const unsigned long long n = F.bytes / 16, step = (unsigned long long)ctas * blockDim.x;
+    ga__lm_vec<unsigned int, 4> q;
+    q.v[0] = q.v[1] = q.v[2] = q.v[3] = 0;
+    for (unsigned long long i = (unsigned long long)cta * blockDim.x + threadIdx.x; i < n; i += step)
+      reinterpret_cast<ga__lm_vec<unsigned int, 4> *>(F.p)[i] = q;
+    /* what is left is less than 16 bytes */
+    if (cta == 0 && threadIdx.x < F.bytes - n * 16) F.p[n * 16 + threadIdx.x] = 0;
+    return;
+  }
+  const unsigned int lane = threadIdx.x % 32, warps = blockDim.x / 32;
+  for (unsigned long long r = F.r0 + (unsigned long long)cta * warps + threadIdx.x / 32; r < F.r1;
+       r += (unsigned long long)ctas * warps)
+    for (unsigned int v = lane; v < L.nv; v += 32) ga__eg_zero_row(L, F.p, r, v);
+}
+
+/* ---- sorting ---- */
+#define GA_EG_BITS 9
+#define GA_EG_DIGITS (1 << GA_EG_BITS)
+#define GA_EG_THREADS GA_EG_DIGITS /* a thread for each digit */
+#define GA_EG_WARPS (GA_EG_THREADS / 32)
+#define GA_EG_KEYS 4 /* a thread's keys of one round */
+#define GA_EG_ROUND (GA_EG_THREADS * GA_EG_KEYS)
+
+struct ga__eg_sort {
+  unsigned int n;      /* tokens */
+  unsigned int tiles;  /* CTAs that sort */
+  unsigned int tile;   /* tokens of each, a multiple of GA_EG_ROUND */
+  unsigned int passes; /* their number; this one's is `pass` */
+  unsigned int pass;
+};
+
+static __device__ __forceinline__ unsigned int ga__eg_key(const ga__em_layout &L, const char *ids,
+                                                          unsigned int i, int *err) {
+  const long long r = ga__em_row(L, ids, i);
+  if (r == -2 && err != nullptr) *err = -1;
+  return r < 0 ? (unsigned int)L.v : (unsigned int)r;
+}
+
+/* counts[pass][digit][tile]: how many keys of a tile have the digit. The first pass's are counted
+ * here, the others' are set to zero for ga_eg_scatter to add to. */
+extern "C" __global__ void __launch_bounds__(GA_EG_THREADS)
+ga_eg_count(const __grid_constant__ ga__em_layout L, const __grid_constant__ ga__eg_sort S,
+            const __grid_constant__ ga__eg_fill F, unsigned int *counts, const char *ids, int *err) {
+  ga__grid_dependency_sync();
+  if (blockIdx.x >= S.tiles) {
+    ga__eg_zeros(L, F, blockIdx.x - S.tiles, gridDim.x - S.tiles);
+    return;
+  }
+  __shared__ unsigned int hist[GA_EG_DIGITS];
+  const unsigned int d = threadIdx.x, tile = blockIdx.x;
+  hist[d] = 0;
+  __syncthreads();
+  const unsigned int lo = tile * S.tile, hi = S.n - lo < S.tile ? S.n : lo + S.tile;
+  for (unsigned int i = lo + threadIdx.x; i < hi; i += GA_EG_THREADS)
+    atomicAdd(&hist[ga__eg_key(L, ids, i, err) & (GA_EG_DIGITS - 1)], 1u);
+  __syncthreads();
+  counts[d * S.tiles + tile] = hist[d];
+  for (unsigned int p = 1; p < S.passes; p++)
+    counts[(p * GA_EG_DIGITS + d) * S.tiles + tile] = 0;
+}
+
+/* One pass: every key goes behind all with a smaller digit and, with an equal digit, behind those
+ * that stand before it. The first pass takes the ids themselves. */
+extern "C" __global__ void __launch_bounds__(GA_EG_THREADS)
+ga_eg_scatter(const __grid_constant__ ga__em_layout L, const __grid_constant__ ga__eg_sort S,
+              const __grid_constant__ ga__eg_fill F, unsigned int *counts, const char *ids,
+              const unsigned int *key_in, const unsigned int *order_in, unsigned int *key,
+              unsigned int *order) {
+  ga__grid_dependency_sync();
+  if (blockIdx.x >= S.tiles) {
+    ga__eg_zeros(L, F, blockIdx.x - S.tiles, gridDim.x - S.tiles);
+    return;
+  }
+  __shared__ unsigned int cnt[GA_EG_WARPS][GA_EG_DIGITS];
+  __shared__ unsigned int sums[GA_EG_WARPS];
+  const unsigned int d = threadIdx.x, lane = d % 32, warp = d / 32, tile = blockIdx.x;
+  const unsigned int shift = S.pass * GA_EG_BITS;
+
+  /* where the digit's keys of this tile begin */
+  const unsigned int *c = counts + (S.pass * GA_EG_DIGITS + d) * S.tiles;
+  unsigned int total = 0, before = 0;
+  for (unsigned int t = 0; t < S.tiles; t++) {
+    const unsigned int x = c[t];
+    total += x;
+    before += t < tile ? x : 0;
+  }
+  unsigned int scan = total;
+#pragma unroll
+  for (int s = 1; s < 32; s *= 2) {
+    const unsigned int o = __shfl_up_sync(0xffffffffu, scan, s);
+    if (lane >= (unsigned int)s) scan += o;
+  }
+  if (lane == 31) sums[warp] = scan;
+  __syncthreads();
+  unsigned int base = scan - total + before;
+  for (unsigned int w = 0; w < warp; w++) base += sums[w];
+
+  const unsigned int lo = tile * S.tile, hi = S.n - lo < S.tile ? S.n : lo + S.tile;
+  for (unsigned int i0 = lo; i0 < hi; i0 += GA_EG_ROUND) {
+    unsigned int k[GA_EG_KEYS], o[GA_EG_KEYS], rank[GA_EG_KEYS];
+#pragma unroll
+    for (int j = 0; j < GA_EG_KEYS; j++) { /* a warp's keys are adjacent */
+      const unsigned int i = i0 + (warp * GA_EG_KEYS + j) * 32 + lane;
+      k[j] = o[j] = 0;
+      if (i < hi) {
+        k[j] = S.pass == 0 ? ga__eg_key(L, ids, i, nullptr) : key_in[i];
+        o[j] = S.pass == 0 ? i : order_in[i];
+      }
+    }
+    for (int w = 0; w < GA_EG_WARPS; w++) cnt[w][d] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < GA_EG_KEYS; j++) {
+      const unsigned int i = i0 + (warp * GA_EG_KEYS + j) * 32 + lane;
+      const unsigned int digit = i < hi ? (k[j] >> shift) & (GA_EG_DIGITS - 1) : GA_EG_DIGITS;
+      const unsigned int same = __match_any_sync(0xffffffffu, digit);
+      const unsigned int seen = i < hi ? cnt[warp][digit] : 0;
+      rank[j] = seen + __popc(same & ((1u << lane) - 1));
+      __syncwarp();
+      if (i < hi && __ffs(same) - 1 == (int)lane) cnt[warp][digit] = seen + __popc(same);
+      __syncwarp();
+    }
+    __syncthreads();
+    for (int w = 0; w < GA_EG_WARPS; w++) { /* the digit's place for each warp */
+      const unsigned int x = cnt[w][d];
+      cnt[w][d] = base;
+      base += x;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < GA_EG_KEYS; j++) {
+      const unsigned int i = i0 + (warp * GA_EG_KEYS + j) * 32 + lane;
+      if (i < hi) {
+        const unsigned int at = cnt[warp][(k[j] >> shift) & (GA_EG_DIGITS - 1)] + rank[j];
+        key[at] = k[j];
+        order[at] = o[j];
+        if (S.pass + 1 < S.passes)
+          atomicAdd(&counts[((S.pass + 1) * GA_EG_DIGITS + ((k[j] >> (shift + GA_EG_BITS)) & (GA_EG_DIGITS - 1))) * S.tiles + at / S.tile], 1u);
+      }
+    }
+    __syncthreads();
+  }
+}
+
+/* ---- summing ---- */
 #define GA_EG_U 8
 
-static __device__ __forceinline__ void ga__eg_park(GA_EM_F_T *part, unsigned long long slot,
-                                                   unsigned int nv, unsigned int v,
-                                                   const GA_EM_F_T acc[GA_EM_E]) {
-  GA_EM_F_T *p = part + (slot * nv + v) * GA_EM_E;
+static __device__ __forceinline__ void ga__eg_park(GA_EM_F_T *p, const GA_EM_F_T acc[GA_EM_E]) {
 #pragma unroll
   for (int j = 0; j < GA_EM_E; j++) p[j] = acc[j];
+}
+
+/* Sums sorted tokens [lo, hi) of n at vector position v. head, tail: where the parts of the run
+ * that began before lo, and of the one that goes on behind hi, are parked. */
+static __device__ __forceinline__ void ga__eg_chunk(const ga__em_layout &L, char *dtable,
+                                                    const char *dout, const unsigned int *key,
+                                                    const unsigned int *order, unsigned int n,
+                                                    unsigned int lo, unsigned int hi, unsigned int v,
+                                                    GA_EM_F_T *head, GA_EM_F_T *tail) {
+  const unsigned int none = (unsigned int)L.v;
+  unsigned int cur = key[lo];
+  int open_head = lo > 0 && key[lo - 1] == cur;
+  GA_EM_F_T acc[GA_EM_E];
+#pragma unroll
+  for (int j = 0; j < GA_EM_E; j++) acc[j] = 0;
+  const char *col = dout + (long long)v * GA_EM_E * L.t_col;
+  for (unsigned int i = lo; i < hi && cur != none; i += GA_EG_U) {
+    unsigned int k[GA_EG_U];
+    ga__lm_vec<GA_EM_A_T, GA_EM_E> x[GA_EG_U];
+#pragma unroll
+    for (int u = 0; u < GA_EG_U; u++) k[u] = i + u < hi ? key[i + u] : none;
+#pragma unroll
+    for (int u = 0; u < GA_EG_U; u++)
+      if (k[u] != none)
+        x[u] = *reinterpret_cast<const ga__lm_vec<GA_EM_A_T, GA_EM_E> *>(
+            col + ga__lm_offset<GA_EM_ND>(order[i + u], L.dims, L.t_str));
+#pragma unroll
+    for (int u = 0; u < GA_EG_U; u++) {
+      if (i + u >= hi) break;
+      if (k[u] != cur) { /* the run ends inside the chunk */
+        if (open_head) ga__eg_park(head, acc);
+        else ga__eg_write(L, dtable, cur, v, acc);
+        open_head = 0;
+        cur = k[u];
+#pragma unroll
+        for (int j = 0; j < GA_EM_E; j++) acc[j] = 0;
+        if (cur == none) break;
+      }
+#pragma unroll
+      for (int j = 0; j < GA_EM_E; j++) acc[j] += (GA_EM_F_T)ga__lm_get(x[u].v[j]);
+    }
+  }
+  if (cur == none) return;
+  if (open_head) ga__eg_park(head, acc);
+  else if (hi < n && key[hi] == cur) ga__eg_park(tail, acc);
+  else ga__eg_write(L, dtable, cur, v, acc);
+}
+
+/* Joins the run that starts in chunk c (tokens c * size ...) and goes on in the next, if there is
+ * one. part: the chunks' parked rows at this vector position, heads and tails in turn, `step`
+ * elements apart. */
+static __device__ __forceinline__ void ga__eg_join_run(const ga__em_layout &L, char *dtable,
+                                                       const unsigned int *key, unsigned int c,
+                                                       unsigned int size, unsigned int chunks,
+                                                       unsigned int v, const GA_EM_F_T *part,
+                                                       size_t step) {
+  const unsigned int lo = c * size, next = lo + size; /* next < n: chunk c + 1 exists */
+  const unsigned int cur = key[next];
+  if (cur == (unsigned int)L.v || key[next - 1] != cur) return;
+  if (key[lo] == cur && lo > 0 && key[lo - 1] == cur) return; /* it began earlier */
+  GA_EM_F_T acc[GA_EM_E];
+  const GA_EM_F_T *p = part + (2 * (size_t)c + 1) * step;
+#pragma unroll
+  for (int j = 0; j < GA_EM_E; j++) acc[j] = p[j];
+  for (unsigned int d = c + 1; d < chunks && key[d * size] == cur; d++) {
+    p = part + 2 * (size_t)d * step;
+#pragma unroll
+    for (int j = 0; j < GA_EM_E; j++) acc[j] += p[j];
+  }
+  ga__eg_write(L, dtable, cur, v, acc);
 }
 
 extern "C" __global__ void __launch_bounds__(256)
@@ -179,46 +376,9 @@ ga_eg_sum(const __grid_constant__ ga__em_layout L, char *dtable, const char *dou
   const unsigned int v = blockIdx.y * blockDim.x + threadIdx.x;
   const unsigned int c = blockIdx.x * blockDim.y + threadIdx.y;
   if (v >= L.nv || c >= L.chunks) return;
-  const unsigned int n = (unsigned int)L.n;
-  const unsigned int lo = c * L.chunk, hi = n - lo < L.chunk ? n : lo + L.chunk;
-  const unsigned int none = (unsigned int)L.v;
-  unsigned int cur = key[lo];
-  int open_head = lo > 0 && key[lo - 1] == cur; /* the run began in an earlier chunk */
-  GA_EM_F_T acc[GA_EM_E];
-#pragma unroll
-  for (int j = 0; j < GA_EM_E; j++) acc[j] = 0;
-  for (unsigned int i = lo; i < hi && cur != none; i += GA_EG_U) {
-    unsigned int k[GA_EG_U];
-    GA_EM_F_T x[GA_EG_U][GA_EM_E];
-#pragma unroll
-    for (int u = 0; u < GA_EG_U; u++) k[u] = i + u < hi ? key[i + u] : none;
-#pragma unroll
-    for (int u = 0; u < GA_EG_U; u++)
-      if (k[u] != none)
-        ga__em_load<GA_EM_A_T>(x[u],
-                               dout + ga__lm_offset<GA_EM_ND>(order[i + u], L.dims, L.t_str) +
-                                   (long long)v * GA_EM_E * L.t_col,
-                               L.t_col);
-#pragma unroll
-    for (int u = 0; u < GA_EG_U; u++) {
-      if (i + u >= hi) break;
-      if (k[u] != cur) { /* the run ends inside the chunk */
-        if (open_head) ga__eg_park(part, 2ULL * c, L.nv, v, acc);
-        else ga__eg_write(L, dtable, cur, v, acc);
-        open_head = 0;
-        cur = k[u];
-#pragma unroll
-        for (int j = 0; j < GA_EM_E; j++) acc[j] = 0;
-        if (cur == none) break;
-      }
-#pragma unroll
-      for (int j = 0; j < GA_EM_E; j++) acc[j] += x[u][j];
-    }
-  }
-  if (cur == none) return;
-  if (open_head) ga__eg_park(part, 2ULL * c, L.nv, v, acc);
-  else if (hi < n && key[hi] == cur) ga__eg_park(part, 2ULL * c + 1, L.nv, v, acc);
-  else ga__eg_write(L, dtable, cur, v, acc);
+  const unsigned int n = (unsigned int)L.n, lo = c * L.chunk, hi = n - lo < L.chunk ? n : lo + L.chunk;
+  GA_EM_F_T *head = part + (2 * (size_t)c * L.nv + v) * GA_EM_E;
+  ga__eg_chunk(L, dtable, dout, key, order, n, lo, hi, v, head, head + (size_t)L.nv * GA_EM_E);
 }
 
 extern "C" __global__ void __launch_bounds__(256)
@@ -228,20 +388,71 @@ ga_eg_join(const __grid_constant__ ga__em_layout L, char *dtable, const unsigned
   const unsigned int v = blockIdx.y * blockDim.x + threadIdx.x;
   const unsigned int c = blockIdx.x * blockDim.y + threadIdx.y;
   if (v >= L.nv || c + 1 >= L.chunks) return;
-  const unsigned int lo = c * L.chunk, next = lo + L.chunk; /* next < n: chunk c + 1 exists */
-  const unsigned int cur = key[next];
-  /* only the chunk in which a crossing run starts joins it */
-  if (cur == (unsigned int)L.v || key[next - 1] != cur) return;
-  if (key[lo] == cur && lo > 0 && key[lo - 1] == cur) return;
-  GA_EM_F_T acc[GA_EM_E];
-  const GA_EM_F_T *p = part + ((2ULL * c + 1) * L.nv + v) * GA_EM_E;
-#pragma unroll
-  for (int j = 0; j < GA_EM_E; j++) acc[j] = p[j];
-  for (unsigned int d = c + 1; d < L.chunks && key[d * L.chunk] == cur; d++) {
-    p = part + (2ULL * d * L.nv + v) * GA_EM_E;
-#pragma unroll
-    for (int j = 0; j < GA_EM_E; j++) acc[j] += p[j];
+  ga__eg_join_run(L, dtable, key, c, L.chunk, L.chunks, v, part + (size_t)v * GA_EM_E,
+                  (size_t)L.nv * GA_EM_E);
+}
+
+/* ---- few tokens ---- */
+#define GA_EG_FEW 512 /* tokens at most */
+#define GA_EG_FEW_WARPS 8
+#define GA_EG_TX 32   /* vector positions of a CTA at most; blockDim.x * blockDim.y is 256 */
+
+/* CTA (x, y) owns L.chunk rows from x * L.chunk and the vectors of slice y. */
+extern "C" __global__ void __launch_bounds__(256)
+ga_eg_direct(const __grid_constant__ ga__em_layout L, char *dtable, const char *dout,
+             const char *ids, int *err) {
+  ga__grid_dependency_sync();
+  __shared__ unsigned int row[GA_EG_FEW], token[GA_EG_FEW], key[GA_EG_FEW], order[GA_EG_FEW];
+  __shared__ unsigned int found[GA_EG_FEW_WARPS];
+  __shared__ GA_EM_F_T part[256 * 2 * GA_EM_E];
+  const unsigned int tid = threadIdx.y * blockDim.x + threadIdx.x, lane = tid % 32, warp = tid / 32;
+  const unsigned int n = (unsigned int)L.n;
+  const unsigned long long r0 = (unsigned long long)blockIdx.x * L.chunk;
+  const unsigned long long r1 = L.v - r0 < L.chunk ? L.v : r0 + L.chunk;
+  /* the tokens of these rows, in their order */
+  unsigned int m = 0;
+  for (unsigned int i0 = 0; i0 < n; i0 += 256) {
+    const unsigned int i = i0 + tid;
+    unsigned long long r = L.v;
+    if (i < n) r = ga__eg_key(L, ids, i, blockIdx.x == 0 && blockIdx.y == 0 ? err : nullptr);
+    const int mine = r >= r0 && r < r1;
+    const unsigned int all = __ballot_sync(0xffffffffu, mine);
+    if (lane == 0) found[warp] = __popc(all);
+    __syncthreads();
+    unsigned int at = m + __popc(all & ((1u << lane) - 1));
+    for (unsigned int w = 0; w < GA_EG_FEW_WARPS; w++) {
+      at += w < warp ? found[w] : 0;
+      m += found[w];
+    }
+    if (mine) {
+      row[at] = (unsigned int)r;
+      token[at] = i;
+    }
+    __syncthreads();
   }
-  ga__eg_write(L, dtable, cur, v, acc);
+  /* sorted by row: a token's place is the number of those before it */
+  for (unsigned int i = tid; i < m; i += 256) {
+    const unsigned int k = row[i];
+    unsigned int at = 0;
+    for (unsigned int j = 0; j < m; j++) at += row[j] < k || (row[j] == k && j < i);
+    key[at] = k;
+    order[at] = token[i];
+  }
+  const unsigned int v = blockIdx.y * blockDim.x + threadIdx.x;
+#if !GA_EM_ACCUMULATE
+  if (v < L.nv)
+    for (unsigned long long r = r0 + threadIdx.y; r < r1; r += blockDim.y) ga__eg_zero_row(L, dtable, r, v);
+#endif
+  __syncthreads();
+  if (m == 0) return;
+  const unsigned int size = (m + blockDim.y - 1) / blockDim.y, chunks = (m + size - 1) / size;
+  const unsigned int c = threadIdx.y;
+  GA_EM_F_T *mine = part + threadIdx.x * GA_EM_E;
+  const size_t step = (size_t)blockDim.x * GA_EM_E;
+  if (v < L.nv && c < chunks)
+    ga__eg_chunk(L, dtable, dout, key, order, m, c * size, m - c * size < size ? m : (c + 1) * size, v,
+                 mine + 2 * c * step, mine + (2 * c + 1) * step);
+  __syncthreads();
+  if (v < L.nv && c + 1 < chunks) ga__eg_join_run(L, dtable, key, c, size, chunks, v, mine, step);
 }
 #endif

@@ -170,6 +170,7 @@ def grad_tol(want, size, counts, dtype, f64):
 
 GRAD_CASES = [  # tokens, rows, width
     (1, 1, 1), (1, 5, 8), (2, 1, 3), (7, 3, 16), (40, 6, 5), (64, 64, 24), (100, 2, 9), (257, 30, 12), (300, 1, 4),
+    (512, 40, 33), (513, 3, 4), (2600, 600, 9), (5000, 511, 3), (700, 300000, 1),
 ]
 
 
@@ -227,7 +228,7 @@ def test_embed_gradient_negative_ids_and_all_padding(api, ctx, rng):
 def test_embed_gradient_strides_and_growing_calls(api, ctx, rng):
     """one operator for calls of growing and shrinking size; strided ids, dout and dtable"""
     op = api.GpuEmbedGrad(ctx)
-    for tokens, rows, width, dtype in ((5, 4, 8, "f4"), (120, 9, 24, "f2"), (3, 4, 8, "f4"), (70, 40, 6, "f2")):
+    for tokens, rows, width, dtype in ((5, 4, 8, "f4"), (1300, 9, 24, "f2"), (300, 4, 8, "f4"), (3000, 600, 6, "f2")):
         dout = rng.standard_normal((2, tokens, width)).astype(dtype)
         tok = rng.integers(0, rows, (2, tokens + 1)).astype(np.int64)
         d, _, _ = strided(api, ctx, dout)
