@@ -200,6 +200,7 @@ void GpuEmbedGrad_free(GpuEmbedGrad *eg) {
 #define EG_BITS 9        /* GA_EG_BITS */
 #define EG_THREADS 512   /* GA_EG_THREADS */
 #define EG_ROUND 2048    /* GA_EG_ROUND */
+#define EG_GROUP_THREADS 1024
 #define EG_MAX_TILES 128 /* every sorting CTA reads all tiles' counts: 256 KiB at most */
 
 static int launch_direct(GpuEmbedGrad *eg, em_layout *L, uint64_t key, CUdeviceptr *p_dt,
@@ -253,8 +254,8 @@ int GpuEmbedGrad_call(GpuEmbedGrad *eg, GpuArray *dtable, const GpuArray *dout, 
   ga_lead lead;
   eg_fill F;
   eg_sort S;
-  CUdeviceptr p_dt, p_do, p_ids, p_err, p_counts, p_key[2], p_order[2], p_part;
-  void *params[9];
+  CUdeviceptr p_dt, p_do, p_ids, p_err, p_counts, p_key[2], p_order[2], p_off, p_part;
+  void *params[10];
   unsigned grid[3] = {1, 1, 1}, block[3], flat[3] = {EG_THREADS, 1, 1}, g1[3] = {1, 1, 1}, e, ny, bits, last;
   unsigned long long groups;
   size_t fsize, list, cbytes, es;
@@ -303,8 +304,9 @@ int GpuEmbedGrad_call(GpuEmbedGrad *eg, GpuArray *dtable, const GpuArray *dout, 
   ga_lm_geometry(L.nv, block, &ny);
   if (ny > 65535) return ga_err_set(ctx->err, GA_XLARGE_ERROR, "Too long rows for one call");
   grid[1] = ny;
-  /* Chunks: enough groups to fill the device about twice, none shorter than one step. */
-  groups = (unsigned long long)ctx->num_sms * 4096 / ((unsigned long long)block[0] * ny);
+  /* Chunks: threads for half the device, which with EG_STEP loads of a thread in flight keep the
+   * memory busy; more and shorter ones only leave more parts to join. None shorter than one step. */
+  groups = (unsigned long long)ctx->num_sms * EG_GROUP_THREADS / ((unsigned long long)block[0] * ny);
   if (groups == 0) groups = 1;
   L.chunk = (unsigned)((L.n + groups - 1) / groups);
   L.chunk = (L.chunk + EG_STEP - 1) / EG_STEP * EG_STEP;
@@ -319,16 +321,17 @@ int GpuEmbedGrad_call(GpuEmbedGrad *eg, GpuArray *dtable, const GpuArray *dout, 
   S.passes = (bits + EG_BITS - 1) / EG_BITS;
 
   fsize = dout->typecode == GA_DOUBLE || dtable->typecode == GA_DOUBLE ? 8 : 4;
-  list = ((size_t)L.n * 4 + 511) / 512 * 512;
+  list = ((size_t)(L.n + EG_STEP) * 4 + 511) / 512 * 512;
   cbytes = (size_t)S.passes * EG_THREADS * S.tiles * 4;
-  err = ga_workspace_need(ctx, &eg->ws, cbytes + 4 * list + 2 * (size_t)L.chunks * L.nv * e * fsize);
+  err = ga_workspace_need(ctx, &eg->ws, cbytes + 6 * list + 2 * (size_t)L.chunks * L.nv * e * fsize);
   if (err != GA_NO_ERROR) return err;
   p_counts = eg->ws.cur->ptr;
   p_key[0] = p_counts + cbytes;
   p_order[0] = p_key[0] + list;
   p_key[1] = p_order[0] + list;
   p_order[1] = p_key[1] + list;
-  p_part = p_order[1] + list;
+  p_off = p_order[1] + list;
+  p_part = p_off + 2 * list;
 
   /* the CTAs that write zeros: what the device holds beside the sorting ones */
   g1[0] = S.tiles + (accumulate ? 0 : ctx->num_sms * 4 > S.tiles + ctx->num_sms ? ctx->num_sms * 4 - S.tiles : ctx->num_sms);
@@ -346,6 +349,7 @@ int GpuEmbedGrad_call(GpuEmbedGrad *eg, GpuArray *dtable, const GpuArray *dout, 
     params[6] = &p_order[1 - S.pass % 2];
     params[7] = &p_key[S.pass % 2];
     params[8] = &p_order[S.pass % 2];
+    params[9] = &p_off;
     err = ga_launch(ctx, scatter, g1, flat, 0, params);
   }
   last = (S.passes - 1) % 2;
@@ -355,7 +359,7 @@ int GpuEmbedGrad_call(GpuEmbedGrad *eg, GpuArray *dtable, const GpuArray *dout, 
     params[1] = &p_dt;
     params[2] = &p_do;
     params[3] = &p_key[last];
-    params[4] = &p_order[last];
+    params[4] = &p_off;
     params[5] = &p_part;
     err = ga_launch(ctx, sum, grid, block, 0, params);
   }

@@ -45,53 +45,95 @@ static __device__ __forceinline__ unsigned int ga__cn_find(const ga__cn_layout &
   return lo;
 }
 
-/* Vector w of an array: elements w * E - skip ..., those inside [0, n); the others read as 0. */
-template <typename T, int E>
-static __device__ __forceinline__ ga__lm_vec<T, E> ga__cn_load(const char *src, unsigned long long n,
-                                                               unsigned int skip,
-                                                               unsigned long long w) {
-  const unsigned long long i0 = w * E - skip; /* wraps below the start */
-  if (w * E >= skip && i0 + E <= n)
-    return *reinterpret_cast<const ga__lm_vec<T, E> *>(src + (long long)i0 * (long long)sizeof(T));
-  ga__lm_vec<T, E> q;
-#pragma unroll
-  for (int j = 0; j < E; j++) {
-    q.v[j] = T();
-    if (i0 + j < n) q.v[j] = reinterpret_cast<const T *>(src)[i0 + j];
-  }
-  return q;
+/* A block of an array: 8 vectors of a thread. */
+#define GA_CN_U 8
+struct ga__cn_at {
+  const ga__cn_item *t;
+  unsigned int skip;     /* elements of the first vector below the array's start */
+  unsigned long long w0; /* the thread's first vector */
+  int inner;             /* every vector of the block is whole */
+};
+
+template <int ES>
+static __device__ __forceinline__ ga__cn_at ga__cn_open(const ga__cn_item &t, unsigned int b) {
+  const unsigned int E = 16 / ES;
+  ga__cn_at a;
+  const unsigned long long w = (unsigned long long)(b - t.first) * GA_CN_VECS;
+  a.t = &t;
+  a.skip = (unsigned int)((size_t)t.src & 15) / ES;
+  a.w0 = w + threadIdx.x;
+  a.inner = w * E >= a.skip && (w + GA_CN_VECS) * E - a.skip <= t.n;
+  return a;
 }
 
-/* squares of one vector: exact in float for halves, summed over 8 of them before they go to
- * double; floats and doubles are squared in double, so that no finite value overflows or vanishes */
-static __device__ __forceinline__ double ga__cn_squares(const ga__lm_vec<ga_half, 8> &q) {
-  float s = 0.0f;
+/* The thread's vectors; elements outside the array read as 0. */
+template <int ES>
+static __device__ __forceinline__ void ga__cn_load(ga__lm_raw<16> q[GA_CN_U], const ga__cn_at &a) {
+  const unsigned int E = 16 / ES;
+  const char *base = a.t->src - a.skip * ES; /* on a 16-byte boundary */
+  if (a.inner) {
 #pragma unroll
-  for (int j = 0; j < 8; j++) {
-    const float x = ga_half2float(q.v[j]);
-    s = fmaf(x, x, s);
+    for (int u = 0; u < GA_CN_U; u++)
+      q[u] = ga__lm_load<ga__lm_raw<16> >(base + (a.w0 + u * GA_CN_THREADS) * 16);
+    return;
   }
-  return (double)s;
+#pragma unroll
+  for (int u = 0; u < GA_CN_U; u++) {
+    const unsigned long long w = a.w0 + u * GA_CN_THREADS, i = w * E - a.skip; /* wraps below the start */
+    if (w * E >= a.skip && i + E <= a.t->n) {
+      q[u] = ga__lm_load<ga__lm_raw<16> >(base + w * 16);
+      continue;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j++) q[u].w[j] = 0;
+#pragma unroll
+    for (int j = 0; j < (int)E; j++)
+      if (i + j < a.t->n) {
+        const ga__lm_raw<ES> one = ga__lm_load<ga__lm_raw<ES> >(a.t->src + (i + j) * ES);
+        if (ES == 2) q[u].w[j / 2] |= (unsigned int)one.w[0] << (16 * (j & 1));
+        else
+          for (int h = 0; h < (ES < 4 ? 1 : ES / 4); h++) q[u].w[j * (ES / 4) + h] = one.w[h];
+      }
+  }
 }
-template <typename T, int E>
-static __device__ __forceinline__ double ga__cn_squares(const ga__lm_vec<T, E> &q) {
+
+/* Squares of a vector, summed in float pairs: those of halfs are exact and 8 of them are summed
+ * before they go to double; floats and doubles are squared in double, so that no finite value
+ * overflows or vanishes. */
+static __device__ __forceinline__ double ga__cn_squares(const ga__lm_raw<16> &q, ga_half) {
+  ga__f2 s = ga__f2_of(0.0f, 0.0f);
+  float a, b;
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    ga__unpack_h2(q.w[j], a, b);
+    const ga__f2 x = ga__f2_of(a, b);
+    s = ga__f2_fma(x, x, s);
+  }
+  ga__f2_to(s, a, b);
+  return (double)(a + b);
+}
+static __device__ __forceinline__ double ga__cn_squares(const ga__lm_raw<16> &q, ga_float) {
   double s = 0.0;
 #pragma unroll
-  for (int j = 0; j < E; j++) s = fma((double)q.v[j], (double)q.v[j], s);
+  for (int j = 0; j < 4; j++) {
+    const double x = (double)__uint_as_float(q.w[j]);
+    s = fma(x, x, s);
+  }
   return s;
 }
+static __device__ __forceinline__ double ga__cn_squares(const ga__lm_raw<16> &q, ga_double) {
+  double x[2];
+  ga__lm_get<ga_double, 2>(x, q);
+  return fma(x[1], x[1], x[0] * x[0]);
+}
 
-#define GA_CN_U 8
-template <typename T, int E>
+template <typename T>
 static __device__ __forceinline__ double ga__cn_block(const ga__cn_item &t, unsigned int b) {
-  const unsigned int skip = (unsigned int)((size_t)t.src & 15) / (unsigned int)sizeof(T);
-  const unsigned long long w0 = (unsigned long long)(b - t.first) * GA_CN_VECS + threadIdx.x;
-  ga__lm_vec<T, E> q[GA_CN_U];
-#pragma unroll
-  for (int u = 0; u < GA_CN_U; u++) q[u] = ga__cn_load<T, E>(t.src, t.n, skip, w0 + u * GA_CN_THREADS);
+  ga__lm_raw<16> q[GA_CN_U];
+  ga__cn_load<(int)sizeof(T)>(q, ga__cn_open<(int)sizeof(T)>(t, b));
   double s = 0.0;
 #pragma unroll
-  for (int u = 0; u < GA_CN_U; u++) s += ga__cn_squares(q[u]);
+  for (int u = 0; u < GA_CN_U; u++) s += ga__cn_squares(q[u], T());
   return s;
 }
 
@@ -104,9 +146,9 @@ ga_cn_norm(const __grid_constant__ ga__cn_layout L, double *part, ga__cn_result 
   double s = 0.0;
   for (unsigned int b = blockIdx.x; b < L.blocks; b += gridDim.x) {
     const ga__cn_item &t = L.item[ga__cn_find(L, b)];
-    if (t.stype == 0) s += ga__cn_block<ga_half, 8>(t, b);
-    else if (t.stype == 1) s += ga__cn_block<ga_float, 4>(t, b);
-    else s += ga__cn_block<ga_double, 2>(t, b);
+    if (t.stype == 0) s += ga__cn_block<ga_half>(t, b);
+    else if (t.stype == 1) s += ga__cn_block<ga_float>(t, b);
+    else s += ga__cn_block<ga_double>(t, b);
   }
   const unsigned int lane = threadIdx.x % 32;
 #pragma unroll
@@ -145,27 +187,34 @@ ga_cn_norm(const __grid_constant__ ga__cn_layout L, double *part, ga__cn_result 
   }
 }
 
-template <typename T, typename D, typename F, int E>
+template <typename T, typename D, typename F>
 static __device__ __forceinline__ void ga__cn_scale(const ga__cn_item &t, unsigned int b, F factor) {
-  const unsigned int skip = (unsigned int)((size_t)t.src & 15) / (unsigned int)sizeof(T);
-  const unsigned long long w0 = (unsigned long long)(b - t.first) * GA_CN_VECS + threadIdx.x;
+  const int E = 16 / (int)sizeof(T);
   typedef ga__lm_vec<D, E> vec;
-  const int aligned = (((size_t)t.dst - (size_t)skip * sizeof(D)) & (alignof(vec) - 1)) == 0;
-  ga__lm_vec<T, E> q[GA_CN_U];
-#pragma unroll
-  for (int u = 0; u < GA_CN_U; u++) q[u] = ga__cn_load<T, E>(t.src, t.n, skip, w0 + u * GA_CN_THREADS);
+  const ga__cn_at a = ga__cn_open<(int)sizeof(T)>(t, b);
+  char *base = t.dst - a.skip * sizeof(D);
+  const int aligned = ((size_t)base & (alignof(vec) - 1)) == 0;
+  ga__lm_raw<16> q[GA_CN_U];
+  ga__cn_load<(int)sizeof(T)>(q, a);
 #pragma unroll
   for (int u = 0; u < GA_CN_U; u++) {
-    const unsigned long long w = w0 + u * GA_CN_THREADS, i0 = w * E - skip;
-    vec o;
+    const unsigned long long w = a.w0 + u * GA_CN_THREADS, i = w * E - a.skip;
+    F x[E];
+    ga__lm_get<T, E>(x, q[u]);
 #pragma unroll
-    for (int j = 0; j < E; j++) ga__lm_put(&o.v[j], (F)ga__lm_get(q[u].v[j]) * factor);
-    if (aligned && w * E >= skip && i0 + E <= t.n) {
-      *reinterpret_cast<vec *>(t.dst + (long long)i0 * (long long)sizeof(D)) = o;
+    for (int j = 0; j < E; j++) x[j] *= factor;
+    if (aligned && (a.inner || (w * E >= a.skip && i + E <= t.n))) {
+      vec o;
+      ga__lm_put<D, E>(o, x);
+      ga__lm_store(base + w * sizeof(vec), o);
     } else {
 #pragma unroll
       for (int j = 0; j < E; j++)
-        if (i0 + j < t.n) reinterpret_cast<D *>(t.dst)[i0 + j] = o.v[j];
+        if (i + j < t.n) {
+          ga__lm_vec<D, 1> o;
+          ga__lm_put<D, 1>(o, x + j);
+          ga__lm_store(t.dst + (i + j) * sizeof(D), o);
+        }
     }
   }
 }
@@ -181,12 +230,12 @@ ga_cn_scale(const __grid_constant__ ga__cn_layout L, const ga__cn_result *res) {
     /* an array that stays where it is and is multiplied by one is what it was */
     if (t.dst == t.src && t.stype == t.dtype && factor == 1.0) continue;
     if (t.stype == 0) {
-      if (t.dtype == 0) ga__cn_scale<ga_half, ga_half, float, 8>(t, b, f);
-      else ga__cn_scale<ga_half, ga_float, float, 8>(t, b, f);
+      if (t.dtype == 0) ga__cn_scale<ga_half, ga_half, float>(t, b, f);
+      else ga__cn_scale<ga_half, ga_float, float>(t, b, f);
     } else if (t.stype == 1) {
-      ga__cn_scale<ga_float, ga_float, float, 4>(t, b, f);
+      ga__cn_scale<ga_float, ga_float, float>(t, b, f);
     } else {
-      ga__cn_scale<ga_double, ga_double, double, 2>(t, b, factor);
+      ga__cn_scale<ga_double, ga_double, double>(t, b, factor);
     }
   }
 }

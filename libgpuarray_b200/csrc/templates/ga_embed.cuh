@@ -40,16 +40,8 @@ static __device__ __forceinline__ long long ga__em_row(const ga__em_layout &L, c
   return r < 0 || r >= (long long)L.v ? -2 : r;
 }
 
-template <typename T>
-static __device__ __forceinline__ void ga__em_load(GA_EM_F_T x[GA_EM_E], const char *p, long long col) {
-  if (GA_EM_E == 1) {
-    x[0] = (GA_EM_F_T)ga__lm_get(*reinterpret_cast<const T *>(p));
-  } else {
-    const ga__lm_vec<T, GA_EM_E> q = *reinterpret_cast<const ga__lm_vec<T, GA_EM_E> *>(p);
-#pragma unroll
-    for (int j = 0; j < GA_EM_E; j++) x[j] = (GA_EM_F_T)ga__lm_get(q.v[j]);
-  }
-}
+typedef ga__lm_vec<GA_EM_A_T, GA_EM_E> ga__em_in;
+typedef ga__lm_vec<GA_EM_O_T, GA_EM_E> ga__em_out;
 
 #ifdef GA_EM_BUILD_LOOKUP
 #define GA_EM_U 4
@@ -69,23 +61,21 @@ ga_embed(const __grid_constant__ ga__em_layout L, char *out, const char *table, 
   long long row[GA_EM_U];
 #pragma unroll
   for (int u = 0; u < GA_EM_U; u++) row[u] = t0 + u < L.n ? ga__em_row(L, ids, t0 + u) : -3;
-  GA_EM_F_T x[GA_EM_U][GA_EM_E];
+  ga__em_in q[GA_EM_U];
 #pragma unroll
-  for (int u = 0; u < GA_EM_U; u++) {
-#pragma unroll
-    for (int j = 0; j < GA_EM_E; j++) x[u][j] = 0;
-    if (row[u] >= 0)
-      ga__em_load<GA_EM_A_T>(x[u], table + row[u] * L.v_row + (long long)v * GA_EM_E * L.v_col, L.v_col);
-  }
+  for (int u = 0; u < GA_EM_U; u++)
+    if (row[u] >= 0) q[u] = ga__lm_load<ga__em_in>(table + row[u] * L.v_row + (long long)v * GA_EM_E * L.v_col);
 #pragma unroll
   for (int u = 0; u < GA_EM_U; u++) {
     if (row[u] == -2 && v == 0 && err != nullptr) *err = -1;
     if (row[u] < -1) continue;
-    char *p = out + ga__lm_offset<GA_EM_ND>(t0 + u, L.dims, L.t_str) + (long long)v * GA_EM_E * L.t_col;
-    ga__lm_vec<GA_EM_O_T, GA_EM_E> q;
+    GA_EM_F_T x[GA_EM_E];
+    ga__lm_get<GA_EM_A_T, GA_EM_E>(x, q[u]);
 #pragma unroll
-    for (int j = 0; j < GA_EM_E; j++) ga__lm_put(&q.v[j], x[u][j] * scale);
-    *reinterpret_cast<ga__lm_vec<GA_EM_O_T, GA_EM_E> *>(p) = q;
+    for (int j = 0; j < GA_EM_E; j++) x[j] = row[u] < 0 ? (GA_EM_F_T)0 : x[j] * scale;
+    ga__em_out o;
+    ga__lm_put<GA_EM_O_T, GA_EM_E>(o, x);
+    ga__lm_store(out + ga__lm_offset<GA_EM_ND>(t0 + u, L.dims, L.t_str) + (long long)v * GA_EM_E * L.t_col, o);
   }
 }
 #endif
@@ -122,36 +112,36 @@ static __device__ __forceinline__ void ga__eg_write(const ga__em_layout &L, char
                                                     const GA_EM_F_T acc[GA_EM_E]) {
   const GA_EM_F_T scale = (GA_EM_F_T)L.scale;
   char *p = dtable + (long long)row * L.v_row + (long long)v * GA_EM_E * L.v_col;
-  ga__lm_vec<GA_EM_O_T, GA_EM_E> q;
+  GA_EM_F_T x[GA_EM_E];
+  ga__em_out q;
 #if GA_EM_ACCUMULATE
-  GA_EM_F_T old[GA_EM_E];
-  ga__em_load<GA_EM_O_T>(old, p, L.v_col);
+  ga__lm_get<GA_EM_O_T, GA_EM_E>(x, ga__lm_load<ga__em_out>(p));
 #pragma unroll
-  for (int j = 0; j < GA_EM_E; j++) ga__lm_put(&q.v[j], old[j] + acc[j] * scale);
+  for (int j = 0; j < GA_EM_E; j++) x[j] += acc[j] * scale;
 #else
 #pragma unroll
-  for (int j = 0; j < GA_EM_E; j++) ga__lm_put(&q.v[j], acc[j] * scale);
+  for (int j = 0; j < GA_EM_E; j++) x[j] = acc[j] * scale;
 #endif
-  *reinterpret_cast<ga__lm_vec<GA_EM_O_T, GA_EM_E> *>(p) = q;
+  ga__lm_put<GA_EM_O_T, GA_EM_E>(q, x);
+  ga__lm_store(p, q);
 }
 
 static __device__ __forceinline__ void ga__eg_zero_row(const ga__em_layout &L, char *dtable,
                                                        unsigned long long row, unsigned int v) {
-  ga__lm_vec<GA_EM_O_T, GA_EM_E> q;
+  ga__em_out q;
 #pragma unroll
-  for (int j = 0; j < GA_EM_E; j++) ga__lm_put(&q.v[j], (GA_EM_F_T)0);
-  *reinterpret_cast<ga__lm_vec<GA_EM_O_T, GA_EM_E> *>(dtable + (long long)row * L.v_row +
-                                                     (long long)v * GA_EM_E * L.v_col) = q;
+  for (int j = 0; j < (int)(sizeof(q.w) / sizeof(q.w[0])); j++) q.w[j] = 0;
+  ga__lm_store(dtable + (long long)row * L.v_row + (long long)v * GA_EM_E * L.v_col, q);
 }
 
 static __device__ __forceinline__ void ga__eg_zeros(const ga__em_layout &L, const ga__eg_fill &F,
                                                     unsigned int cta, unsigned int ctas) {
   if (F.bytes > 0) {
     const unsigned long long n = F.bytes / 16, step = (unsigned long long)ctas * blockDim.x;
-    ga__lm_vec<unsigned int, 4> q;
-    q.v[0] = q.v[1] = q.v[2] = q.v[3] = 0;
+    ga__lm_raw<16> q;
+    q.w[0] = q.w[1] = q.w[2] = q.w[3] = 0;
     for (unsigned long long i = (unsigned long long)cta * blockDim.x + threadIdx.x; i < n; i += step)
-      reinterpret_cast<ga__lm_vec<unsigned int, 4> *>(F.p)[i] = q;
+      ga__lm_store(F.p + i * 16, q);
     /* what is left is less than 16 bytes */
     if (cta == 0 && threadIdx.x < F.bytes - n * 16) F.p[n * 16 + threadIdx.x] = 0;
     return;
@@ -209,12 +199,13 @@ ga_eg_count(const __grid_constant__ ga__em_layout L, const __grid_constant__ ga_
 }
 
 /* One pass: every key goes behind all with a smaller digit and, with an equal digit, behind those
- * that stand before it. The first pass takes the ids themselves. */
+ * that stand before it. The first pass takes the ids themselves; the last one leaves the byte
+ * offsets of the tokens' rows of dout, so that the sums need no division. */
 extern "C" __global__ void __launch_bounds__(GA_EG_THREADS)
 ga_eg_scatter(const __grid_constant__ ga__em_layout L, const __grid_constant__ ga__eg_sort S,
               const __grid_constant__ ga__eg_fill F, unsigned int *counts, const char *ids,
               const unsigned int *key_in, const unsigned int *order_in, unsigned int *key,
-              unsigned int *order) {
+              unsigned int *order, long long *off) {
   ga__grid_dependency_sync();
   if (blockIdx.x >= S.tiles) {
     ga__eg_zeros(L, F, blockIdx.x - S.tiles, gridDim.x - S.tiles);
@@ -282,9 +273,12 @@ ga_eg_scatter(const __grid_constant__ ga__em_layout L, const __grid_constant__ g
       if (i < hi) {
         const unsigned int at = cnt[warp][(k[j] >> shift) & (GA_EG_DIGITS - 1)] + rank[j];
         key[at] = k[j];
-        order[at] = o[j];
-        if (S.pass + 1 < S.passes)
+        if (S.pass + 1 == S.passes) {
+          off[at] = ga__lm_offset<GA_EM_ND>(o[j], L.dims, L.t_str);
+        } else {
+          order[at] = o[j];
           atomicAdd(&counts[((S.pass + 1) * GA_EG_DIGITS + ((k[j] >> (shift + GA_EG_BITS)) & (GA_EG_DIGITS - 1))) * S.tiles + at / S.tile], 1u);
+        }
       }
     }
     __syncthreads();
@@ -293,17 +287,21 @@ ga_eg_scatter(const __grid_constant__ ga__em_layout L, const __grid_constant__ g
 
 /* ---- summing ---- */
 #define GA_EG_U 8
+#define GA_EG_J 4
 
 static __device__ __forceinline__ void ga__eg_park(GA_EM_F_T *p, const GA_EM_F_T acc[GA_EM_E]) {
 #pragma unroll
   for (int j = 0; j < GA_EM_E; j++) p[j] = acc[j];
 }
 
-/* Sums sorted tokens [lo, hi) of n at vector position v. head, tail: where the parts of the run
- * that began before lo, and of the one that goes on behind hi, are parked. */
+/* Sums sorted tokens [lo, hi) of n at vector position v; off: their rows of dout. head, tail:
+ * where the parts of the run that began before lo, and of the one that goes on behind hi, are
+ * parked. Both lists may be read up to GA_EG_U - 1 entries beyond hi, by vectors where WIDE (lo a
+ * multiple of GA_EG_U). */
+template <int WIDE>
 static __device__ __forceinline__ void ga__eg_chunk(const ga__em_layout &L, char *dtable,
                                                     const char *dout, const unsigned int *key,
-                                                    const unsigned int *order, unsigned int n,
+                                                    const long long *off, unsigned int n,
                                                     unsigned int lo, unsigned int hi, unsigned int v,
                                                     GA_EM_F_T *head, GA_EM_F_T *tail) {
   const unsigned int none = (unsigned int)L.v;
@@ -314,29 +312,45 @@ static __device__ __forceinline__ void ga__eg_chunk(const ga__em_layout &L, char
   for (int j = 0; j < GA_EM_E; j++) acc[j] = 0;
   const char *col = dout + (long long)v * GA_EM_E * L.t_col;
   for (unsigned int i = lo; i < hi && cur != none; i += GA_EG_U) {
-    unsigned int k[GA_EG_U];
-    ga__lm_vec<GA_EM_A_T, GA_EM_E> x[GA_EG_U];
+    struct alignas(16) {
+      unsigned int v[GA_EG_U];
+    } k;
+    struct alignas(16) {
+      long long v[GA_EG_U];
+    } at;
+    ga__em_in q[GA_EG_U];
+    if (WIDE) {
+      k = *reinterpret_cast<const decltype(k) *>(key + i);
+      at = *reinterpret_cast<const decltype(at) *>(off + i);
+    } else {
 #pragma unroll
-    for (int u = 0; u < GA_EG_U; u++) k[u] = i + u < hi ? key[i + u] : none;
+      for (int u = 0; u < GA_EG_U; u++) {
+        k.v[u] = key[i + u];
+        at.v[u] = off[i + u];
+      }
+    }
 #pragma unroll
-    for (int u = 0; u < GA_EG_U; u++)
-      if (k[u] != none)
-        x[u] = *reinterpret_cast<const ga__lm_vec<GA_EM_A_T, GA_EM_E> *>(
-            col + ga__lm_offset<GA_EM_ND>(order[i + u], L.dims, L.t_str));
+    for (int u = 0; u < GA_EG_U; u++) {
+      if (i + u >= hi) k.v[u] = none;
+      if (k.v[u] != none)
+        q[u] = ga__lm_load<ga__em_in>(col + at.v[u]);
+    }
 #pragma unroll
     for (int u = 0; u < GA_EG_U; u++) {
       if (i + u >= hi) break;
-      if (k[u] != cur) { /* the run ends inside the chunk */
+      if (k.v[u] != cur) { /* the run ends inside the chunk */
         if (open_head) ga__eg_park(head, acc);
         else ga__eg_write(L, dtable, cur, v, acc);
         open_head = 0;
-        cur = k[u];
+        cur = k.v[u];
 #pragma unroll
         for (int j = 0; j < GA_EM_E; j++) acc[j] = 0;
         if (cur == none) break;
       }
+      GA_EM_F_T x[GA_EM_E];
+      ga__lm_get<GA_EM_A_T, GA_EM_E>(x, q[u]);
 #pragma unroll
-      for (int j = 0; j < GA_EM_E; j++) acc[j] += (GA_EM_F_T)ga__lm_get(x[u].v[j]);
+      for (int j = 0; j < GA_EM_E; j++) acc[j] += x[j];
     }
   }
   if (cur == none) return;
@@ -361,24 +375,41 @@ static __device__ __forceinline__ void ga__eg_join_run(const ga__em_layout &L, c
   const GA_EM_F_T *p = part + (2 * (size_t)c + 1) * step;
 #pragma unroll
   for (int j = 0; j < GA_EM_E; j++) acc[j] = p[j];
-  for (unsigned int d = c + 1; d < chunks && key[d * size] == cur; d++) {
-    p = part + 2 * (size_t)d * step;
+  /* GA_EG_J parts are fetched together with the keys that tell whether they belong to the run */
+  for (unsigned int d = c + 1, more = 1; more && d < chunks; d += GA_EG_J) {
+    GA_EM_F_T x[GA_EG_J][GA_EM_E];
+    unsigned int k[GA_EG_J];
 #pragma unroll
-    for (int j = 0; j < GA_EM_E; j++) acc[j] += p[j];
+    for (int u = 0; u < GA_EG_J; u++)
+      if (d + u < chunks) {
+        k[u] = key[(d + u) * size];
+        p = part + 2 * (size_t)(d + u) * step;
+#pragma unroll
+        for (int j = 0; j < GA_EM_E; j++) x[u][j] = p[j];
+      }
+#pragma unroll
+    for (int u = 0; u < GA_EG_J; u++) {
+      if (!more || d + u >= chunks || k[u] != cur) {
+        more = 0;
+        continue;
+      }
+#pragma unroll
+      for (int j = 0; j < GA_EM_E; j++) acc[j] += x[u][j];
+    }
   }
   ga__eg_write(L, dtable, cur, v, acc);
 }
 
 extern "C" __global__ void __launch_bounds__(256)
 ga_eg_sum(const __grid_constant__ ga__em_layout L, char *dtable, const char *dout,
-          const unsigned int *key, const unsigned int *order, GA_EM_F_T *part) {
+          const unsigned int *key, const long long *off, GA_EM_F_T *part) {
   ga__grid_dependency_sync();
   const unsigned int v = blockIdx.y * blockDim.x + threadIdx.x;
   const unsigned int c = blockIdx.x * blockDim.y + threadIdx.y;
   if (v >= L.nv || c >= L.chunks) return;
   const unsigned int n = (unsigned int)L.n, lo = c * L.chunk, hi = n - lo < L.chunk ? n : lo + L.chunk;
   GA_EM_F_T *head = part + (2 * (size_t)c * L.nv + v) * GA_EM_E;
-  ga__eg_chunk(L, dtable, dout, key, order, n, lo, hi, v, head, head + (size_t)L.nv * GA_EM_E);
+  ga__eg_chunk<1>(L, dtable, dout, key, off, n, lo, hi, v, head, head + (size_t)L.nv * GA_EM_E);
 }
 
 extern "C" __global__ void __launch_bounds__(256)
@@ -402,7 +433,8 @@ extern "C" __global__ void __launch_bounds__(256)
 ga_eg_direct(const __grid_constant__ ga__em_layout L, char *dtable, const char *dout,
              const char *ids, int *err) {
   ga__grid_dependency_sync();
-  __shared__ unsigned int row[GA_EG_FEW], token[GA_EG_FEW], key[GA_EG_FEW], order[GA_EG_FEW];
+  __shared__ unsigned int row[GA_EG_FEW], token[GA_EG_FEW], key[GA_EG_FEW + GA_EG_U];
+  __shared__ long long off[GA_EG_FEW + GA_EG_U];
   __shared__ unsigned int found[GA_EG_FEW_WARPS];
   __shared__ GA_EM_F_T part[256 * 2 * GA_EM_E];
   const unsigned int tid = threadIdx.y * blockDim.x + threadIdx.x, lane = tid % 32, warp = tid / 32;
@@ -436,7 +468,7 @@ ga_eg_direct(const __grid_constant__ ga__em_layout L, char *dtable, const char *
     unsigned int at = 0;
     for (unsigned int j = 0; j < m; j++) at += row[j] < k || (row[j] == k && j < i);
     key[at] = k;
-    order[at] = token[i];
+    off[at] = ga__lm_offset<GA_EM_ND>(token[i], L.dims, L.t_str);
   }
   const unsigned int v = blockIdx.y * blockDim.x + threadIdx.x;
 #if !GA_EM_ACCUMULATE
@@ -450,7 +482,7 @@ ga_eg_direct(const __grid_constant__ ga__em_layout L, char *dtable, const char *
   GA_EM_F_T *mine = part + threadIdx.x * GA_EM_E;
   const size_t step = (size_t)blockDim.x * GA_EM_E;
   if (v < L.nv && c < chunks)
-    ga__eg_chunk(L, dtable, dout, key, order, m, c * size, m - c * size < size ? m : (c + 1) * size, v,
+    ga__eg_chunk<0>(L, dtable, dout, key, off, m, c * size, m - c * size < size ? m : (c + 1) * size, v,
                  mine + 2 * c * step, mine + (2 * c + 1) * step);
   __syncthreads();
   if (v < L.nv && c + 1 < chunks) ga__eg_join_run(L, dtable, key, c, size, chunks, v, mine, step);

@@ -6,23 +6,106 @@
 #include "cluda.h"
 #include "ga_lm_ptx.cuh"
 
-/* ---- element <-> arithmetic type ---- */
-static __device__ __forceinline__ float ga__lm_get(ga_half v) { return ga_half2float(v); }
-static __device__ __forceinline__ float ga__lm_get(ga_float v) { return v; }
-static __device__ __forceinline__ double ga__lm_get(ga_double v) { return v; }
-static __device__ __forceinline__ void ga__lm_put(ga_half *p, float v) { *p = ga_float2half(v); }
-/* a double narrows to half through float: two roundings, each to nearest */
-static __device__ __forceinline__ void ga__lm_put(ga_half *p, double v) { *p = ga_float2half((float)v); }
-static __device__ __forceinline__ void ga__lm_put(ga_float *p, float v) { *p = v; }
-static __device__ __forceinline__ void ga__lm_put(ga_float *p, double v) { *p = (float)v; }
-static __device__ __forceinline__ void ga__lm_put(ga_double *p, float v) { *p = (double)v; }
-static __device__ __forceinline__ void ga__lm_put(ga_double *p, double v) { *p = v; }
-
-/* N elements moved by one access (N * sizeof(T) is 1, 2, 4, 8 or 16 bytes, or a multiple of 16) */
-template <typename T, int N>
-struct alignas((sizeof(T) * N) > 16 ? 16 : (sizeof(T) * N)) ga__lm_vec {
-  T v[N];
+/* ---- N elements of type T moved by one access, and as arithmetic type F ----
+ *
+ * They travel as 32-bit words: vectors declared as arrays of 2-byte elements
+ * are taken apart into as many loads or byte moves. */
+template <int BYTES>
+struct alignas(BYTES > 16 ? 16 : BYTES) ga__lm_raw {
+  unsigned int w[BYTES / 4];
 };
+template <>
+struct alignas(2) ga__lm_raw<2> {
+  unsigned short w[1];
+};
+template <typename T, int N>
+using ga__lm_vec = ga__lm_raw<(int)sizeof(T) * N>;
+
+template <typename R>
+static __device__ __forceinline__ R ga__lm_load(const char *p) {
+  return *reinterpret_cast<const R *>(p);
+}
+template <typename R>
+static __device__ __forceinline__ void ga__lm_store(char *p, const R &q) {
+  *reinterpret_cast<R *>(p) = q;
+}
+
+template <typename T>
+struct ga__lm_type;
+template <>
+struct ga__lm_type<ga_half> {
+  template <int N, typename F>
+  static __device__ __forceinline__ void get(F x[N], const ga__lm_raw<2 * N> &q) {
+    if (N == 1) {
+      ga_half h;
+      h.data = (ga_ushort)q.w[0];
+      x[0] = (F)ga_half2float(h);
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < N / 2; j++) {
+      float a, b;
+      ga__unpack_h2(q.w[j], a, b);
+      x[2 * j] = (F)a;
+      x[2 * j + 1] = (F)b;
+    }
+  }
+  /* a double narrows to half through float: two roundings, each to nearest */
+  template <int N, typename F>
+  static __device__ __forceinline__ void put(ga__lm_raw<2 * N> &q, const F x[N]) {
+    if (N == 1) {
+      q.w[0] = ga_float2half((float)x[0]).data;
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < N / 2; j++) q.w[j] = ga__pack_h2((float)x[2 * j], (float)x[2 * j + 1]);
+  }
+};
+template <>
+struct ga__lm_type<ga_float> {
+  template <int N, typename F>
+  static __device__ __forceinline__ void get(F x[N], const ga__lm_raw<4 * N> &q) {
+#pragma unroll
+    for (int j = 0; j < N; j++) x[j] = (F)__uint_as_float(q.w[j]);
+  }
+  template <int N, typename F>
+  static __device__ __forceinline__ void put(ga__lm_raw<4 * N> &q, const F x[N]) {
+#pragma unroll
+    for (int j = 0; j < N; j++) q.w[j] = __float_as_uint((float)x[j]);
+  }
+};
+template <>
+struct ga__lm_type<ga_double> {
+  template <int N, typename F>
+  static __device__ __forceinline__ void get(F x[N], const ga__lm_raw<8 * N> &q) {
+#pragma unroll
+    for (int j = 0; j < N; j++) {
+      const unsigned long long u = (unsigned long long)q.w[2 * j + 1] << 32 | q.w[2 * j];
+      double d;
+      memcpy(&d, &u, 8);
+      x[j] = (F)d;
+    }
+  }
+  template <int N, typename F>
+  static __device__ __forceinline__ void put(ga__lm_raw<8 * N> &q, const F x[N]) {
+#pragma unroll
+    for (int j = 0; j < N; j++) {
+      const double d = (double)x[j];
+      unsigned long long u;
+      memcpy(&u, &d, 8);
+      q.w[2 * j] = (unsigned int)u;
+      q.w[2 * j + 1] = (unsigned int)(u >> 32);
+    }
+  }
+};
+template <typename T, int N, typename F>
+static __device__ __forceinline__ void ga__lm_get(F x[N], const ga__lm_vec<T, N> &q) {
+  ga__lm_type<T>::template get<N, F>(x, q);
+}
+template <typename T, int N, typename F>
+static __device__ __forceinline__ void ga__lm_put(ga__lm_vec<T, N> &q, const F x[N]) {
+  ga__lm_type<T>::template put<N, F>(q, x);
+}
 
 #define GA_LM_MAXD 4
 

@@ -571,29 +571,26 @@ ga_lp_rows(const __grid_constant__ ga__lp_layout L, const char *logits, const ch
 #ifdef GA_LP_BUILD_GRAD
 #define GA_LP_U 4
 
-static __device__ __forceinline__ void ga__lp_store(char *g, long long col, unsigned int i,
+/* Elements i ... of the gradient's row: all of a vector's, or those from `skip` on that the row of
+ * n has. */
+static __device__ __forceinline__ void ga__lp_store(char *g, long long col, long long i, unsigned int skip,
                                                     unsigned int n, const float x[2 * GA_LP_PAIRS],
                                                     int whole) {
-  /* elements i ... of the row (a whole vector, or those of it that are there) */
   typedef ga__lm_vec<GA_LP_G_T, GA_LP_E> vec;
-  if (whole && col == (long long)sizeof(GA_LP_G_T) &&
-      ((size_t)(g + (long long)i * col) & (alignof(vec) - 1)) == 0) {
+  char *p = g + i * col;
+  if (whole && col == (long long)sizeof(GA_LP_G_T) && ((size_t)p & (alignof(vec) - 1)) == 0) {
     vec q;
-#if GA_LP_GTYPE == 0
-    unsigned int w[GA_LP_PAIRS];
-#pragma unroll
-    for (int k = 0; k < GA_LP_PAIRS; k++) w[k] = ga__pack_h2(x[2 * k], x[2 * k + 1]);
-    memcpy(&q, w, sizeof(q));
-#else
-#pragma unroll
-    for (int j = 0; j < GA_LP_E; j++) q.v[j] = x[j];
-#endif
-    *reinterpret_cast<vec *>(g + (long long)i * col) = q;
+    ga__lm_put<GA_LP_G_T, GA_LP_E>(q, x);
+    ga__lm_store(p, q);
     return;
   }
 #pragma unroll
   for (int j = 0; j < GA_LP_E; j++)
-    if (i + j < n) ga__lm_put(reinterpret_cast<GA_LP_G_T *>(g + (long long)(i + j) * col), x[j]);
+    if (j >= (int)skip && i + j < (long long)n) {
+      ga__lm_vec<GA_LP_G_T, 1> q;
+      ga__lm_put<GA_LP_G_T, 1>(q, x + j);
+      ga__lm_store(p + j * col, q);
+    }
 }
 
 /* A thread owns up to GA_LP_U vectors of a row; the row's numbers come from the forward pass, so
@@ -673,16 +670,8 @@ ga_lp_grad(const __grid_constant__ ga__lp_layout L, char *dlogits, const char *l
           if (at == j) x[j] += L.scale * a;
       }
     }
-    const int whole = ga__lp_whole(L, r, w);
-    const unsigned int i0 = w * GA_LP_E < r.skip ? 0 : w * GA_LP_E - r.skip;
-    if (!whole && w * GA_LP_E < r.skip) { /* the row starts inside this vector */
-#pragma unroll
-      for (int j = 0; j < GA_LP_E; j++)
-        if (j >= (int)r.skip && j - r.skip < L.v)
-          ga__lm_put(reinterpret_cast<GA_LP_G_T *>(g + (long long)(j - r.skip) * L.o_col[4]), x[j]);
-    } else {
-      ga__lp_store(g, L.o_col[4], i0, L.v, x, whole);
-    }
+    const long long i = (long long)w * GA_LP_E - r.skip; /* below 0 where the row starts inside the vector */
+    ga__lp_store(g, L.o_col[4], i, i < 0 ? r.skip : 0, L.v, x, ga__lp_whole(L, r, w));
   }
 }
 #endif
