@@ -12,8 +12,9 @@
  *  - Element types are GA_HALF, GA_FLOAT and GA_DOUBLE in any mixture; ids are
  *    GA_INT, GA_UINT, GA_LONG or GA_ULONG. Products and sums are taken in float,
  *    or in double where an array is GA_DOUBLE, and rounded once when written.
+ *    scale is finite as a float.
  *  - Offsets and strides of all arrays are honoured (adjacent row elements on
- *    16-byte boundaries are fastest). A destination must not overlap the other
+ *    16- or 32-byte boundaries are fastest). A destination must not overlap the other
  *    arrays, nor may two of its elements share a place.
  *  - GA_EMBED_PAD: tokens whose id equals `pad` (compared before the rule for
  *    negative ids) give a row of zeros and add nothing to the gradient.

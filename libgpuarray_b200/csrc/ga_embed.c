@@ -1,5 +1,6 @@
 /* Token embedding and its gradient (include/gpuarray/embedding.h; kernels in
  * templates/ga_embed.cuh). */
+#include <math.h>
 #include "private.h"
 
 typedef struct em_layout { /* the templates' ga__em_layout */
@@ -74,7 +75,7 @@ static unsigned vector_width(const GpuArray *in, const GpuArray *out, size_t wid
   for (; e > 1; e /= 2) {
     int ok = width % e == 0;
     for (k = 0; k < 2 && ok; k++) {
-      size_t es = gpuarray_get_elsize(a[k]->typecode), b = es * e > 16 ? 16 : es * e;
+      size_t es = gpuarray_get_elsize(a[k]->typecode), b = es * e;
       if (a[k]->strides[a[k]->nd - 1] != (ssize_t)es) ok = 0;
       if ((a[k]->data->ptr + a[k]->offset) % b != 0) ok = 0;
       for (i = 0; i + 1 < a[k]->nd; i++)
@@ -112,8 +113,9 @@ static int fill(gpucontext *ctx, em_layout *L, ga_lead *lead, const GpuArray *by
 }
 
 /* what both calls refuse before anything is enqueued */
-static int check_call(gpucontext *ctx, const GpuArray *by_row, int flags, int allowed) {
+static int check_call(gpucontext *ctx, const GpuArray *by_row, double scale, int flags, int allowed) {
   if (flags & ~allowed) return ga_err_fmt(ctx->err, GA_INVALID_ERROR, "Unknown flags 0x%x", flags);
+  if (!isfinite((float)scale)) return ga_err_set(ctx->err, GA_VALUE_ERROR, "scale is not a finite float");
   if (by_row->dimensions[0] > 0x7fffffffUL || by_row->dimensions[1] > 0x7fffffffUL)
     return ga_err_set(ctx->err, GA_XLARGE_ERROR, "The table has more than 2^31 - 1 rows or columns");
   if (ISSET(flags, GA_EMBED_CHECK) && ga_lm_capturing(ctx))
@@ -121,6 +123,10 @@ static int check_call(gpucontext *ctx, const GpuArray *by_row, int flags, int al
                       "A checked call waits and cannot be captured into a graph");
   return GA_NO_ERROR;
 }
+
+#define EM_TOKENS 256 /* GA_EM_TOKENS of the template */
+#define EM_MOST 64
+#define EM_CTAS 6     /* CTAs of 256 threads for every SM */
 
 int GpuArray_embed(GpuArray *out, const GpuArray *table, const GpuArray *ids, double scale,
                    ssize_t pad, int flags) {
@@ -141,7 +147,7 @@ int GpuArray_embed(GpuArray *out, const GpuArray *table, const GpuArray *ids, do
       (err = ga_lm_check(ctx, ids, "ids", 0)) != GA_NO_ERROR ||
       (err = check_types(ctx, table, out, ids)) != GA_NO_ERROR ||
       (err = check_shapes(ctx, out, "out", table, ids)) != GA_NO_ERROR ||
-      (err = check_call(ctx, table, flags, GA_EMBED_PAD | GA_EMBED_CHECK)) != GA_NO_ERROR)
+      (err = check_call(ctx, table, scale, flags, GA_EMBED_PAD | GA_EMBED_CHECK)) != GA_NO_ERROR)
     return err;
   e = vector_width(table, out, table->dimensions[1]);
   err = fill(ctx, &L, &lead, out, table, ids, scale, pad, flags, e);
@@ -152,7 +158,11 @@ int GpuArray_embed(GpuArray *out, const GpuArray *table, const GpuArray *ids, do
                      emit, &fn);
   if (err != GA_NO_ERROR) return err;
   ga_lm_geometry(L.nv, block, &grid[1]);
-  blocks = (L.n + block[1] * 4 - 1) / (block[1] * 4);
+  /* Tokens of a group: as many as leave a few groups for every SM, at most EM_TOKENS of a CTA */
+  L.chunk = EM_TOKENS / block[1] < EM_MOST ? EM_TOKENS / block[1] : EM_MOST;
+  while (L.chunk > 1 && (L.n + L.chunk - 1) / L.chunk * grid[1] < (unsigned long long)ctx->num_sms * EM_CTAS * block[1])
+    L.chunk /= 2;
+  blocks = (L.n + (unsigned long long)block[1] * L.chunk - 1) / (block[1] * L.chunk);
   if (blocks > 0x7fffffffULL || grid[1] > 65535)
     return ga_err_set(ctx->err, GA_XLARGE_ERROR, "Too many tokens or too long rows for one call");
   grid[0] = (unsigned)blocks;
@@ -269,7 +279,7 @@ int GpuEmbedGrad_call(GpuEmbedGrad *eg, GpuArray *dtable, const GpuArray *dout, 
       (err = ga_lm_check(ctx, ids, "ids", 0)) != GA_NO_ERROR ||
       (err = check_types(ctx, dout, dtable, ids)) != GA_NO_ERROR ||
       (err = check_shapes(ctx, dout, "dout", dtable, ids)) != GA_NO_ERROR ||
-      (err = check_call(ctx, dtable, flags, GA_EMBED_PAD | GA_EMBED_CHECK | GA_EMBED_ACCUMULATE)) !=
+      (err = check_call(ctx, dtable, scale, flags, GA_EMBED_PAD | GA_EMBED_CHECK | GA_EMBED_ACCUMULATE)) !=
           GA_NO_ERROR)
     return err;
   accumulate = ISSET(flags, GA_EMBED_ACCUMULATE);

@@ -217,9 +217,15 @@ int GpuLogProbs_call(GpuLogProbs *lp, GpuArray *logp, GpuArray *entropy, GpuArra
   v.ent = entropy != NULL;
   v.top = top_logp != NULL || top_ids != NULL;
   e = v.contig ? 16 / (unsigned)es : 1;
-  v.threads = 256;
+  v.threads = getenv("LPT") ? (unsigned)atoi(getenv("LPT")) : 256;
   v.cluster = 1;
-  v.group = !v.top && row_vectors(&L, e) <= 512 ? 32 : 256;
+  v.group = !v.top && row_vectors(&L, e) <= 512 ? 32 : v.threads;
+  /* Few rows: several CTAs share one, as long as the device holds them all and each has at least
+   * one full step of loads. */
+  if (v.group > 32)
+    while (v.cluster < (getenv("LPC") ? (unsigned)atoi(getenv("LPC")) : 8u) && L.rows * v.cluster * 2 * v.threads <= (unsigned long long)ctx->num_sms * 2048 &&
+           row_vectors(&L, e) >= (unsigned long long)v.cluster * 2 * v.threads * 4)
+      v.cluster *= 2;
   err = ga_lm_kernel(ctx, "ga_lp_rows", variant_key(&v), emit, &fn);
   if (err != GA_NO_ERROR) return err;
   block[0] = v.threads;

@@ -44,38 +44,60 @@ typedef ga__lm_vec<GA_EM_A_T, GA_EM_E> ga__em_in;
 typedef ga__lm_vec<GA_EM_O_T, GA_EM_E> ga__em_out;
 
 #ifdef GA_EM_BUILD_LOOKUP
-#define GA_EM_U 4
-/* A thread owns one vector position of the row and GA_EM_U tokens, so that
- * GA_EM_U independent loads are in flight behind one round trip for the ids.
- * Bound by memory: a row is read once per token (tokens that repeat find it in
- * L2) and written once. */
+#define GA_EM_U 8        /* loads of a thread in flight */
+#define GA_EM_TOKENS 256 /* of a CTA's groups at most */
+#define GA_EM_NOWHERE (-0x7fffffffffffffffLL) /* no offset of an array */
+/* A group of threads (blockIdx.x, threadIdx.y) owns L.chunk tokens and one slice of their rows, a
+ * vector position per thread. It first finds the tokens' rows and places together, a token per
+ * thread, so that neither the ids' round trip nor the divisions of their dimensions come with
+ * every vector; then GA_EM_U rows at a time are in flight.
+ * Bound by memory: a row is read once per token (tokens that repeat find it in L2) and written
+ * once. */
 extern "C" __global__ void __launch_bounds__(256)
 ga_embed(const __grid_constant__ ga__em_layout L, char *out, const char *table, const char *ids,
          int *err) {
   ga__grid_dependency_sync();
+  __shared__ long long from[GA_EM_TOKENS], to[GA_EM_TOKENS];
+  const unsigned int tid = threadIdx.y * blockDim.x + threadIdx.x, threads = blockDim.x * blockDim.y;
+  const unsigned long long first = (unsigned long long)blockIdx.x * blockDim.y * L.chunk;
+  const unsigned int here = blockDim.y * L.chunk; /* tokens of all groups of this CTA */
+  for (unsigned int i = tid; i < here; i += threads) {
+    long long row = -2, place = 0;
+    if (first + i < L.n) {
+      row = ga__em_row(L, ids, first + i);
+      place = ga__lm_offset<GA_EM_ND>(first + i, L.dims, L.t_str);
+      if (row == -2 && blockIdx.y == 0 && err != nullptr) *err = -1;
+    }
+    from[i] = row < 0 ? GA_EM_NOWHERE : row * L.v_row; /* padding: nothing is read */
+    to[i] = row < -1 ? GA_EM_NOWHERE : place;          /* no such row: nothing is written */
+  }
+  __syncthreads();
   const unsigned int v = blockIdx.y * blockDim.x + threadIdx.x;
-  const unsigned long long t0 =
-      ((unsigned long long)blockIdx.x * blockDim.y + threadIdx.y) * GA_EM_U;
-  if (v >= L.nv || t0 >= L.n) return;
+  if (v >= L.nv) return;
   const GA_EM_F_T scale = (GA_EM_F_T)L.scale;
-  long long row[GA_EM_U];
+  const char *col = table + (long long)v * GA_EM_E * L.v_col;
+  char *dst = out + (long long)v * GA_EM_E * L.t_col;
+  const unsigned int t1 = (threadIdx.y + 1) * L.chunk;
+  for (unsigned int t = threadIdx.y * L.chunk; t < t1; t += GA_EM_U) {
+    ga__em_in q[GA_EM_U];
 #pragma unroll
-  for (int u = 0; u < GA_EM_U; u++) row[u] = t0 + u < L.n ? ga__em_row(L, ids, t0 + u) : -3;
-  ga__em_in q[GA_EM_U];
+    for (int u = 0; u < GA_EM_U; u++) {
 #pragma unroll
-  for (int u = 0; u < GA_EM_U; u++)
-    if (row[u] >= 0) q[u] = ga__lm_load<ga__em_in>(table + row[u] * L.v_row + (long long)v * GA_EM_E * L.v_col);
+      for (int j = 0; j < (int)(sizeof(q[u].w) / sizeof(q[u].w[0])); j++) q[u].w[j] = 0;
+      if (t + u < t1 && to[t + u] != GA_EM_NOWHERE && from[t + u] != GA_EM_NOWHERE)
+        q[u] = ga__lm_load<ga__em_in>(col + from[t + u]);
+    }
 #pragma unroll
-  for (int u = 0; u < GA_EM_U; u++) {
-    if (row[u] == -2 && v == 0 && err != nullptr) *err = -1;
-    if (row[u] < -1) continue;
-    GA_EM_F_T x[GA_EM_E];
-    ga__lm_get<GA_EM_A_T, GA_EM_E>(x, q[u]);
+    for (int u = 0; u < GA_EM_U; u++) {
+      if (t + u >= t1 || to[t + u] == GA_EM_NOWHERE) continue;
+      GA_EM_F_T x[GA_EM_E];
+      ga__lm_get<GA_EM_A_T, GA_EM_E>(x, q[u]);
 #pragma unroll
-    for (int j = 0; j < GA_EM_E; j++) x[j] = row[u] < 0 ? (GA_EM_F_T)0 : x[j] * scale;
-    ga__em_out o;
-    ga__lm_put<GA_EM_O_T, GA_EM_E>(o, x);
-    ga__lm_store(out + ga__lm_offset<GA_EM_ND>(t0 + u, L.dims, L.t_str) + (long long)v * GA_EM_E * L.t_col, o);
+      for (int j = 0; j < GA_EM_E; j++) x[j] *= scale;
+      ga__em_out o;
+      ga__lm_put<GA_EM_O_T, GA_EM_E>(o, x);
+      ga__lm_store(dst + to[t + u], o);
+    }
   }
 }
 #endif
@@ -107,15 +129,22 @@ struct ga__eg_fill {
   unsigned long long r0, r1; /* rows, otherwise */
 };
 
+static __device__ __forceinline__ char *ga__eg_place(const ga__em_layout &L, char *dtable,
+                                                     unsigned int row, unsigned int v) {
+  return dtable + (long long)row * L.v_row + (long long)v * GA_EM_E * L.v_col;
+}
+
+/* `old`: what the row holds so far, read ahead by the caller (used where it is added to) */
 static __device__ __forceinline__ void ga__eg_write(const ga__em_layout &L, char *dtable,
                                                     unsigned int row, unsigned int v,
-                                                    const GA_EM_F_T acc[GA_EM_E]) {
+                                                    const GA_EM_F_T acc[GA_EM_E],
+                                                    const ga__em_out &old) {
   const GA_EM_F_T scale = (GA_EM_F_T)L.scale;
-  char *p = dtable + (long long)row * L.v_row + (long long)v * GA_EM_E * L.v_col;
+  char *p = ga__eg_place(L, dtable, row, v);
   GA_EM_F_T x[GA_EM_E];
   ga__em_out q;
 #if GA_EM_ACCUMULATE
-  ga__lm_get<GA_EM_O_T, GA_EM_E>(x, ga__lm_load<ga__em_out>(p));
+  ga__lm_get<GA_EM_O_T, GA_EM_E>(x, old);
 #pragma unroll
   for (int j = 0; j < GA_EM_E; j++) x[j] += acc[j] * scale;
 #else
@@ -287,7 +316,7 @@ ga_eg_scatter(const __grid_constant__ ga__em_layout L, const __grid_constant__ g
 
 /* ---- summing ---- */
 #define GA_EG_U 8
-#define GA_EG_J 4
+#define GA_EG_J 8
 
 static __device__ __forceinline__ void ga__eg_park(GA_EM_F_T *p, const GA_EM_F_T acc[GA_EM_E]) {
 #pragma unroll
@@ -310,6 +339,7 @@ static __device__ __forceinline__ void ga__eg_chunk(const ga__em_layout &L, char
   GA_EM_F_T acc[GA_EM_E];
 #pragma unroll
   for (int j = 0; j < GA_EM_E; j++) acc[j] = 0;
+  ga__em_out old; /* of row `cur` */
   const char *col = dout + (long long)v * GA_EM_E * L.t_col;
   for (unsigned int i = lo; i < hi && cur != none; i += GA_EG_U) {
     struct alignas(16) {
@@ -319,6 +349,9 @@ static __device__ __forceinline__ void ga__eg_chunk(const ga__em_layout &L, char
       long long v[GA_EG_U];
     } at;
     ga__em_in q[GA_EG_U];
+#if GA_EM_ACCUMULATE
+    ga__em_out held[GA_EG_U]; /* the rows that the tokens' runs are added to */
+#endif
     if (WIDE) {
       k = *reinterpret_cast<const decltype(k) *>(key + i);
       at = *reinterpret_cast<const decltype(at) *>(off + i);
@@ -335,14 +368,25 @@ static __device__ __forceinline__ void ga__eg_chunk(const ga__em_layout &L, char
       if (k.v[u] != none)
         q[u] = ga__lm_load<ga__em_in>(col + at.v[u]);
     }
+#if GA_EM_ACCUMULATE
+    /* read with the tokens' rows, not when a run ends: once a run, at its first token here */
+#pragma unroll
+    for (int u = 0; u < GA_EG_U; u++)
+      if (k.v[u] != none && (u == 0 ? k.v[u] != cur || i == lo : k.v[u] != k.v[u - 1]))
+        held[u] = ga__lm_load<ga__em_out>(ga__eg_place(L, dtable, k.v[u], v));
+    if (i == lo) old = held[0];
+#endif
 #pragma unroll
     for (int u = 0; u < GA_EG_U; u++) {
       if (i + u >= hi) break;
       if (k.v[u] != cur) { /* the run ends inside the chunk */
         if (open_head) ga__eg_park(head, acc);
-        else ga__eg_write(L, dtable, cur, v, acc);
+        else ga__eg_write(L, dtable, cur, v, acc, old);
         open_head = 0;
         cur = k.v[u];
+#if GA_EM_ACCUMULATE
+        old = held[u];
+#endif
 #pragma unroll
         for (int j = 0; j < GA_EM_E; j++) acc[j] = 0;
         if (cur == none) break;
@@ -356,7 +400,7 @@ static __device__ __forceinline__ void ga__eg_chunk(const ga__em_layout &L, char
   if (cur == none) return;
   if (open_head) ga__eg_park(head, acc);
   else if (hi < n && key[hi] == cur) ga__eg_park(tail, acc);
-  else ga__eg_write(L, dtable, cur, v, acc);
+  else ga__eg_write(L, dtable, cur, v, acc, old);
 }
 
 /* Joins the run that starts in chunk c (tokens c * size ...) and goes on in the next, if there is
@@ -375,6 +419,10 @@ static __device__ __forceinline__ void ga__eg_join_run(const ga__em_layout &L, c
   const GA_EM_F_T *p = part + (2 * (size_t)c + 1) * step;
 #pragma unroll
   for (int j = 0; j < GA_EM_E; j++) acc[j] = p[j];
+  ga__em_out old;
+#if GA_EM_ACCUMULATE
+  old = ga__lm_load<ga__em_out>(ga__eg_place(L, dtable, cur, v));
+#endif
   /* GA_EG_J parts are fetched together with the keys that tell whether they belong to the run */
   for (unsigned int d = c + 1, more = 1; more && d < chunks; d += GA_EG_J) {
     GA_EM_F_T x[GA_EG_J][GA_EM_E];
@@ -397,7 +445,7 @@ static __device__ __forceinline__ void ga__eg_join_run(const ga__em_layout &L, c
       for (int j = 0; j < GA_EM_E; j++) acc[j] += x[u][j];
     }
   }
-  ga__eg_write(L, dtable, cur, v, acc);
+  ga__eg_write(L, dtable, cur, v, acc, old);
 }
 
 extern "C" __global__ void __launch_bounds__(256)

@@ -8,10 +8,10 @@
 
 /* ---- N elements of type T moved by one access, and as arithmetic type F ----
  *
- * They travel as 32-bit words: vectors declared as arrays of 2-byte elements
+ * They travel as 32-bit words, up to 8 of them: vectors declared as arrays of 2-byte elements
  * are taken apart into as many loads or byte moves. */
-template <int BYTES>
-struct alignas(BYTES > 16 ? 16 : BYTES) ga__lm_raw {
+template <int BYTES> /* 4 to 32, a power of two */
+struct alignas(BYTES) ga__lm_raw {
   unsigned int w[BYTES / 4];
 };
 template <>
@@ -23,11 +23,18 @@ using ga__lm_vec = ga__lm_raw<(int)sizeof(T) * N>;
 
 template <typename R>
 static __device__ __forceinline__ R ga__lm_load(const char *p) {
-  return *reinterpret_cast<const R *>(p);
+  if constexpr (sizeof(R) == 32) {
+    R q;
+    ga__ld32(q.w, p);
+    return q;
+  } else {
+    return *reinterpret_cast<const R *>(p);
+  }
 }
 template <typename R>
 static __device__ __forceinline__ void ga__lm_store(char *p, const R &q) {
-  *reinterpret_cast<R *>(p) = q;
+  if constexpr (sizeof(R) == 32) ga__st32(p, q.w);
+  else *reinterpret_cast<R *>(p) = q;
 }
 
 template <typename T>

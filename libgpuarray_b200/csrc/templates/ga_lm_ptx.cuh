@@ -61,6 +61,19 @@ static __device__ __forceinline__ ga__f2 ga__f2_fma(ga__f2 a, ga__f2 b, ga__f2 c
   return r;
 }
 
+/* 32 bytes of global memory by one access (p 32-byte aligned; sm_100) */
+static __device__ __forceinline__ void ga__ld32(unsigned int w[8], const char *p) {
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+               : "l"(p)
+               : "memory");
+}
+static __device__ __forceinline__ void ga__st32(char *p, const unsigned int w[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]),
+               "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
+
 /* Sum over the warp, the same in every lane */
 static __device__ __forceinline__ unsigned int ga__warp_sum_u32(unsigned int v) {
   return __reduce_add_sync(0xffffffffu, v);
@@ -75,10 +88,10 @@ static __device__ __forceinline__ unsigned int ga__cluster_rank() {
 /* Barrier over the cluster's threads in two halves; what each wrote to any CTA's shared
  * memory before its arrival is visible to all after their wait. */
 static __device__ __forceinline__ void ga__cluster_arrive() {
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.arrive.release;" ::: "memory");
 }
 static __device__ __forceinline__ void ga__cluster_wait() {
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
 }
 /* Stores 8 bytes at the place that `p` (this CTA's shared memory) has in CTA `rank`'s. */
 static __device__ __forceinline__ void ga__cluster_put(void *p, unsigned int rank,

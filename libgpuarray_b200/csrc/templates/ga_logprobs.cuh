@@ -222,12 +222,13 @@ struct ga__lp_top_smem {
 /* The `top` largest keys of vectors [v0, v1) of the row, into out[0..32) of this CTA's or the
  * cluster's first CTA's shared memory (0 where there are fewer). All threads of the CTA.
  *
- * `first` is the vector in which this thread's first largest element lies. The thread's largest
- * key bounds its others, so the top-th largest of the threads' largest keys, tau, is a lower
- * bound for the top-th largest of all, and every key above it belongs to one of the `top`
- * threads that reach it: only their vectors are read again. Where NaNs made `first` unusable, or
- * the keys above tau are too many to hold (a row that hides its largest elements in few threads'
- * vectors), tau is found by halving over the whole row. */
+ * `first` is the vector in which this thread's first largest element lies. The largest keys of
+ * 32 disjoint groups of threads are keys of 32 elements, so the top-th largest of them, tau, is a
+ * lower bound for the top-th largest of all, and every key above it belongs to a thread whose
+ * largest reaches it: only those threads' vectors are read again. (Half the groups' largest lie
+ * above tau where 16 alternatives are asked for; the keys above it are then about 20.) Where NaNs
+ * made `first` unusable, or the keys above tau are too many to hold (a row that hides its largest
+ * elements in few threads' vectors), tau is found by halving over the whole row. */
 static __device__ void ga__lp_top(const ga__lp_layout &L, const ga__lp_row &r, unsigned int v0,
                                   unsigned int v1, unsigned int first, int odd, ga__lp_top_smem &S) {
   const unsigned int tid = threadIdx.x;
@@ -243,43 +244,20 @@ static __device__ void ga__lp_top(const ga__lp_layout &L, const ga__lp_row &r, u
     S.ncand = 0;
   }
   __syncthreads();
-  if (tid < 32) {
-    unsigned long long b[GA_LP_THREADS / 32], lo = 0, hi = 0, low;
+  if (tid < 32) { /* the largest of every 32nd thread's, and their order: 32 keys in one warp */
+    unsigned long long high = 0;
 #pragma unroll
     for (int j = 0; j < GA_LP_THREADS / 32; j++) {
-      b[j] = S.best[j * 32 + tid];
-      lo = b[j] > lo ? b[j] : lo;
+      const unsigned long long b = S.best[j * 32 + tid];
+      high = b > high ? b : high;
     }
-    hi = low = lo;
+    unsigned int place = 0;
 #pragma unroll
-    for (int d = 16; d > 0; d /= 2) { /* the lanes' largest: 32 keys, all at least `lo` */
-      const unsigned long long h = __shfl_xor_sync(0xffffffffu, hi, d), l = __shfl_xor_sync(0xffffffffu, low, d);
-      hi = h > hi ? h : hi;
-      low = l < low ? l : low;
+    for (int j = 0; j < 32; j++) {
+      const unsigned long long o = __shfl_sync(0xffffffffu, high, j);
+      place += o > high || (o == high && j < (int)tid); /* equal: both 0, no key */
     }
-    lo = low;
-    hi = hi + 1;
-    /* at least `top` keys reach lo (or all there are, where a lane has none), fewer reach hi; keys
-     * differ, so halving ends with exactly `top` of them */
-    unsigned int at_lo = 0;
-    if (lo == 0) lo = 1;
-#pragma unroll
-    for (int j = 0; j < GA_LP_THREADS / 32; j++) at_lo += b[j] >= lo;
-    at_lo = ga__warp_sum_u32(at_lo);
-    while (at_lo > L.top && hi - lo > 1) {
-      const unsigned long long mid = lo + (hi - lo) / 2;
-      unsigned int c = 0;
-#pragma unroll
-      for (int j = 0; j < GA_LP_THREADS / 32; j++) c += b[j] >= mid;
-      c = ga__warp_sum_u32(c);
-      if (c >= L.top) {
-        lo = mid;
-        at_lo = c;
-      } else {
-        hi = mid;
-      }
-    }
-    if (tid == 0) S.tau = lo;
+    if (place == L.top - 1) S.tau = high > 0 ? high : 1; /* fewer than `top` keys: everything */
   }
   __syncthreads();
   unsigned long long tau = S.tau;
@@ -478,10 +456,19 @@ ga_lp_rows(const __grid_constant__ ga__lp_layout L, const char *logits, const ch
   __shared__ ga__lp_state warps[GA_LP_THREADS / 32];
   if (threadIdx.x % 32 == 0) warps[threadIdx.x / 32] = st;
   __syncthreads();
-  /* every thread merges the warps' states in the same order: the same bits everywhere */
-  st = warps[0];
-#pragma unroll 1
-  for (int i = 1; i < GA_LP_THREADS / 32; i++) st = ga__lp_merge(st, warps[i], c);
+  /* every warp merges the warps' states in the same order: the same bits everywhere */
+  st = warps[threadIdx.x % (GA_LP_THREADS / 32)];
+#pragma unroll
+  for (int d = GA_LP_THREADS / 64; d > 0; d /= 2) {
+    ga__lp_state o;
+    o.m = __shfl_xor_sync(0xffffffffu, st.m, d);
+    o.s = __shfl_xor_sync(0xffffffffu, st.s, d);
+    o.t = __shfl_xor_sync(0xffffffffu, st.t, d);
+    st = ga__lp_merge(st, o, c);
+  }
+  st.m = __shfl_sync(0xffffffffu, st.m, 0);
+  st.s = __shfl_sync(0xffffffffu, st.s, 0);
+  st.t = __shfl_sync(0xffffffffu, st.t, 0);
 #endif
 #if GA_LP_CLUSTER > 1
   ga__cluster_wait(); /* every CTA of the cluster runs */

@@ -746,6 +746,9 @@ def test_embed_refusals(api, ctx):
         refused(api, api.GA_VALUE_ERROR, lambda: call(e(ctx, (3, 8), np.float32), table, ids))
         refused(api, api.GA_VALUE_ERROR, lambda: call(e(ctx, (8,), np.float32), table, ids))
         refused(api, api.GA_VALUE_ERROR, lambda: call(out, e(ctx, (5, 8, 1), np.float32), ids))
+    for bad in (INF, float("nan"), 1e300):
+        refused(api, api.GA_VALUE_ERROR, lambda: api.embed(out, table, ids, scale=bad))
+        refused(api, api.GA_VALUE_ERROR, lambda: op(table, out, ids, scale=bad))
     # a destination whose elements share places, one that may not be written, one beyond its buffer
     shared = api.GpuArray.from_pointer(ctx, out.devptr, (4, 8), np.float32, strides=(0, 4))
     refused(api, api.GA_VALUE_ERROR, lambda: api.embed(shared, table, ids))

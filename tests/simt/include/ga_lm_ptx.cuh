@@ -75,6 +75,14 @@ static inline unsigned int ga__max_h2(unsigned int a, unsigned int b) {
   ga__unpack_h2(b, bl, bh);
   return ga__pack_h2(fmaxf(al, bl), fmaxf(ah, bh));
 }
+static inline void ga__ld32(unsigned int w[8], const char *p) {
+  if ((size_t)p % 32 != 0) abort();
+  memcpy(w, p, 32);
+}
+static inline void ga__st32(char *p, const unsigned int w[8]) {
+  if ((size_t)p % 32 != 0) abort();
+  memcpy(p, w, 32);
+}
 struct ga__f2 {
   float a, b;
 };
