@@ -260,7 +260,7 @@ int GpuClipNorm_call(GpuClipNorm *cn, GpuArray *norm, GpuArray *const *dst,
       at = n;
     }
     if (L->blocks == 0) continue;
-    grid[0] = L->blocks < cn->ctas ? L->blocks : cn->ctas;
+    grid[0] = L->blocks;
     err = ga_launch(ctx, fs, grid, block, 0, params);
     if (err != GA_NO_ERROR) return err;
   }

@@ -14,11 +14,6 @@ typedef struct em_layout { /* the templates' ga__em_layout */
   long long t_col, v_row, v_col;
 } em_layout;
 
-typedef struct eg_fill { /* the templates' ga__eg_fill */
-  CUdeviceptr p;
-  unsigned long long bytes, r0, r1;
-} eg_fill;
-
 typedef struct eg_sort { /* the templates' ga__eg_sort */
   unsigned int n, tiles, tile, passes, pass;
 } eg_sort;
@@ -30,17 +25,20 @@ struct _GpuEmbedGrad {
 
 static int is_real(int tc) { return tc == GA_HALF || tc == GA_FLOAT || tc == GA_DOUBLE; }
 
-/* key: A type | O type << 8 | id type << 16 | E << 24 | ND << 32 | gradient << 40 | accumulate << 41 */
+/* key: A type | O type << 8 | id type << 16 | E << 24 | ND << 32 | gradient << 40 |
+ * accumulate << 41 | C << 48 | rounds of the one-launch sort << 56 */
 static void emit(ga_strb *sb, uint64_t key) {
   const int a = (int)(key & 0xff), o = (int)((key >> 8) & 0xff), i = (int)((key >> 16) & 0xff);
   ga_strb_printf(sb,
                  "#include \"cluda.h\"\n#define %s\n#define GA_EM_A_T %s\n#define GA_EM_O_T %s\n"
                  "#define GA_EM_I_T %s\n#define GA_EM_F_T %s\n#define GA_EM_E %u\n"
-                 "#define GA_EM_ND %u\n#define GA_EM_ACCUMULATE %u\n#include \"ga_embed.cuh\"\n",
+                 "#define GA_EM_ND %u\n#define GA_EM_ACCUMULATE %u\n#define GA_EM_C %u\n"
+                 "#define GA_EG_ROUNDS %u\n#include \"ga_embed.cuh\"\n",
                  (key >> 40) & 1 ? "GA_EM_BUILD_GRAD" : "GA_EM_BUILD_LOOKUP", ga_ctype(a), ga_ctype(o),
                  ga_ctype(i), a == GA_DOUBLE || o == GA_DOUBLE ? "ga_double" : "ga_float",
                  (unsigned)((key >> 24) & 0xff), (unsigned)((key >> 32) & 0xff),
-                 (unsigned)((key >> 41) & 1));
+                 (unsigned)((key >> 41) & 1), (unsigned)((key >> 48) & 0xff),
+                 (key >> 56) ? (unsigned)(key >> 56) : 1u);
 }
 
 static int check_types(gpucontext *ctx, const GpuArray *a, const GpuArray *o, const GpuArray *ids) {
@@ -84,6 +82,12 @@ static unsigned vector_width(const GpuArray *in, const GpuArray *out, size_t wid
     if (ok) break;
   }
   return e;
+}
+
+/* Vectors of a thread: 16 bytes of the array that is read. */
+static unsigned vectors_of_thread(const GpuArray *in, unsigned e) {
+  const unsigned b = (unsigned)gpuarray_get_elsize(in->typecode) * e;
+  return b >= 16 ? 1 : 16 / b;
 }
 
 static int fill(gpucontext *ctx, em_layout *L, ga_lead *lead, const GpuArray *by_token,
@@ -136,7 +140,7 @@ int GpuArray_embed(GpuArray *out, const GpuArray *table, const GpuArray *ids, do
   ga_lead lead;
   CUdeviceptr p_out, p_table, p_ids, p_err;
   void *params[5];
-  unsigned grid[3] = {1, 1, 1}, block[3], e;
+  unsigned grid[3] = {1, 1, 1}, block[3], e, c;
   unsigned long long blocks;
   int err;
 
@@ -150,14 +154,16 @@ int GpuArray_embed(GpuArray *out, const GpuArray *table, const GpuArray *ids, do
       (err = check_call(ctx, table, scale, flags, GA_EMBED_PAD | GA_EMBED_CHECK)) != GA_NO_ERROR)
     return err;
   e = vector_width(table, out, table->dimensions[1]);
+  c = vectors_of_thread(table, e);
   err = fill(ctx, &L, &lead, out, table, ids, scale, pad, flags, e);
   if (err != GA_NO_ERROR || L.n == 0 || L.nv == 0) return err;
   err = ga_lm_kernel(ctx, "ga_embed",
                      (uint64_t)table->typecode | (uint64_t)out->typecode << 8 |
-                         (uint64_t)ids->typecode << 16 | (uint64_t)e << 24 | (uint64_t)lead.nd << 32,
+                         (uint64_t)ids->typecode << 16 | (uint64_t)e << 24 | (uint64_t)lead.nd << 32 |
+                         (uint64_t)c << 48,
                      emit, &fn);
   if (err != GA_NO_ERROR) return err;
-  ga_lm_geometry(L.nv, block, &grid[1]);
+  ga_lm_geometry((L.nv + c - 1) / c, 256, block, &grid[1]);
   /* Tokens of a group: as many as leave a few groups for every SM, at most EM_TOKENS of a CTA */
   L.chunk = EM_TOKENS / block[1] < EM_MOST ? EM_TOKENS / block[1] : EM_MOST;
   while (L.chunk > 1 && (L.n + L.chunk - 1) / L.chunk * grid[1] < (unsigned long long)ctx->num_sms * EM_CTAS * block[1])
@@ -204,16 +210,20 @@ void GpuEmbedGrad_free(GpuEmbedGrad *eg) {
 }
 
 /* constants of the template */
-#define EG_STEP 8        /* GA_EG_U */
+#define EG_STEP 8        /* a multiple of GA_EG_U */
+#define EG_X 64          /* threads along the rows: four or more share the joining of a run */
 #define EG_FEW 512       /* GA_EG_FEW */
 #define EG_TX 32         /* GA_EG_TX */
 #define EG_BITS 9        /* GA_EG_BITS */
 #define EG_THREADS 512   /* GA_EG_THREADS */
 #define EG_ROUND 2048    /* GA_EG_ROUND */
 #define EG_GROUP_THREADS 1024
+#define EG_CLUSTER 8     /* GA_EG_CLUSTER */
+#define EG_MAX_ROUNDS 4  /* of EG_ROUND tokens for each CTA of the cluster */
+#define EG_SHARED (16 * 512 * 4 + 8 * 512 * 4 + 512 * 4 + 16 * 4) /* ga__eg_shared without `keys` */
 #define EG_MAX_TILES 128 /* every sorting CTA reads all tiles' counts: 256 KiB at most */
 
-static int launch_direct(GpuEmbedGrad *eg, em_layout *L, uint64_t key, CUdeviceptr *p_dt,
+static int launch_direct(GpuEmbedGrad *eg, em_layout *L, uint64_t key, unsigned c, CUdeviceptr *p_dt,
                          CUdeviceptr *p_do, CUdeviceptr *p_ids, CUdeviceptr *p_err) {
   gpucontext *ctx = eg->ctx;
   const ga_function *fn;
@@ -222,9 +232,9 @@ static int launch_direct(GpuEmbedGrad *eg, em_layout *L, uint64_t key, CUdevicep
   unsigned long long ctas;
   int err = ga_lm_kernel(ctx, "ga_eg_direct", key, emit, &fn);
   if (err != GA_NO_ERROR) return err;
-  while (block[0] < EG_TX && block[0] < L->nv) block[0] *= 2;
+  while (block[0] < EG_TX && block[0] * c < L->nv) block[0] *= 2;
   block[1] = 256 / block[0];
-  grid[1] = (L->nv + block[0] - 1) / block[0];
+  grid[1] = (L->nv + block[0] * c - 1) / (block[0] * c);
   if (grid[1] > 65535) return ga_err_set(ctx->err, GA_XLARGE_ERROR, "Too long rows for one call");
   /* the slices of all row ranges fill the device about once */
   ctas = (unsigned long long)ctx->num_sms * 8 / grid[1];
@@ -239,38 +249,45 @@ static int launch_direct(GpuEmbedGrad *eg, em_layout *L, uint64_t key, CUdevicep
   return ga_launch(ctx, fn, grid, block, 0, params);
 }
 
-/* The part `i` of `parts` of dtable's rows for the CTAs beside a sorting launch to write zeros to. */
-static void fill_part(eg_fill *F, const em_layout *L, CUdeviceptr p_dt, unsigned e, size_t es,
-                      int accumulate, unsigned i, unsigned parts) {
-  const unsigned long long row = (unsigned long long)L->nv * e * es, all = row * L->v;
-  memset(F, 0, sizeof(*F));
-  F->p = p_dt;
-  if (accumulate) return;
-  if (L->v_col == (long long)es && (L->v_row == (long long)row || L->v == 1) && p_dt % 16 == 0) {
-    const unsigned long long step = (all / parts + 15) / 16 * 16, lo = step * i < all ? step * i : all;
-    F->p = p_dt + lo;
-    F->bytes = i + 1 == parts || all - lo < step ? all - lo : step;
+/* Zeros for all rows of dtable, beside the launch before this one. */
+static int launch_zeros(GpuEmbedGrad *eg, const em_layout *L, uint64_t key, CUdeviceptr *p_dt, unsigned e,
+                        size_t es) {
+  gpucontext *ctx = eg->ctx;
+  const ga_function *fn;
+  const unsigned long long row = (unsigned long long)L->nv * e * es;
+  unsigned long long bytes = 0, ctas;
+  void *params[3];
+  unsigned grid[3] = {1, 1, 1}, block[3] = {EG_THREADS, 1, 1};
+  int err = ga_lm_kernel(ctx, "ga_eg_zero", key, emit, &fn);
+  if (err != GA_NO_ERROR) return err;
+  if (L->v_col == (long long)es && (L->v_row == (long long)row || L->v == 1) && *p_dt % 16 == 0) {
+    bytes = row * L->v;
+    ctas = (bytes + EG_THREADS * 64 - 1) / (EG_THREADS * 64);
   } else {
-    F->r0 = L->v * i / parts;
-    F->r1 = L->v * (i + 1) / parts;
+    ctas = (L->v + EG_THREADS / 32 - 1) / (EG_THREADS / 32);
   }
+  if (ctas > 0x7fffffffULL) return ga_err_set(ctx->err, GA_XLARGE_ERROR, "The table is too large");
+  grid[0] = ctas ? (unsigned)ctas : 1;
+  params[0] = (void *)L;
+  params[1] = p_dt;
+  params[2] = &bytes;
+  return ga_launch(ctx, fn, grid, block, 0, params);
 }
 
 int GpuEmbedGrad_call(GpuEmbedGrad *eg, GpuArray *dtable, const GpuArray *dout, const GpuArray *ids,
                       double scale, ssize_t pad, int flags) {
   gpucontext *ctx;
-  const ga_function *count, *scatter, *sum, *join;
+  const ga_function *sort, *count, *scatter, *sum, *join;
   em_layout L;
   ga_lead lead;
-  eg_fill F;
   eg_sort S;
   CUdeviceptr p_dt, p_do, p_ids, p_err, p_counts, p_key[2], p_order[2], p_off, p_part;
-  void *params[10];
-  unsigned grid[3] = {1, 1, 1}, block[3], flat[3] = {EG_THREADS, 1, 1}, g1[3] = {1, 1, 1}, e, ny, bits, last;
+  void *params[9];
+  unsigned grid[3] = {1, 1, 1}, block[3], flat[3] = {EG_THREADS, 1, 1}, g1[3] = {1, 1, 1}, e, c, ny, bits, last, rounds = 1;
   unsigned long long groups;
   size_t fsize, list, cbytes, es;
   uint64_t key;
-  int err, accumulate;
+  int err, accumulate, one;
 
   if (eg == NULL) return GA_INVALID_ERROR;
   ctx = eg->ctx;
@@ -285,6 +302,7 @@ int GpuEmbedGrad_call(GpuEmbedGrad *eg, GpuArray *dtable, const GpuArray *dout, 
   accumulate = ISSET(flags, GA_EMBED_ACCUMULATE);
   es = gpuarray_get_elsize(dtable->typecode);
   e = vector_width(dout, dtable, dtable->dimensions[1]);
+  c = vectors_of_thread(dout, e);
   err = fill(ctx, &L, &lead, dout, dtable, ids, scale, pad, flags, e);
   if (err != GA_NO_ERROR) return err;
   if (L.n > 0x7fffffffULL)
@@ -292,77 +310,100 @@ int GpuEmbedGrad_call(GpuEmbedGrad *eg, GpuArray *dtable, const GpuArray *dout, 
   if (L.nv == 0 || (L.n == 0 && accumulate)) return GA_NO_ERROR;
 
   key = (uint64_t)dout->typecode | (uint64_t)dtable->typecode << 8 | (uint64_t)ids->typecode << 16 |
-        (uint64_t)e << 24 | (uint64_t)lead.nd << 32 | (uint64_t)1 << 40 | (uint64_t)accumulate << 41;
+        (uint64_t)e << 24 | (uint64_t)lead.nd << 32 | (uint64_t)1 << 40 | (uint64_t)accumulate << 41 |
+        (uint64_t)c << 48;
   p_dt = dtable->data->ptr + dtable->offset;
   p_do = dout->data->ptr + dout->offset;
   p_ids = ids->data->ptr + ids->offset;
   p_err = ISSET(flags, GA_EMBED_CHECK) ? ga_lm_err_word(ctx) : 0;
 
   if (L.n <= EG_FEW && L.v > 0) {
-    err = launch_direct(eg, &L, key, &p_dt, &p_do, &p_ids, &p_err);
+    err = launch_direct(eg, &L, key, c, &p_dt, &p_do, &p_ids, &p_err);
     if (err == GA_NO_ERROR && ISSET(flags, GA_EMBED_CHECK))
       err = ga_lm_err_take(ctx, "A token id is outside the table");
     return err;
   }
 
-  if ((err = ga_lm_kernel(ctx, "ga_eg_count", key, emit, &count)) != GA_NO_ERROR ||
-      (err = ga_lm_kernel(ctx, "ga_eg_scatter", key, emit, &scatter)) != GA_NO_ERROR ||
-      (err = ga_lm_kernel(ctx, "ga_eg_sum", key, emit, &sum)) != GA_NO_ERROR ||
+  if ((err = ga_lm_kernel(ctx, "ga_eg_sum", key, emit, &sum)) != GA_NO_ERROR ||
       (err = ga_lm_kernel(ctx, "ga_eg_join", key, emit, &join)) != GA_NO_ERROR)
     return err;
 
-  ga_lm_geometry(L.nv, block, &ny);
+  ga_lm_geometry((L.nv + c - 1) / c, EG_X, block, &ny);
   if (ny > 65535) return ga_err_set(ctx->err, GA_XLARGE_ERROR, "Too long rows for one call");
   grid[1] = ny;
   /* Chunks: threads for half the device, which with EG_STEP loads of a thread in flight keep the
    * memory busy; more and shorter ones only leave more parts to join. None shorter than one step. */
-  groups = (unsigned long long)ctx->num_sms * EG_GROUP_THREADS / ((unsigned long long)block[0] * ny);
+  groups = (unsigned long long)ctx->num_sms * (getenv("EGT") ? (unsigned)atoi(getenv("EGT")) : EG_GROUP_THREADS) / ((unsigned long long)block[0] * ny);
   if (groups == 0) groups = 1;
   L.chunk = (unsigned)((L.n + groups - 1) / groups);
   L.chunk = (L.chunk + EG_STEP - 1) / EG_STEP * EG_STEP;
   L.chunks = (unsigned)((L.n + L.chunk - 1) / L.chunk);
 
   S.n = (unsigned)L.n;
-  S.tiles = (unsigned)((L.n + EG_ROUND - 1) / EG_ROUND);
-  if (S.tiles > EG_MAX_TILES) S.tiles = EG_MAX_TILES;
-  S.tile = (unsigned)(((L.n + S.tiles - 1) / S.tiles + EG_ROUND - 1) / EG_ROUND * EG_ROUND);
-  S.tiles = (unsigned)((L.n + S.tile - 1) / S.tile);
   for (bits = 1; bits < 32 && (L.v >> bits) != 0; bits++) {} /* keys go up to V */
   S.passes = (bits + EG_BITS - 1) / EG_BITS;
+  S.pass = 0;
+  one = L.n <= (unsigned long long)EG_CLUSTER * EG_ROUND * EG_MAX_ROUNDS;
+  if (one) {
+    S.tiles = EG_CLUSTER;
+    for (rounds = 1; (unsigned long long)EG_CLUSTER * EG_ROUND * rounds < L.n; rounds *= 2) {}
+    S.tile = EG_ROUND * rounds;
+  } else {
+    S.tiles = (unsigned)((L.n + EG_ROUND - 1) / EG_ROUND);
+    if (S.tiles > EG_MAX_TILES) S.tiles = EG_MAX_TILES;
+    S.tile = (unsigned)(((L.n + S.tiles - 1) / S.tiles + EG_ROUND - 1) / EG_ROUND * EG_ROUND);
+    S.tiles = (unsigned)((L.n + S.tile - 1) / S.tile);
+  }
 
   fsize = dout->typecode == GA_DOUBLE || dtable->typecode == GA_DOUBLE ? 8 : 4;
   list = ((size_t)(L.n + EG_STEP) * 4 + 511) / 512 * 512;
-  cbytes = (size_t)S.passes * EG_THREADS * S.tiles * 4;
-  err = ga_workspace_need(ctx, &eg->ws, cbytes + 6 * list + 2 * (size_t)L.chunks * L.nv * e * fsize);
+  cbytes = one ? 0 : (size_t)S.passes * EG_THREADS * S.tiles * 4;
+  /* the sorted keys and offsets; for many tokens the counts and the lists between the passes */
+  err = ga_workspace_need(ctx, &eg->ws, 3 * list + (one ? 0 : cbytes + 3 * list) +
+                                            2 * (size_t)L.chunks * ny * block[0] * c * e * fsize);
   if (err != GA_NO_ERROR) return err;
-  p_counts = eg->ws.cur->ptr;
-  p_key[0] = p_counts + cbytes;
-  p_order[0] = p_key[0] + list;
-  p_key[1] = p_order[0] + list;
-  p_order[1] = p_key[1] + list;
-  p_off = p_order[1] + list;
+  p_key[0] = eg->ws.cur->ptr;
+  p_off = p_key[0] + list;
   p_part = p_off + 2 * list;
+  if (!one) {
+    p_key[1] = p_part;
+    p_order[0] = p_key[1] + list;
+    p_order[1] = p_order[0] + list;
+    p_counts = p_order[1] + list;
+    p_part = p_counts + cbytes;
+  }
 
-  /* the CTAs that write zeros: what the device holds beside the sorting ones */
-  g1[0] = S.tiles + (accumulate ? 0 : ctx->num_sms * 4 > S.tiles + ctx->num_sms ? ctx->num_sms * 4 - S.tiles : ctx->num_sms);
   params[0] = &L;
   params[1] = &S;
-  params[2] = &F;
-  params[3] = &p_counts;
-  params[4] = &p_ids;
-  params[5] = &p_err;
-  fill_part(&F, &L, p_dt, e, es, accumulate, 0, S.passes + 1);
-  err = ga_launch(ctx, count, g1, flat, 0, params);
-  for (S.pass = 0; S.pass < S.passes && err == GA_NO_ERROR; S.pass++) {
-    fill_part(&F, &L, p_dt, e, es, accumulate, S.pass + 1, S.passes + 1);
-    params[5] = &p_key[1 - S.pass % 2];
-    params[6] = &p_order[1 - S.pass % 2];
-    params[7] = &p_key[S.pass % 2];
-    params[8] = &p_order[S.pass % 2];
-    params[9] = &p_off;
-    err = ga_launch(ctx, scatter, g1, flat, 0, params);
+  g1[0] = S.tiles;
+  if (one) {
+    if ((err = ga_lm_kernel(ctx, "ga_eg_sort_all", key | (uint64_t)rounds << 56, emit, &sort)) != GA_NO_ERROR)
+      return err;
+    params[2] = &p_ids;
+    params[3] = &p_key[0];
+    params[4] = &p_off;
+    params[5] = &p_err;
+    last = 0;
+    err = ga_launch(ctx, sort, g1, flat, EG_SHARED + (size_t)S.tile * 8, params);
+  } else {
+    if ((err = ga_lm_kernel(ctx, "ga_eg_count", key, emit, &count)) != GA_NO_ERROR ||
+        (err = ga_lm_kernel(ctx, "ga_eg_scatter", key, emit, &scatter)) != GA_NO_ERROR)
+      return err;
+    params[2] = &p_counts;
+    params[3] = &p_ids;
+    params[4] = &p_err;
+    err = ga_launch(ctx, count, g1, flat, 0, params);
+    last = (S.passes - 1) % 2;
+    for (; S.pass < S.passes && err == GA_NO_ERROR; S.pass++) {
+      params[4] = &p_key[1 - S.pass % 2];
+      params[5] = &p_order[1 - S.pass % 2];
+      params[6] = &p_key[S.pass % 2];
+      params[7] = &p_order[S.pass % 2];
+      params[8] = &p_off;
+      err = ga_launch(ctx, scatter, g1, flat, 0, params);
+    }
   }
-  last = (S.passes - 1) % 2;
+  if (err == GA_NO_ERROR && !accumulate && L.v > 0) err = launch_zeros(eg, &L, key, &p_dt, e, es);
 
   if (err == GA_NO_ERROR) {
     grid[0] = (L.chunks + block[1] - 1) / block[1];
@@ -376,6 +417,7 @@ int GpuEmbedGrad_call(GpuEmbedGrad *eg, GpuArray *dtable, const GpuArray *dout, 
   if (err == GA_NO_ERROR && L.chunks > 1) {
     params[2] = &p_key[last];
     params[3] = &p_part;
+    grid[0] = L.chunks - 1;
     err = ga_launch(ctx, join, grid, block, 0, params);
   }
   if (err == GA_NO_ERROR && ISSET(flags, GA_EMBED_CHECK))

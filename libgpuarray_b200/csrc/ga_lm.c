@@ -181,8 +181,8 @@ int ga_lm_err_take(gpucontext *ctx, const char *what) {
 
 /* ----------------------------------------------------------------- geometry */
 
-void ga_lm_geometry(unsigned long long nv, unsigned block[3], unsigned int *ny) {
-  unsigned long long y = (nv + 255) / 256, x;
+void ga_lm_geometry(unsigned long long nv, unsigned most, unsigned block[3], unsigned int *ny) {
+  unsigned long long y = (nv + most - 1) / most, x;
   if (nv == 0) y = 1;
   x = (nv + y - 1) / y;
   if (x > 16) x = (x + 31) / 32 * 32;

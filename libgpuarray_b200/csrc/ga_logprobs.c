@@ -242,6 +242,7 @@ int GpuLogProbs_call(GpuLogProbs *lp, GpuArray *logp, GpuArray *entropy, GpuArra
   return err;
 }
 
+#define LP_CTAS 16 /* of 256 threads, 4 of which an SM holds at once */
 #define LP_U 4 /* vectors of a thread in the gradient kernel: GA_LP_U of the template */
 
 int GpuLogProbs_grad(GpuLogProbs *lp, GpuArray *dlogits, const GpuArray *logits,
@@ -298,8 +299,13 @@ int GpuLogProbs_grad(GpuLogProbs *lp, GpuArray *dlogits, const GpuArray *logits,
   e = v.contig ? 16 / (unsigned)es : 1;
   err = ga_lm_kernel(ctx, "ga_lp_grad", variant_key(&v), emit, &fn);
   if (err != GA_NO_ERROR) return err;
-  ga_lm_geometry((row_vectors(&L, e) + LP_U - 1) / LP_U, block, &grid[1]);
+  ga_lm_geometry((row_vectors(&L, e) + LP_U - 1) / LP_U, 256, block, &grid[1]);
   grid[0] = (unsigned)((L.rows + block[1] - 1) / block[1]);
+  /* A CTA takes as many steps along its row as leave LP_CTAS for every SM. */
+  {
+    unsigned long long want = ((unsigned long long)ctx->num_sms * (getenv("LPG") ? (unsigned)atoi(getenv("LPG")) : LP_CTAS) + grid[0] - 1) / grid[0];
+    if (grid[1] > want) grid[1] = (unsigned)want;
+  }
   p[0] = at(dlogits);
   p[1] = at(logits);
   p[2] = at(targets);

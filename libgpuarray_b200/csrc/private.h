@@ -309,9 +309,9 @@ GA_HIDDEN void ga_workspace_free(ga_workspace *ws);
 GA_HIDDEN CUdeviceptr ga_lm_err_word(gpucontext *ctx);
 /* Waits for the stream; GA_VALUE_ERROR (and the word back at zero) if it was set. */
 GA_HIDDEN int ga_lm_err_take(gpucontext *ctx, const char *what);
-/* Threads along vectors and rows of a block for rows of nv vectors: 256 threads, whole warps
- * along the vectors where there are that many; *ny blocks cover the row. */
-GA_HIDDEN void ga_lm_geometry(unsigned long long nv, unsigned block[3], unsigned int *ny);
+/* Threads along vectors and rows of a block for rows of nv vectors: 256 threads, at most `most`
+ * (32 to 256) along the vectors, whole warps where there are that many; *ny blocks cover the row. */
+GA_HIDDEN void ga_lm_geometry(unsigned long long nv, unsigned most, unsigned block[3], unsigned int *ny);
 
 /* Combination of per-GPU partial results through peer memory (ga_comm.c). */
 struct _gpucomm;

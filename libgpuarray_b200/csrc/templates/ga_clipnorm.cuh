@@ -219,23 +219,22 @@ static __device__ __forceinline__ void ga__cn_scale(const ga__cn_item &t, unsign
   }
 }
 
+/* A block for each CTA, not a fixed share of the blocks: the SMs are not equally fast. */
 extern "C" __global__ void __launch_bounds__(GA_CN_THREADS)
 ga_cn_scale(const __grid_constant__ ga__cn_layout L, const ga__cn_result *res) {
   ga__grid_dependency_sync();
   const double factor = __ldcg(&res->factor);
   const float f = (float)factor;
-  for (unsigned int i = blockIdx.x; i < L.blocks; i += gridDim.x) {
-    const unsigned int b = L.blocks - 1 - i;
-    const ga__cn_item &t = L.item[ga__cn_find(L, b)];
-    /* an array that stays where it is and is multiplied by one is what it was */
-    if (t.dst == t.src && t.stype == t.dtype && factor == 1.0) continue;
-    if (t.stype == 0) {
-      if (t.dtype == 0) ga__cn_scale<ga_half, ga_half, float>(t, b, f);
-      else ga__cn_scale<ga_half, ga_float, float>(t, b, f);
-    } else if (t.stype == 1) {
-      ga__cn_scale<ga_float, ga_float, float>(t, b, f);
-    } else {
-      ga__cn_scale<ga_double, ga_double, double>(t, b, factor);
-    }
+  const unsigned int b = L.blocks - 1 - blockIdx.x;
+  const ga__cn_item &t = L.item[ga__cn_find(L, b)];
+  /* an array that stays where it is and is multiplied by one is what it was */
+  if (t.dst == t.src && t.stype == t.dtype && factor == 1.0) return;
+  if (t.stype == 0) {
+    if (t.dtype == 0) ga__cn_scale<ga_half, ga_half, float>(t, b, f);
+    else ga__cn_scale<ga_half, ga_float, float>(t, b, f);
+  } else if (t.stype == 1) {
+    ga__cn_scale<ga_float, ga_float, float>(t, b, f);
+  } else {
+    ga__cn_scale<ga_double, ga_double, double>(t, b, factor);
   }
 }

@@ -9,7 +9,8 @@
  *
  * Defines needed: GA_EM_BUILD_LOOKUP or GA_EM_BUILD_GRAD, GA_EM_A_T (table, or
  * dout), GA_EM_O_T (out, or dtable), GA_EM_I_T (ids), GA_EM_F_T (arithmetic),
- * GA_EM_E (elements of a vector), GA_EM_ND (leading dimensions). */
+ * GA_EM_E (elements of a vector), GA_EM_C (vectors of a thread), GA_EM_ND
+ * (leading dimensions). */
 #include "ga_lm_common.cuh"
 
 struct ga__em_layout {
@@ -40,8 +41,65 @@ static __device__ __forceinline__ long long ga__em_row(const ga__em_layout &L, c
   return r < 0 || r >= (long long)L.v ? -2 : r;
 }
 
-typedef ga__lm_vec<GA_EM_A_T, GA_EM_E> ga__em_in;
-typedef ga__lm_vec<GA_EM_O_T, GA_EM_E> ga__em_out;
+/* A thread's part of a row: GA_EM_C vectors of GA_EM_E elements, blockDim.x vectors apart. Rows
+ * that start off the boundary of a 16-byte vector are moved in narrower ones; several of them in
+ * one thread keep as many bytes in flight. */
+#define GA_EM_N (GA_EM_E * GA_EM_C)
+typedef ga__lm_vec<GA_EM_A_T, GA_EM_E> ga__em_in1;
+typedef ga__lm_vec<GA_EM_O_T, GA_EM_E> ga__em_out1;
+struct ga__em_in {
+  ga__em_in1 c[GA_EM_C];
+};
+struct ga__em_out {
+  ga__em_out1 c[GA_EM_C];
+};
+struct ga__em_pos {
+  unsigned int v; /* the first vector's position; some of the others may lie beyond the row */
+  unsigned int nv;
+};
+static __device__ __forceinline__ ga__em_pos ga__em_here(const ga__em_layout &L) {
+  ga__em_pos p;
+  p.v = blockIdx.y * blockDim.x * GA_EM_C + threadIdx.x;
+  p.nv = L.nv;
+  return p;
+}
+template <typename V, typename R>
+static __device__ __forceinline__ V ga__em_read(const char *row, long long col, ga__em_pos p) {
+  V q;
+#pragma unroll
+  for (int c = 0; c < GA_EM_C; c++) {
+    const unsigned int v = p.v + c * blockDim.x;
+    if (c == 0 || v < p.nv)
+      q.c[c] = ga__lm_load<R>(row + (long long)v * GA_EM_E * col);
+  }
+  return q;
+}
+static __device__ __forceinline__ void ga__em_write(char *row, long long col, ga__em_pos p,
+                                                    const ga__em_out &q) {
+#pragma unroll
+  for (int c = 0; c < GA_EM_C; c++) {
+    const unsigned int v = p.v + c * blockDim.x;
+    if (c == 0 || v < p.nv) ga__lm_store(row + (long long)v * GA_EM_E * col, q.c[c]);
+  }
+}
+template <typename T, typename V>
+static __device__ __forceinline__ void ga__em_get(GA_EM_F_T x[GA_EM_N], const V &q) {
+#pragma unroll
+  for (int c = 0; c < GA_EM_C; c++) ga__lm_get<T, GA_EM_E>(x + c * GA_EM_E, q.c[c]);
+}
+static __device__ __forceinline__ void ga__em_put(ga__em_out &q, const GA_EM_F_T x[GA_EM_N]) {
+#pragma unroll
+  for (int c = 0; c < GA_EM_C; c++) ga__lm_put<GA_EM_O_T, GA_EM_E>(q.c[c], x + c * GA_EM_E);
+}
+template <typename V>
+static __device__ __forceinline__ V ga__em_zero() {
+  V q;
+#pragma unroll
+  for (int c = 0; c < GA_EM_C; c++)
+#pragma unroll
+    for (int j = 0; j < (int)(sizeof(q.c[c].w) / sizeof(q.c[c].w[0])); j++) q.c[c].w[j] = 0;
+  return q;
+}
 
 #ifdef GA_EM_BUILD_LOOKUP
 #define GA_EM_U 8        /* loads of a thread in flight */
@@ -72,37 +130,37 @@ ga_embed(const __grid_constant__ ga__em_layout L, char *out, const char *table, 
     to[i] = row < -1 ? GA_EM_NOWHERE : place;          /* no such row: nothing is written */
   }
   __syncthreads();
-  const unsigned int v = blockIdx.y * blockDim.x + threadIdx.x;
-  if (v >= L.nv) return;
+  const ga__em_pos at = ga__em_here(L);
+  if (at.v >= L.nv) return;
   const GA_EM_F_T scale = (GA_EM_F_T)L.scale;
-  const char *col = table + (long long)v * GA_EM_E * L.v_col;
-  char *dst = out + (long long)v * GA_EM_E * L.t_col;
   const unsigned int t1 = (threadIdx.y + 1) * L.chunk;
   for (unsigned int t = threadIdx.y * L.chunk; t < t1; t += GA_EM_U) {
     ga__em_in q[GA_EM_U];
 #pragma unroll
     for (int u = 0; u < GA_EM_U; u++) {
-#pragma unroll
-      for (int j = 0; j < (int)(sizeof(q[u].w) / sizeof(q[u].w[0])); j++) q[u].w[j] = 0;
+      q[u] = ga__em_zero<ga__em_in>();
       if (t + u < t1 && to[t + u] != GA_EM_NOWHERE && from[t + u] != GA_EM_NOWHERE)
-        q[u] = ga__lm_load<ga__em_in>(col + from[t + u]);
+        q[u] = ga__em_read<ga__em_in, ga__em_in1>(table + from[t + u], L.v_col, at);
     }
 #pragma unroll
     for (int u = 0; u < GA_EM_U; u++) {
       if (t + u >= t1 || to[t + u] == GA_EM_NOWHERE) continue;
-      GA_EM_F_T x[GA_EM_E];
-      ga__lm_get<GA_EM_A_T, GA_EM_E>(x, q[u]);
+      GA_EM_F_T x[GA_EM_N];
+      ga__em_get<GA_EM_A_T>(x, q[u]);
 #pragma unroll
-      for (int j = 0; j < GA_EM_E; j++) x[j] *= scale;
+      for (int j = 0; j < GA_EM_N; j++) x[j] *= scale;
       ga__em_out o;
-      ga__lm_put<GA_EM_O_T, GA_EM_E>(o, x);
-      ga__lm_store(dst + to[t + u], o);
+      ga__em_put(o, x);
+      ga__em_write(out + to[t + u], L.t_col, at, o);
     }
   }
 }
 #endif
 
 #ifdef GA_EM_BUILD_GRAD
+#ifndef GA_EG_ROUNDS
+#define GA_EG_ROUNDS 1
+#endif
 /* The gradient is a sum over SORTED tokens, in launches that depend on nothing
  * but the ids' values, so that the result is the same bits every time.
  *
@@ -110,11 +168,11 @@ ga_embed(const __grid_constant__ ga__em_layout L, char *out, const char *table, 
  * their vectors, picks its tokens from all ids, sorts them in shared memory,
  * writes zeros and sums.
  *
- * Many tokens: the tokens are sorted by row and, within a row, by token (a
- * radix sort of GA_EG_BITS bits a pass: ga_eg_count, then ga_eg_scatter for
- * each pass, which also counts for the next). Tokens that contribute nothing
- * get the key V and go last. The CTAs beyond the sort's write the zeros of the
- * rows, a part of them in each launch, so that the sort hides behind them.
+ * More tokens: they are sorted by row and, within a row, by token (a radix sort
+ * of GA_EG_BITS bits a pass), up to 65536 of them by one cluster in one launch
+ * (ga_eg_sort_all), beyond by ga_eg_count and a ga_eg_scatter for each pass,
+ * which also counts for the next. Tokens that contribute nothing get the key V
+ * and go last. ga_eg_zero writes zeros to all rows beside the sort.
  * Then ga_eg_sum: the sorted tokens are cut into equal chunks; a group of
  * threads sums a chunk's rows, one vector position per thread. A run of equal
  * keys that lies inside the chunk is finished and written; the parts of runs
@@ -122,63 +180,59 @@ ga_embed(const __grid_constant__ ga__em_layout L, char *out, const char *table, 
  * group of the chunk in which a crossing run starts adds its parts in order
  * and writes the row. */
 
-/* zeros for a part of dtable: flat bytes where its rows are adjacent, else row by row */
-struct ga__eg_fill {
-  char *p;
-  unsigned long long bytes; /* > 0: flat */
-  unsigned long long r0, r1; /* rows, otherwise */
-};
-
-static __device__ __forceinline__ char *ga__eg_place(const ga__em_layout &L, char *dtable,
-                                                     unsigned int row, unsigned int v) {
-  return dtable + (long long)row * L.v_row + (long long)v * GA_EM_E * L.v_col;
-}
-
 /* `old`: what the row holds so far, read ahead by the caller (used where it is added to) */
 static __device__ __forceinline__ void ga__eg_write(const ga__em_layout &L, char *dtable,
-                                                    unsigned int row, unsigned int v,
-                                                    const GA_EM_F_T acc[GA_EM_E],
+                                                    unsigned int row, ga__em_pos at,
+                                                    const GA_EM_F_T acc[GA_EM_N],
                                                     const ga__em_out &old) {
   const GA_EM_F_T scale = (GA_EM_F_T)L.scale;
-  char *p = ga__eg_place(L, dtable, row, v);
-  GA_EM_F_T x[GA_EM_E];
+  GA_EM_F_T x[GA_EM_N];
   ga__em_out q;
 #if GA_EM_ACCUMULATE
-  ga__lm_get<GA_EM_O_T, GA_EM_E>(x, old);
+  ga__em_get<GA_EM_O_T>(x, old);
 #pragma unroll
-  for (int j = 0; j < GA_EM_E; j++) x[j] += acc[j] * scale;
+  for (int j = 0; j < GA_EM_N; j++) x[j] += acc[j] * scale;
 #else
 #pragma unroll
-  for (int j = 0; j < GA_EM_E; j++) x[j] = acc[j] * scale;
+  for (int j = 0; j < GA_EM_N; j++) x[j] = acc[j] * scale;
 #endif
-  ga__lm_put<GA_EM_O_T, GA_EM_E>(q, x);
-  ga__lm_store(p, q);
+  ga__em_put(q, x);
+  ga__em_write(dtable + (long long)row * L.v_row, L.v_col, at, q);
+}
+static __device__ __forceinline__ ga__em_out ga__eg_held(const ga__em_layout &L, const char *dtable,
+                                                         unsigned int row, ga__em_pos at) {
+  return ga__em_read<ga__em_out, ga__em_out1>(dtable + (long long)row * L.v_row, L.v_col, at);
 }
 
-static __device__ __forceinline__ void ga__eg_zero_row(const ga__em_layout &L, char *dtable,
-                                                       unsigned long long row, unsigned int v) {
-  ga__em_out q;
-#pragma unroll
-  for (int j = 0; j < (int)(sizeof(q.w) / sizeof(q.w[0])); j++) q.w[j] = 0;
-  ga__lm_store(dtable + (long long)row * L.v_row + (long long)v * GA_EM_E * L.v_col, q);
-}
-
-static __device__ __forceinline__ void ga__eg_zeros(const ga__em_layout &L, const ga__eg_fill &F,
-                                                    unsigned int cta, unsigned int ctas) {
-  if (F.bytes > 0) {
-    const unsigned long long n = F.bytes / 16, step = (unsigned long long)ctas * blockDim.x;
+/* Zeros for the rows, `bytes` of them where the rows are adjacent (0: row by row). One tile or
+ * group of rows for each CTA: handed out one after the other they are written at 7.3 TB/s, by
+ * CTAs that each walk a fixed share of the rows at 6.2 (the SMs are not equally fast).
+ *
+ * It runs beside the launch before it, whose CTAs sort: it does not wait for that one, which
+ * itself released its successor only after waiting for all that came before. Its last CTA stays
+ * until the sort is complete, so that whatever waits for this launch has waited for both. */
+#define GA_EG_ZERO 512
+extern "C" __global__ void __launch_bounds__(GA_EG_ZERO)
+ga_eg_zero(const __grid_constant__ ga__em_layout L, char *dtable, unsigned long long bytes) {
+  ga__grid_dependency_release();
+  if (bytes > 0) {
     ga__lm_raw<16> q;
     q.w[0] = q.w[1] = q.w[2] = q.w[3] = 0;
-    for (unsigned long long i = (unsigned long long)cta * blockDim.x + threadIdx.x; i < n; i += step)
-      ga__lm_store(F.p + i * 16, q);
+    const unsigned long long at = ((unsigned long long)blockIdx.x * 4 * GA_EG_ZERO + threadIdx.x) * 16;
+#pragma unroll
+    for (int u = 0; u < 4; u++)
+      if (at + u * GA_EG_ZERO * 16 + 16 <= bytes) ga__lm_store(dtable + at + u * GA_EG_ZERO * 16, q);
     /* what is left is less than 16 bytes */
-    if (cta == 0 && threadIdx.x < F.bytes - n * 16) F.p[n * 16 + threadIdx.x] = 0;
-    return;
+    const unsigned long long done = bytes / 16 * 16;
+    if (blockIdx.x == 0 && threadIdx.x < bytes - done) dtable[done + threadIdx.x] = 0;
+  } else {
+    const unsigned int lane = threadIdx.x % 32, warps = GA_EG_ZERO / 32;
+    for (unsigned long long r = (unsigned long long)blockIdx.x * warps + threadIdx.x / 32; r < L.v;
+         r += (unsigned long long)gridDim.x * warps)
+      for (unsigned int v = lane; v < L.nv; v += 32)
+        ga__lm_store(dtable + (long long)r * L.v_row + (long long)v * GA_EM_E * L.v_col, ga__em_zero<ga__em_out>().c[0]);
   }
-  const unsigned int lane = threadIdx.x % 32, warps = blockDim.x / 32;
-  for (unsigned long long r = F.r0 + (unsigned long long)cta * warps + threadIdx.x / 32; r < F.r1;
-       r += (unsigned long long)ctas * warps)
-    for (unsigned int v = lane; v < L.nv; v += 32) ga__eg_zero_row(L, F.p, r, v);
+  if (blockIdx.x == gridDim.x - 1) ga__grid_dependency_wait();
 }
 
 /* ---- sorting ---- */
@@ -208,12 +262,8 @@ static __device__ __forceinline__ unsigned int ga__eg_key(const ga__em_layout &L
  * here, the others' are set to zero for ga_eg_scatter to add to. */
 extern "C" __global__ void __launch_bounds__(GA_EG_THREADS)
 ga_eg_count(const __grid_constant__ ga__em_layout L, const __grid_constant__ ga__eg_sort S,
-            const __grid_constant__ ga__eg_fill F, unsigned int *counts, const char *ids, int *err) {
+            unsigned int *counts, const char *ids, int *err) {
   ga__grid_dependency_sync();
-  if (blockIdx.x >= S.tiles) {
-    ga__eg_zeros(L, F, blockIdx.x - S.tiles, gridDim.x - S.tiles);
-    return;
-  }
   __shared__ unsigned int hist[GA_EG_DIGITS];
   const unsigned int d = threadIdx.x, tile = blockIdx.x;
   hist[d] = 0;
@@ -227,20 +277,63 @@ ga_eg_count(const __grid_constant__ ga__em_layout L, const __grid_constant__ ga_
     counts[(p * GA_EG_DIGITS + d) * S.tiles + tile] = 0;
 }
 
-/* One pass: every key goes behind all with a smaller digit and, with an equal digit, behind those
- * that stand before it. The first pass takes the ids themselves; the last one leaves the byte
- * offsets of the tokens' rows of dout, so that the sums need no division. */
+/* The exclusive prefix of x over the CTA's GA_EG_THREADS threads. */
+static __device__ __forceinline__ unsigned int ga__eg_prefix(unsigned int x, unsigned int sums[GA_EG_WARPS]) {
+  const unsigned int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  unsigned int scan = x;
+#pragma unroll
+  for (int s = 1; s < 32; s *= 2) {
+    const unsigned int o = __shfl_up_sync(0xffffffffu, scan, s);
+    if (lane >= (unsigned int)s) scan += o;
+  }
+  if (lane == 31) sums[warp] = scan;
+  __syncthreads();
+  unsigned int r = scan - x;
+  for (unsigned int w = 0; w < warp; w++) r += sums[w];
+  return r;
+}
+
+/* Places of GA_EG_ROUND keys, GA_EG_KEYS of a thread: key j of a thread is key
+ * (warp * GA_EG_KEYS + j) * 32 + lane of the round, there where `live` says so. A key goes behind
+ * those of smaller digits and behind those of its own that stand before it. base: where the keys
+ * of the digit that is this thread's number begin; it moves on. */
+typedef unsigned int ga__eg_table[GA_EG_WARPS][GA_EG_DIGITS];
+static __device__ __forceinline__ void ga__eg_places(const unsigned int digit[GA_EG_KEYS],
+                                                     const int live[GA_EG_KEYS], unsigned int &base,
+                                                     ga__eg_table &cnt, unsigned int at[GA_EG_KEYS]) {
+  const unsigned int d = threadIdx.x, lane = d % 32, warp = d / 32;
+  for (int w = 0; w < GA_EG_WARPS; w++) cnt[w][d] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < GA_EG_KEYS; j++) {
+    const unsigned int same = __match_any_sync(0xffffffffu, live[j] ? digit[j] : GA_EG_DIGITS);
+    const unsigned int seen = live[j] ? cnt[warp][digit[j]] : 0;
+    at[j] = seen + __popc(same & ((1u << lane) - 1));
+    __syncwarp();
+    if (live[j] && __ffs(same) - 1 == (int)lane) cnt[warp][digit[j]] = seen + __popc(same);
+    __syncwarp();
+  }
+  __syncthreads();
+  for (int w = 0; w < GA_EG_WARPS; w++) { /* the digit's place for each warp */
+    const unsigned int x = cnt[w][d];
+    cnt[w][d] = base;
+    base += x;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < GA_EG_KEYS; j++)
+    if (live[j]) at[j] += cnt[warp][digit[j]];
+}
+
+/* One pass over many tokens. The first takes the ids themselves; the last leaves the byte offsets
+ * of the tokens' rows of dout, so that the sums need no division. */
 extern "C" __global__ void __launch_bounds__(GA_EG_THREADS)
 ga_eg_scatter(const __grid_constant__ ga__em_layout L, const __grid_constant__ ga__eg_sort S,
-              const __grid_constant__ ga__eg_fill F, unsigned int *counts, const char *ids,
+              unsigned int *counts, const char *ids,
               const unsigned int *key_in, const unsigned int *order_in, unsigned int *key,
               unsigned int *order, long long *off) {
   ga__grid_dependency_sync();
-  if (blockIdx.x >= S.tiles) {
-    ga__eg_zeros(L, F, blockIdx.x - S.tiles, gridDim.x - S.tiles);
-    return;
-  }
-  __shared__ unsigned int cnt[GA_EG_WARPS][GA_EG_DIGITS];
+  __shared__ ga__eg_table cnt;
   __shared__ unsigned int sums[GA_EG_WARPS];
   const unsigned int d = threadIdx.x, lane = d % 32, warp = d / 32, tile = blockIdx.x;
   const unsigned int shift = S.pass * GA_EG_BITS;
@@ -253,77 +346,143 @@ ga_eg_scatter(const __grid_constant__ ga__em_layout L, const __grid_constant__ g
     total += x;
     before += t < tile ? x : 0;
   }
-  unsigned int scan = total;
-#pragma unroll
-  for (int s = 1; s < 32; s *= 2) {
-    const unsigned int o = __shfl_up_sync(0xffffffffu, scan, s);
-    if (lane >= (unsigned int)s) scan += o;
-  }
-  if (lane == 31) sums[warp] = scan;
-  __syncthreads();
-  unsigned int base = scan - total + before;
-  for (unsigned int w = 0; w < warp; w++) base += sums[w];
+  unsigned int base = ga__eg_prefix(total, sums) + before;
 
   const unsigned int lo = tile * S.tile, hi = S.n - lo < S.tile ? S.n : lo + S.tile;
   for (unsigned int i0 = lo; i0 < hi; i0 += GA_EG_ROUND) {
-    unsigned int k[GA_EG_KEYS], o[GA_EG_KEYS], rank[GA_EG_KEYS];
+    unsigned int k[GA_EG_KEYS], o[GA_EG_KEYS], digit[GA_EG_KEYS], at[GA_EG_KEYS];
+    int live[GA_EG_KEYS];
 #pragma unroll
-    for (int j = 0; j < GA_EG_KEYS; j++) { /* a warp's keys are adjacent */
+    for (int j = 0; j < GA_EG_KEYS; j++) {
       const unsigned int i = i0 + (warp * GA_EG_KEYS + j) * 32 + lane;
       k[j] = o[j] = 0;
-      if (i < hi) {
+      live[j] = i < hi;
+      if (live[j]) {
         k[j] = S.pass == 0 ? ga__eg_key(L, ids, i, nullptr) : key_in[i];
         o[j] = S.pass == 0 ? i : order_in[i];
       }
+      digit[j] = (k[j] >> shift) & (GA_EG_DIGITS - 1);
     }
-    for (int w = 0; w < GA_EG_WARPS; w++) cnt[w][d] = 0;
-    __syncthreads();
+    ga__eg_places(digit, live, base, cnt, at);
 #pragma unroll
     for (int j = 0; j < GA_EG_KEYS; j++) {
-      const unsigned int i = i0 + (warp * GA_EG_KEYS + j) * 32 + lane;
-      const unsigned int digit = i < hi ? (k[j] >> shift) & (GA_EG_DIGITS - 1) : GA_EG_DIGITS;
-      const unsigned int same = __match_any_sync(0xffffffffu, digit);
-      const unsigned int seen = i < hi ? cnt[warp][digit] : 0;
-      rank[j] = seen + __popc(same & ((1u << lane) - 1));
-      __syncwarp();
-      if (i < hi && __ffs(same) - 1 == (int)lane) cnt[warp][digit] = seen + __popc(same);
-      __syncwarp();
-    }
-    __syncthreads();
-    for (int w = 0; w < GA_EG_WARPS; w++) { /* the digit's place for each warp */
-      const unsigned int x = cnt[w][d];
-      cnt[w][d] = base;
-      base += x;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < GA_EG_KEYS; j++) {
-      const unsigned int i = i0 + (warp * GA_EG_KEYS + j) * 32 + lane;
-      if (i < hi) {
-        const unsigned int at = cnt[warp][(k[j] >> shift) & (GA_EG_DIGITS - 1)] + rank[j];
-        key[at] = k[j];
-        if (S.pass + 1 == S.passes) {
-          off[at] = ga__lm_offset<GA_EM_ND>(o[j], L.dims, L.t_str);
-        } else {
-          order[at] = o[j];
-          atomicAdd(&counts[((S.pass + 1) * GA_EG_DIGITS + ((k[j] >> (shift + GA_EG_BITS)) & (GA_EG_DIGITS - 1))) * S.tiles + at / S.tile], 1u);
-        }
+      if (!live[j]) continue;
+      key[at[j]] = k[j];
+      if (S.pass + 1 == S.passes) {
+        off[at[j]] = ga__lm_offset<GA_EM_ND>(o[j], L.dims, L.t_str);
+      } else {
+        const unsigned int next = (k[j] >> (shift + GA_EG_BITS)) & (GA_EG_DIGITS - 1);
+        order[at[j]] = o[j];
+        atomicAdd(&counts[((S.pass + 1) * GA_EG_DIGITS + next) * S.tiles + at[j] / S.tile], 1u);
       }
     }
     __syncthreads();
+  }
+}
+
+/* All passes in one launch, for as many tokens as the shared memory of one cluster holds: CTA r of
+ * the cluster has the tokens, then the sorted keys, from r * GA_EG_TILE on. A pass counts
+ * its digits, gives the counts to all CTAs, and sends every key to its place. */
+#define GA_EG_CLUSTER 8
+#define GA_EG_TILE (GA_EG_ROUND * GA_EG_ROUNDS)
+struct ga__eg_shared {
+  ga__eg_table cnt;
+  unsigned int tab[GA_EG_CLUSTER][GA_EG_DIGITS];
+  unsigned int hist[GA_EG_DIGITS];
+  unsigned int sums[GA_EG_WARPS];
+  unsigned long long keys[GA_EG_TILE]; /* key << 32 | token */
+};
+
+extern "C" __global__ void __cluster_dims__(GA_EG_CLUSTER, 1, 1) __launch_bounds__(GA_EG_THREADS)
+ga_eg_sort_all(const __grid_constant__ ga__em_layout L, const __grid_constant__ ga__eg_sort S,
+               const char *ids, unsigned int *key, long long *off, int *err) {
+  ga__grid_dependency_sync();
+  GA_LM_SHARED_DYNAMIC(ga__eg_shared, sh);
+  ga__cluster_arrive(); /* waited for before the first store to another CTA's shared memory */
+  const unsigned int d = threadIdx.x, lane = d % 32, warp = d / 32, r = blockIdx.x;
+  unsigned int k[GA_EG_ROUNDS][GA_EG_KEYS], o[GA_EG_ROUNDS][GA_EG_KEYS];
+#pragma unroll
+  for (int g = 0; g < GA_EG_ROUNDS; g++)
+#pragma unroll
+    for (int j = 0; j < GA_EG_KEYS; j++) {
+      const unsigned int i = r * GA_EG_TILE + g * GA_EG_ROUND + (warp * GA_EG_KEYS + j) * 32 + lane;
+      o[g][j] = i;
+      k[g][j] = i < S.n ? ga__eg_key(L, ids, i, err) : 0;
+    }
+  ga__cluster_wait();
+  for (unsigned int pass = 0; pass < S.passes; pass++) {
+    const unsigned int shift = pass * GA_EG_BITS;
+    sh.hist[d] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int g = 0; g < GA_EG_ROUNDS; g++)
+#pragma unroll
+      for (int j = 0; j < GA_EG_KEYS; j++)
+        if (r * GA_EG_TILE + g * GA_EG_ROUND + (warp * GA_EG_KEYS + j) * 32 + lane < S.n)
+          atomicAdd(&sh.hist[(k[g][j] >> shift) & (GA_EG_DIGITS - 1)], 1u);
+    __syncthreads();
+    for (unsigned int t = 0; t < GA_EG_CLUSTER; t++) ga__cluster_put(&sh.tab[r][d], t, sh.hist[d]);
+    /* behind this everybody has the counts, and has taken its keys out of `keys` */
+    ga__cluster_arrive();
+    ga__cluster_wait();
+    unsigned int total = 0, before = 0;
+#pragma unroll
+    for (unsigned int t = 0; t < GA_EG_CLUSTER; t++) {
+      const unsigned int x = sh.tab[t][d];
+      total += x;
+      before += t < r ? x : 0;
+    }
+    unsigned int base = ga__eg_prefix(total, sh.sums) + before;
+#pragma unroll
+    for (int g = 0; g < GA_EG_ROUNDS; g++) {
+      unsigned int digit[GA_EG_KEYS], at[GA_EG_KEYS];
+      int live[GA_EG_KEYS];
+#pragma unroll
+      for (int j = 0; j < GA_EG_KEYS; j++) {
+        live[j] = r * GA_EG_TILE + g * GA_EG_ROUND + (warp * GA_EG_KEYS + j) * 32 + lane < S.n;
+        digit[j] = (k[g][j] >> shift) & (GA_EG_DIGITS - 1);
+      }
+      ga__eg_places(digit, live, base, sh.cnt, at);
+#pragma unroll
+      for (int j = 0; j < GA_EG_KEYS; j++) {
+        if (!live[j]) continue;
+        if (pass + 1 == S.passes) {
+          key[at[j]] = k[g][j];
+          off[at[j]] = ga__lm_offset<GA_EM_ND>(o[g][j], L.dims, L.t_str);
+        } else {
+          ga__cluster_put(&sh.keys[at[j] % GA_EG_TILE], at[j] / GA_EG_TILE,
+                          (unsigned long long)k[g][j] << 32 | o[g][j]);
+        }
+      }
+      __syncthreads();
+    }
+    if (pass + 1 == S.passes) return;
+    ga__cluster_arrive(); /* every key has arrived */
+    ga__cluster_wait();
+#pragma unroll
+    for (int g = 0; g < GA_EG_ROUNDS; g++)
+#pragma unroll
+      for (int j = 0; j < GA_EG_KEYS; j++) {
+        const unsigned long long x = sh.keys[g * GA_EG_ROUND + (warp * GA_EG_KEYS + j) * 32 + lane];
+        k[g][j] = (unsigned int)(x >> 32);
+        o[g][j] = (unsigned int)x;
+      }
   }
 }
 
 /* ---- summing ---- */
-#define GA_EG_U 8
-#define GA_EG_J 8
+/* tokens whose rows a thread has in flight, 16 bytes of each. Four of 4 CTAs an SM: 8 of 2 CTAs
+ * are as many bytes, but fewer warps to go on while a run's end is written (two parts of 8190 rows
+ * of 1021 floats: 114 against 134 us). */
+#define GA_EG_U 4
+#define GA_EG_J 4 /* parts a thread has in flight */
 
-static __device__ __forceinline__ void ga__eg_park(GA_EM_F_T *p, const GA_EM_F_T acc[GA_EM_E]) {
+static __device__ __forceinline__ void ga__eg_park(GA_EM_F_T *p, const GA_EM_F_T acc[GA_EM_N]) {
 #pragma unroll
-  for (int j = 0; j < GA_EM_E; j++) p[j] = acc[j];
+  for (int j = 0; j < GA_EM_N; j++) p[j] = acc[j];
 }
 
-/* Sums sorted tokens [lo, hi) of n at vector position v; off: their rows of dout. head, tail:
+/* Sums sorted tokens [lo, hi) of n at a thread's vectors; off: their rows of dout. head, tail:
  * where the parts of the run that began before lo, and of the one that goes on behind hi, are
  * parked. Both lists may be read up to GA_EG_U - 1 entries beyond hi, by vectors where WIDE (lo a
  * multiple of GA_EG_U). */
@@ -331,16 +490,15 @@ template <int WIDE>
 static __device__ __forceinline__ void ga__eg_chunk(const ga__em_layout &L, char *dtable,
                                                     const char *dout, const unsigned int *key,
                                                     const long long *off, unsigned int n,
-                                                    unsigned int lo, unsigned int hi, unsigned int v,
+                                                    unsigned int lo, unsigned int hi, ga__em_pos pos,
                                                     GA_EM_F_T *head, GA_EM_F_T *tail) {
   const unsigned int none = (unsigned int)L.v;
   unsigned int cur = key[lo];
   int open_head = lo > 0 && key[lo - 1] == cur;
-  GA_EM_F_T acc[GA_EM_E];
+  GA_EM_F_T acc[GA_EM_N];
 #pragma unroll
-  for (int j = 0; j < GA_EM_E; j++) acc[j] = 0;
+  for (int j = 0; j < GA_EM_N; j++) acc[j] = 0;
   ga__em_out old; /* of row `cur` */
-  const char *col = dout + (long long)v * GA_EM_E * L.t_col;
   for (unsigned int i = lo; i < hi && cur != none; i += GA_EG_U) {
     struct alignas(16) {
       unsigned int v[GA_EG_U];
@@ -366,14 +524,14 @@ static __device__ __forceinline__ void ga__eg_chunk(const ga__em_layout &L, char
     for (int u = 0; u < GA_EG_U; u++) {
       if (i + u >= hi) k.v[u] = none;
       if (k.v[u] != none)
-        q[u] = ga__lm_load<ga__em_in>(col + at.v[u]);
+        q[u] = ga__em_read<ga__em_in, ga__em_in1>(dout + at.v[u], L.t_col, pos);
     }
 #if GA_EM_ACCUMULATE
     /* read with the tokens' rows, not when a run ends: once a run, at its first token here */
 #pragma unroll
     for (int u = 0; u < GA_EG_U; u++)
       if (k.v[u] != none && (u == 0 ? k.v[u] != cur || i == lo : k.v[u] != k.v[u - 1]))
-        held[u] = ga__lm_load<ga__em_out>(ga__eg_place(L, dtable, k.v[u], v));
+        held[u] = ga__eg_held(L, dtable, k.v[u], pos);
     if (i == lo) old = held[0];
 #endif
 #pragma unroll
@@ -381,94 +539,113 @@ static __device__ __forceinline__ void ga__eg_chunk(const ga__em_layout &L, char
       if (i + u >= hi) break;
       if (k.v[u] != cur) { /* the run ends inside the chunk */
         if (open_head) ga__eg_park(head, acc);
-        else ga__eg_write(L, dtable, cur, v, acc, old);
+        else ga__eg_write(L, dtable, cur, pos, acc, old);
         open_head = 0;
         cur = k.v[u];
 #if GA_EM_ACCUMULATE
         old = held[u];
 #endif
 #pragma unroll
-        for (int j = 0; j < GA_EM_E; j++) acc[j] = 0;
+        for (int j = 0; j < GA_EM_N; j++) acc[j] = 0;
         if (cur == none) break;
       }
-      GA_EM_F_T x[GA_EM_E];
-      ga__lm_get<GA_EM_A_T, GA_EM_E>(x, q[u]);
+      GA_EM_F_T x[GA_EM_N];
+      ga__em_get<GA_EM_A_T>(x, q[u]);
 #pragma unroll
-      for (int j = 0; j < GA_EM_E; j++) acc[j] += x[j];
+      for (int j = 0; j < GA_EM_N; j++) acc[j] += x[j];
     }
   }
   if (cur == none) return;
   if (open_head) ga__eg_park(head, acc);
   else if (hi < n && key[hi] == cur) ga__eg_park(tail, acc);
-  else ga__eg_write(L, dtable, cur, v, acc, old);
+  else ga__eg_write(L, dtable, cur, pos, acc, old);
 }
 
 /* Joins the run that starts in chunk c (tokens c * size ...) and goes on in the next, if there is
- * one. part: the chunks' parked rows at this vector position, heads and tails in turn, `step`
- * elements apart. */
+ * one: of the `ny` threads at a vector position thread y takes every ny-th part, then the first
+ * adds their sums, always in the same order; with ny > 1 all threads of the CTA are here for the
+ * same c. part: the chunks' parked rows at this thread's vectors, heads and tails in turn, `step`
+ * elements apart. sum: with ny > 1, 256 * GA_EM_N entries of shared memory. */
 static __device__ __forceinline__ void ga__eg_join_run(const ga__em_layout &L, char *dtable,
                                                        const unsigned int *key, unsigned int c,
                                                        unsigned int size, unsigned int chunks,
-                                                       unsigned int v, const GA_EM_F_T *part,
-                                                       size_t step) {
+                                                       ga__em_pos pos, const GA_EM_F_T *part,
+                                                       size_t step, unsigned int y, unsigned int ny,
+                                                       GA_EM_F_T *sum) {
   const unsigned int lo = c * size, next = lo + size; /* next < n: chunk c + 1 exists */
   const unsigned int cur = key[next];
   if (cur == (unsigned int)L.v || key[next - 1] != cur) return;
   if (key[lo] == cur && lo > 0 && key[lo - 1] == cur) return; /* it began earlier */
-  GA_EM_F_T acc[GA_EM_E];
-  const GA_EM_F_T *p = part + (2 * (size_t)c + 1) * step;
-#pragma unroll
-  for (int j = 0; j < GA_EM_E; j++) acc[j] = p[j];
+  const int inside = pos.v < L.nv;
+  GA_EM_F_T acc[GA_EM_N];
   ga__em_out old;
+  if (inside) {
+#pragma unroll
+    for (int j = 0; j < GA_EM_N; j++) acc[j] = 0;
+    if (y == 0) {
 #if GA_EM_ACCUMULATE
-  old = ga__lm_load<ga__em_out>(ga__eg_place(L, dtable, cur, v));
+      old = ga__eg_held(L, dtable, cur, pos);
 #endif
-  /* GA_EG_J parts are fetched together with the keys that tell whether they belong to the run */
-  for (unsigned int d = c + 1, more = 1; more && d < chunks; d += GA_EG_J) {
-    GA_EM_F_T x[GA_EG_J][GA_EM_E];
-    unsigned int k[GA_EG_J];
+      const GA_EM_F_T *p = part + (2 * (size_t)c + 1) * step;
 #pragma unroll
-    for (int u = 0; u < GA_EG_J; u++)
-      if (d + u < chunks) {
-        k[u] = key[(d + u) * size];
-        p = part + 2 * (size_t)(d + u) * step;
-#pragma unroll
-        for (int j = 0; j < GA_EM_E; j++) x[u][j] = p[j];
-      }
-#pragma unroll
-    for (int u = 0; u < GA_EG_J; u++) {
-      if (!more || d + u >= chunks || k[u] != cur) {
-        more = 0;
-        continue;
-      }
-#pragma unroll
-      for (int j = 0; j < GA_EM_E; j++) acc[j] += x[u][j];
+      for (int j = 0; j < GA_EM_N; j++) acc[j] = p[j];
     }
+    /* GA_EG_J parts are fetched together with the keys that tell whether they belong to the run */
+    for (unsigned int d = c + 1 + y, more = 1; more && d < chunks; d += GA_EG_J * ny) {
+      GA_EM_F_T x[GA_EG_J][GA_EM_N];
+      unsigned int k[GA_EG_J];
+#pragma unroll
+      for (int u = 0; u < GA_EG_J; u++)
+        if (d + u * ny < chunks) {
+          k[u] = key[(d + u * ny) * size];
+          const GA_EM_F_T *p = part + 2 * (size_t)(d + u * ny) * step;
+#pragma unroll
+          for (int j = 0; j < GA_EM_N; j++) x[u][j] = p[j];
+        }
+#pragma unroll
+      for (int u = 0; u < GA_EG_J; u++) {
+        if (!more || d + u * ny >= chunks || k[u] != cur) {
+          more = 0;
+          continue;
+        }
+#pragma unroll
+        for (int j = 0; j < GA_EM_N; j++) acc[j] += x[u][j];
+      }
+    }
+    if (y > 0) ga__eg_park(sum + (y * blockDim.x + threadIdx.x) * GA_EM_N, acc);
   }
-  ga__eg_write(L, dtable, cur, v, acc, old);
+  if (ny > 1) __syncthreads();
+  if (!inside || y > 0) return;
+  for (unsigned int i = 1; i < ny; i++)
+#pragma unroll
+    for (int j = 0; j < GA_EM_N; j++) acc[j] += sum[(i * blockDim.x + threadIdx.x) * GA_EM_N + j];
+  ga__eg_write(L, dtable, cur, pos, acc, old);
 }
 
-extern "C" __global__ void __launch_bounds__(256)
+/* `part` holds GA_EM_N sums for each thread along the row, two rows of them per chunk. */
+extern "C" __global__ void __launch_bounds__(256, 4)
 ga_eg_sum(const __grid_constant__ ga__em_layout L, char *dtable, const char *dout,
           const unsigned int *key, const long long *off, GA_EM_F_T *part) {
   ga__grid_dependency_sync();
-  const unsigned int v = blockIdx.y * blockDim.x + threadIdx.x;
+  const ga__em_pos pos = ga__em_here(L);
   const unsigned int c = blockIdx.x * blockDim.y + threadIdx.y;
-  if (v >= L.nv || c >= L.chunks) return;
+  if (pos.v >= L.nv || c >= L.chunks) return;
   const unsigned int n = (unsigned int)L.n, lo = c * L.chunk, hi = n - lo < L.chunk ? n : lo + L.chunk;
-  GA_EM_F_T *head = part + (2 * (size_t)c * L.nv + v) * GA_EM_E;
-  ga__eg_chunk<1>(L, dtable, dout, key, off, n, lo, hi, v, head, head + (size_t)L.nv * GA_EM_E);
+  const size_t step = (size_t)gridDim.y * blockDim.x * GA_EM_N;
+  GA_EM_F_T *head = part + 2 * (size_t)c * step + (size_t)(blockIdx.y * blockDim.x + threadIdx.x) * GA_EM_N;
+  ga__eg_chunk<1>(L, dtable, dout, key, off, n, lo, hi, pos, head, head + step);
 }
 
+/* A CTA for each chunk but the last (blockIdx.x) and slice of the rows, with as many threads along
+ * them as in ga_eg_sum; most find nothing to join. */
 extern "C" __global__ void __launch_bounds__(256)
 ga_eg_join(const __grid_constant__ ga__em_layout L, char *dtable, const unsigned int *key,
            const GA_EM_F_T *part) {
   ga__grid_dependency_sync();
-  const unsigned int v = blockIdx.y * blockDim.x + threadIdx.x;
-  const unsigned int c = blockIdx.x * blockDim.y + threadIdx.y;
-  if (v >= L.nv || c + 1 >= L.chunks) return;
-  ga__eg_join_run(L, dtable, key, c, L.chunk, L.chunks, v, part + (size_t)v * GA_EM_E,
-                  (size_t)L.nv * GA_EM_E);
+  __shared__ GA_EM_F_T sum[256 * GA_EM_N];
+  ga__eg_join_run(L, dtable, key, blockIdx.x, L.chunk, L.chunks, ga__em_here(L),
+                  part + (size_t)(blockIdx.y * blockDim.x + threadIdx.x) * GA_EM_N,
+                  (size_t)gridDim.y * blockDim.x * GA_EM_N, threadIdx.y, blockDim.y, sum);
 }
 
 /* ---- few tokens ---- */
@@ -476,7 +653,7 @@ ga_eg_join(const __grid_constant__ ga__em_layout L, char *dtable, const unsigned
 #define GA_EG_FEW_WARPS 8
 #define GA_EG_TX 32   /* vector positions of a CTA at most; blockDim.x * blockDim.y is 256 */
 
-/* CTA (x, y) owns L.chunk rows from x * L.chunk and the vectors of slice y. */
+/* CTA (x, y) owns L.chunk rows from x * L.chunk and slice y of their vectors. */
 extern "C" __global__ void __launch_bounds__(256)
 ga_eg_direct(const __grid_constant__ ga__em_layout L, char *dtable, const char *dout,
              const char *ids, int *err) {
@@ -484,7 +661,7 @@ ga_eg_direct(const __grid_constant__ ga__em_layout L, char *dtable, const char *
   __shared__ unsigned int row[GA_EG_FEW], token[GA_EG_FEW], key[GA_EG_FEW + GA_EG_U];
   __shared__ long long off[GA_EG_FEW + GA_EG_U];
   __shared__ unsigned int found[GA_EG_FEW_WARPS];
-  __shared__ GA_EM_F_T part[256 * 2 * GA_EM_E];
+  __shared__ GA_EM_F_T part[256 * 2 * GA_EM_N];
   const unsigned int tid = threadIdx.y * blockDim.x + threadIdx.x, lane = tid % 32, warp = tid / 32;
   const unsigned int n = (unsigned int)L.n;
   const unsigned long long r0 = (unsigned long long)blockIdx.x * L.chunk;
@@ -518,21 +695,22 @@ ga_eg_direct(const __grid_constant__ ga__em_layout L, char *dtable, const char *
     key[at] = k;
     off[at] = ga__lm_offset<GA_EM_ND>(token[i], L.dims, L.t_str);
   }
-  const unsigned int v = blockIdx.y * blockDim.x + threadIdx.x;
+  const ga__em_pos pos = ga__em_here(L);
 #if !GA_EM_ACCUMULATE
-  if (v < L.nv)
-    for (unsigned long long r = r0 + threadIdx.y; r < r1; r += blockDim.y) ga__eg_zero_row(L, dtable, r, v);
+  if (pos.v < L.nv)
+    for (unsigned long long r = r0 + threadIdx.y; r < r1; r += blockDim.y)
+      ga__em_write(dtable + (long long)r * L.v_row, L.v_col, pos, ga__em_zero<ga__em_out>());
 #endif
   __syncthreads();
   if (m == 0) return;
   const unsigned int size = (m + blockDim.y - 1) / blockDim.y, chunks = (m + size - 1) / size;
   const unsigned int c = threadIdx.y;
-  GA_EM_F_T *mine = part + threadIdx.x * GA_EM_E;
-  const size_t step = (size_t)blockDim.x * GA_EM_E;
-  if (v < L.nv && c < chunks)
-    ga__eg_chunk<0>(L, dtable, dout, key, off, m, c * size, m - c * size < size ? m : (c + 1) * size, v,
+  GA_EM_F_T *mine = part + threadIdx.x * GA_EM_N;
+  const size_t step = (size_t)blockDim.x * GA_EM_N;
+  if (pos.v < L.nv && c < chunks)
+    ga__eg_chunk<0>(L, dtable, dout, key, off, m, c * size, m - c * size < size ? m : (c + 1) * size, pos,
                  mine + 2 * c * step, mine + (2 * c + 1) * step);
   __syncthreads();
-  if (v < L.nv && c + 1 < chunks) ga__eg_join_run(L, dtable, key, c, size, chunks, v, mine, step);
+  if (pos.v < L.nv && c + 1 < chunks) ga__eg_join_run(L, dtable, key, c, size, chunks, pos, mine, step, 0, 1, mine);
 }
 #endif

@@ -74,10 +74,25 @@ static __device__ __forceinline__ void ga__st32(char *p, const unsigned int w[8]
                : "memory");
 }
 
+/* The two halves of ga__grid_dependency_sync(), for a kernel that does not depend on its
+ * predecessor in the stream but on what came before that one. */
+static __device__ __forceinline__ void ga__grid_dependency_wait() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+static __device__ __forceinline__ void ga__grid_dependency_release() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 /* Sum over the warp, the same in every lane */
 static __device__ __forceinline__ unsigned int ga__warp_sum_u32(unsigned int v) {
   return __reduce_add_sync(0xffffffffu, v);
 }
+
+/* Shared memory of a kernel: one struct, of fixed size or with a tail whose size the launch gives */
+#define GA_LM_SHARED(type, name) __shared__ type name
+#define GA_LM_SHARED_DYNAMIC(type, name)                          \
+  extern __shared__ unsigned long long ga__dynamic_shared[];      \
+  type &name = *reinterpret_cast<type *>(ga__dynamic_shared)
 
 /* ---- thread-block clusters ---- */
 static __device__ __forceinline__ unsigned int ga__cluster_rank() {
@@ -94,11 +109,19 @@ static __device__ __forceinline__ void ga__cluster_wait() {
   asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
 }
 /* Stores 8 bytes at the place that `p` (this CTA's shared memory) has in CTA `rank`'s. */
-static __device__ __forceinline__ void ga__cluster_put(void *p, unsigned int rank,
+static __device__ __forceinline__ void ga__cluster_put(unsigned long long *p, unsigned int rank,
                                                        unsigned long long v) {
   const unsigned int s = (unsigned int)__cvta_generic_to_shared(p);
   asm volatile("{.reg .u32 a;\n\tmapa.shared::cluster.u32 a, %0, %1;\n\t"
                "st.shared::cluster.u64 [a], %2;}" ::"r"(s), "r"(rank), "l"(v)
+               : "memory");
+}
+/* The same with 4 bytes. */
+static __device__ __forceinline__ void ga__cluster_put(unsigned int *p, unsigned int rank,
+                                                       unsigned int v) {
+  const unsigned int s = (unsigned int)__cvta_generic_to_shared(p);
+  asm volatile("{.reg .u32 a;\n\tmapa.shared::cluster.u32 a, %0, %1;\n\t"
+               "st.shared::cluster.u32 [a], %2;}" ::"r"(s), "r"(rank), "r"(v)
                : "memory");
 }
 #endif

@@ -213,61 +213,37 @@ struct ga__lp_top_smem {
   unsigned long long cand[GA_LP_CAND];
   unsigned long long best[GA_LP_THREADS];
   unsigned long long out[GA_LP_CLUSTER * 32]; /* the CTAs' lists, in the first CTA of a cluster */
-  unsigned long long tau;
+  unsigned int high[GA_LP_THREADS];
   unsigned int list[GA_LP_THREADS];
-  unsigned int nlist, ncand;
-  unsigned int count;
+  unsigned int nlist, ncand, count;
 };
 
-/* The `top` largest keys of vectors [v0, v1) of the row, into out[0..32) of this CTA's or the
- * cluster's first CTA's shared memory (0 where there are fewer). All threads of the CTA.
- *
- * `first` is the vector in which this thread's first largest element lies. The largest keys of
- * 32 disjoint groups of threads are keys of 32 elements, so the top-th largest of them, tau, is a
- * lower bound for the top-th largest of all, and every key above it belongs to a thread whose
- * largest reaches it: only those threads' vectors are read again. (Half the groups' largest lie
- * above tau where 16 alternatives are asked for; the keys above it are then about 20.) Where NaNs
- * made `first` unusable, or the keys above tau are too many to hold (a row that hides its largest
- * elements in few threads' vectors), tau is found by halving over the whole row. */
-static __device__ void ga__lp_top(const ga__lp_layout &L, const ga__lp_row &r, unsigned int v0,
-                                  unsigned int v1, unsigned int first, int odd, ga__lp_top_smem &S) {
-  const unsigned int tid = threadIdx.x;
-  unsigned long long k[2 * GA_LP_PAIRS], mine = 0;
-  if (v0 + tid < v1) {
-    ga__lp_keys(L, r, first, k);
+/* The top-th largest of the lanes' keys, at least 1 (0: no key); the same in every lane. */
+template <typename K>
+static __device__ __forceinline__ K ga__lp_nth(K mine, unsigned int top) {
+  const unsigned int lane = threadIdx.x % 32;
+  unsigned int place = 0;
 #pragma unroll
-    for (int j = 0; j < 2 * GA_LP_PAIRS; j++) mine = k[j] > mine ? k[j] : mine;
+  for (int j = 0; j < 32; j++) {
+    const K o = __shfl_sync(0xffffffffu, mine, j);
+    place += o > mine || (o == mine && j < (int)lane);
   }
-  S.best[tid] = mine;
-  if (tid == 0) {
-    S.nlist = 0;
-    S.ncand = 0;
-  }
-  __syncthreads();
-  if (tid < 32) { /* the largest of every 32nd thread's, and their order: 32 keys in one warp */
-    unsigned long long high = 0;
-#pragma unroll
-    for (int j = 0; j < GA_LP_THREADS / 32; j++) {
-      const unsigned long long b = S.best[j * 32 + tid];
-      high = b > high ? b : high;
-    }
-    unsigned int place = 0;
-#pragma unroll
-    for (int j = 0; j < 32; j++) {
-      const unsigned long long o = __shfl_sync(0xffffffffu, high, j);
-      place += o > high || (o == high && j < (int)tid); /* equal: both 0, no key */
-    }
-    if (place == L.top - 1) S.tau = high > 0 ? high : 1; /* fewer than `top` keys: everything */
-  }
-  __syncthreads();
-  unsigned long long tau = S.tau;
-  if (!odd && mine >= tau) S.list[atomicAdd(&S.nlist, 1u)] = tid;
-  __syncthreads();
+  const unsigned int who = __ballot_sync(0xffffffffu, place == top - 1);
+  const K t = __shfl_sync(0xffffffffu, mine, __ffs(who) - 1);
+  return t > 0 ? t : 1;
+}
+
+/* Appends the keys from `tau` on of the listed threads' vectors (or of all) to the candidates. */
+static __device__ __forceinline__ void ga__lp_collect(const ga__lp_layout &L, const ga__lp_row &r,
+                                                      unsigned int v0, unsigned int v1, int all,
+                                                      unsigned long long tau, ga__lp_top_smem &S) {
   const unsigned int per = (v1 - v0 + GA_LP_THREADS - 1) / GA_LP_THREADS;
-  const unsigned int items = S.nlist * per;
-  for (unsigned int it = tid; it < items; it += GA_LP_THREADS) {
-    const unsigned int w = v0 + S.list[it / per] + (it % per) * GA_LP_THREADS;
+  const unsigned int items = all ? v1 - v0 : S.nlist * per;
+  for (unsigned int it = threadIdx.x; it < items; it += GA_LP_THREADS) {
+    if (*(volatile unsigned int *)&S.ncand > GA_LP_CAND) break; /* too many: they are not used */
+    const unsigned int w = v0 + (all ? it : S.list[it / per] + (it % per) * GA_LP_THREADS);
     if (w >= v1) continue;
+    unsigned long long k[2 * GA_LP_PAIRS];
     ga__lp_keys(L, r, w, k);
 #pragma unroll
     for (int j = 0; j < 2 * GA_LP_PAIRS; j++)
@@ -277,7 +253,68 @@ static __device__ void ga__lp_top(const ga__lp_layout &L, const ga__lp_row &r, u
       }
   }
   __syncthreads();
+}
+
+/* The `top` largest keys of vectors [v0, v1) of the row, into out[0..32) of this CTA's or the
+ * cluster's first CTA's shared memory (0 where there are fewer). All threads of the CTA, after a
+ * barrier behind which S.high has every thread's largest value and the counters are 0; m: this
+ * thread's.
+ *
+ * The largest values of 32 disjoint groups of threads are values of 32 elements, so the top-th
+ * largest of them, tau, is a lower bound for the top-th largest of all, and every element that
+ * reaches it belongs to a thread whose largest does: only those threads' vectors are read again.
+ * (For 20 alternatives of 256 threads they are about 30.) Where more elements reach tau than can
+ * be held (equal values: rows with fewer numbers than alternatives, constants), the same is done
+ * with keys that break ties by the index; where that is still too much (a row that hides its
+ * largest elements in few threads' vectors) or NaNs are about (`odd`), tau is found by halving
+ * over the row. */
+static __device__ void ga__lp_top(const ga__lp_layout &L, const ga__lp_row &r, unsigned int v0,
+                                  unsigned int v1, float m, int odd, ga__lp_top_smem &S) {
+  const unsigned int tid = threadIdx.x, lane = tid % 32;
+  unsigned long long k[2 * GA_LP_PAIRS], tau = 0;
+  if (!odd) {
+    unsigned int high = 0;
+#pragma unroll
+    for (int j = 0; j < GA_LP_THREADS / 32; j++) {
+      const unsigned int b = S.high[j * 32 + lane];
+      high = b > high ? b : high;
+    }
+    tau = (unsigned long long)ga__lp_nth(high, L.top) << 32;
+    const float minus_inf = __uint_as_float(0xff800000u);
+    const int few = (tau >> 32) == (ga__lp_key(minus_inf, 0) >> 32); /* fewer above -inf than asked for */
+    if (!few) {
+      if (v0 + tid < v1 && ga__lp_key(m, 0) >= tau) S.list[atomicAdd(&S.nlist, 1u)] = tid;
+      __syncthreads();
+      ga__lp_collect(L, r, v0, v1, 0, tau, S);
+    }
+    if (few || S.ncand > GA_LP_CAND) { /* the same in every thread */
+      unsigned long long mine = 0;
+      for (unsigned int w = v0 + tid; w < v1; w += GA_LP_THREADS) /* its first place */
+        if (ga__lp_max(ga__lp_load(L, r, w)) >= m) {
+          ga__lp_keys(L, r, w, k);
+#pragma unroll
+          for (int j = 0; j < 2 * GA_LP_PAIRS; j++) mine = k[j] > mine ? k[j] : mine;
+          break;
+        }
+      S.best[tid] = mine;
+      __syncthreads();
+      if (tid == 0) S.nlist = S.ncand = 0;
+      unsigned long long most = 0;
+#pragma unroll
+      for (int j = 0; j < GA_LP_THREADS / 32; j++) {
+        const unsigned long long b = S.best[j * 32 + lane];
+        most = b > most ? b : most;
+      }
+      tau = ga__lp_nth(most, L.top);
+      __syncthreads();
+      if (mine >= tau) S.list[atomicAdd(&S.nlist, 1u)] = tid;
+      __syncthreads();
+      ga__lp_collect(L, r, v0, v1, 0, tau, S);
+    }
+  }
   if (odd || S.ncand > GA_LP_CAND) { /* the same in every thread */
+    /* the first count is of all there is; after it fewer than `top` keys reach hi and at least as
+     * many lo, and keys differ: 64 halvings end with exactly `top` */
     unsigned long long lo = 1, hi = ~0ULL; /* above every key: the largest value, inf, has 0xff800000 */
     for (int step = 0; step < 66; step++) {
       const unsigned long long mid = step == 0 ? 1 : lo + (hi - lo) / 2;
@@ -291,7 +328,7 @@ static __device__ void ga__lp_top(const ga__lp_layout &L, const ga__lp_row &r, u
         for (int j = 0; j < 2 * GA_LP_PAIRS; j++) c += k[j] >= mid;
       }
       c = ga__warp_sum_u32(c);
-      if (tid % 32 == 0) atomicAdd(&S.count, c);
+      if (lane == 0) atomicAdd(&S.count, c);
       __syncthreads();
       c = S.count;
       if (c >= L.top || step == 0) lo = mid;
@@ -301,28 +338,20 @@ static __device__ void ga__lp_top(const ga__lp_layout &L, const ga__lp_row &r, u
     tau = lo;
     if (tid == 0) S.ncand = 0;
     __syncthreads();
-    for (unsigned int w = v0 + tid; w < v1; w += GA_LP_THREADS) {
-      ga__lp_keys(L, r, w, k);
-#pragma unroll
-      for (int j = 0; j < 2 * GA_LP_PAIRS; j++)
-        if (k[j] >= tau) {
-          const unsigned int at = atomicAdd(&S.ncand, 1u);
-          if (at < GA_LP_CAND) S.cand[at] = k[j];
-        }
-    }
-    __syncthreads();
+    ga__lp_collect(L, r, v0, v1, 1, tau, S);
   }
   /* a key's place is the number of larger ones */
   const unsigned int n = S.ncand < GA_LP_CAND ? S.ncand : GA_LP_CAND;
 #if GA_LP_CLUSTER > 1
   const unsigned int slot = ga__cluster_rank() * 32;
-  for (unsigned int i = tid + n; i < L.top; i += GA_LP_THREADS) ga__cluster_put(&S.out[slot + i], 0, 0);
+  for (unsigned int i = tid + n; i < L.top; i += GA_LP_THREADS) ga__cluster_put(&S.out[slot + i], 0, 0ULL);
 #else
   for (unsigned int i = tid + n; i < L.top; i += GA_LP_THREADS) S.out[i] = 0;
 #endif
   for (unsigned int i = tid; i < n; i += GA_LP_THREADS) {
     const unsigned long long key = S.cand[i];
     unsigned int place = 0;
+#pragma unroll 4
     for (unsigned int j = 0; j < n; j++) place += S.cand[j] > key;
     if (place < L.top) {
 #if GA_LP_CLUSTER > 1
@@ -334,6 +363,14 @@ static __device__ void ga__lp_top(const ga__lp_layout &L, const ga__lp_row &r, u
   }
 }
 #endif
+
+struct ga__lp_shared {
+#if GA_LP_TOP
+  ga__lp_top_smem tops;
+#endif
+  unsigned long long parts[GA_LP_CLUSTER][2]; /* the CTAs' states, in the first CTA of a cluster */
+  ga__lp_state warps[GA_LP_THREADS / 32];
+};
 
 extern "C" __global__ void __launch_bounds__(GA_LP_THREADS)
 #if GA_LP_CLUSTER > 1
@@ -375,13 +412,9 @@ ga_lp_rows(const __grid_constant__ ga__lp_layout L, const char *logits, const ch
   ga__lp_state st = {GA_LP_NOTHING, 0.0f, 0.0f};
   ga__f2 s2 = ga__f2_of(0.0f, 0.0f), t2 = s2;
   const ga__f2 c2 = ga__f2_of(c, c);
-#if GA_LP_TOP
-  unsigned int first = v0 + lane; /* the vector of this thread's first largest element */
-  float best = __uint_as_float(0xff800000u);
-#endif
   for (unsigned int w = v0 + lane; w < v1; w += GA_LP_GROUP * GA_LP_U) {
     ga__lp_words q[GA_LP_U];
-    float vm[GA_LP_U], top = __uint_as_float(0xff800000u);
+    float top = GA_LP_NOTHING;
     if (GA_LP_CONTIG && w > 0 && w + (GA_LP_U - 1) * GA_LP_GROUP < v1 &&
         w + (GA_LP_U - 1) * GA_LP_GROUP + 1 < r.nv) { /* neither the row's first nor its last vector */
 #pragma unroll
@@ -399,18 +432,7 @@ ga_lp_rows(const __grid_constant__ ga__lp_layout L, const char *logits, const ch
       }
     }
 #pragma unroll
-    for (int u = 0; u < GA_LP_U; u++) {
-      vm[u] = ga__lp_max(q[u]);
-      top = fmaxf(top, vm[u]);
-    }
-#if GA_LP_TOP
-    if (top > best) {
-#pragma unroll
-      for (int u = GA_LP_U - 1; u >= 0; u--)
-        if (vm[u] == top) first = w + u * GA_LP_GROUP;
-      best = top;
-    }
-#endif
+    for (int u = 0; u < GA_LP_U; u++) top = fmaxf(top, ga__lp_max(q[u]));
     if (top > st.m) {
       const float d = ga__max_nan((st.m - top) * c, GA_LP_YMIN), f = ga__ex2(d);
       const ga__f2 f2 = ga__f2_of(f, f);
@@ -444,6 +466,13 @@ ga_lp_rows(const __grid_constant__ ga__lp_layout L, const char *logits, const ch
     ga__f2_to(t2, a, b);
     st.t = a + b;
   }
+  GA_LM_SHARED(ga__lp_shared, sh);
+#if GA_LP_TOP
+  ga__lp_top_smem &tops = sh.tops;
+  const float most = st.s == 0.0f ? __uint_as_float(0xff800000u) : st.m; /* this thread's largest */
+  tops.high[threadIdx.x] = v0 + lane < v1 ? (unsigned int)(ga__lp_key(most, 0) >> 32) : 0;
+  if (threadIdx.x == 0) tops.nlist = tops.ncand = 0;
+#endif
 #pragma unroll
   for (int d = 16; d > 0; d /= 2) {
     ga__lp_state o;
@@ -453,11 +482,10 @@ ga_lp_rows(const __grid_constant__ ga__lp_layout L, const char *logits, const ch
     st = ga__lp_merge(st, o, c);
   }
 #if GA_LP_GROUP > 32
-  __shared__ ga__lp_state warps[GA_LP_THREADS / 32];
-  if (threadIdx.x % 32 == 0) warps[threadIdx.x / 32] = st;
+  if (threadIdx.x % 32 == 0) sh.warps[threadIdx.x / 32] = st;
   __syncthreads();
   /* every warp merges the warps' states in the same order: the same bits everywhere */
-  st = warps[threadIdx.x % (GA_LP_THREADS / 32)];
+  st = sh.warps[threadIdx.x % (GA_LP_THREADS / 32)];
 #pragma unroll
   for (int d = GA_LP_THREADS / 64; d > 0; d /= 2) {
     ga__lp_state o;
@@ -474,15 +502,13 @@ ga_lp_rows(const __grid_constant__ ga__lp_layout L, const char *logits, const ch
   ga__cluster_wait(); /* every CTA of the cluster runs */
 #endif
 #if GA_LP_TOP
-  __shared__ ga__lp_top_smem tops;
-  ga__lp_top(L, r, v0, v1, first, !(st.s == st.s), tops);
+  ga__lp_top(L, r, v0, v1, most, !(st.s == st.s), tops);
 #endif
 #if GA_LP_CLUSTER > 1
   /* the CTAs' states and lists meet in the first one */
-  __shared__ unsigned long long parts[GA_LP_CLUSTER][2];
   if (threadIdx.x == 0) {
-    ga__cluster_put(&parts[part][0], 0, (unsigned long long)__float_as_uint(st.m) << 32 | __float_as_uint(st.s));
-    ga__cluster_put(&parts[part][1], 0, (unsigned long long)__float_as_uint(st.t));
+    ga__cluster_put(&sh.parts[part][0], 0, (unsigned long long)__float_as_uint(st.m) << 32 | __float_as_uint(st.s));
+    ga__cluster_put(&sh.parts[part][1], 0, (unsigned long long)__float_as_uint(st.t));
   }
   ga__cluster_arrive();
   ga__cluster_wait();
@@ -490,9 +516,9 @@ ga_lp_rows(const __grid_constant__ ga__lp_layout L, const char *logits, const ch
 #pragma unroll 1
   for (int i = 0; i < GA_LP_CLUSTER; i++) {
     ga__lp_state o;
-    o.m = __uint_as_float((unsigned int)(parts[i][0] >> 32));
-    o.s = __uint_as_float((unsigned int)parts[i][0]);
-    o.t = __uint_as_float((unsigned int)parts[i][1]);
+    o.m = __uint_as_float((unsigned int)(sh.parts[i][0] >> 32));
+    o.s = __uint_as_float((unsigned int)sh.parts[i][0]);
+    o.t = __uint_as_float((unsigned int)sh.parts[i][1]);
     st = i == 0 ? o : ga__lp_merge(st, o, c);
   }
 #endif
@@ -538,8 +564,9 @@ ga_lp_rows(const __grid_constant__ ga__lp_layout L, const char *logits, const ch
     unsigned int place = i;
 #if GA_LP_CLUSTER > 1
     place = 0;
-    for (unsigned int j = 0; j < n; j++)
-      if (j % 32 < L.top) place += tops.out[j] > key;
+    for (unsigned int l = 0; l < GA_LP_CLUSTER; l++)
+#pragma unroll 4
+      for (unsigned int j = 0; j < L.top; j++) place += tops.out[l * 32 + j] > key;
     if (place >= L.top) continue;
 #endif
     if (topv != nullptr)
@@ -580,17 +607,35 @@ static __device__ __forceinline__ void ga__lp_store(char *g, long long col, long
     }
 }
 
-/* A thread owns up to GA_LP_U vectors of a row; the row's numbers come from the forward pass, so
- * that the logits are read once and the gradient written once. dlogits may be the logits. */
+/* A CTA walks a part of a row (blockDim.y rows where they are short), GA_LP_U vectors of a thread
+ * at a time, the next ones fetched before the present ones are written. The row's numbers come from
+ * the forward pass, so that the logits are read once and the gradient written once: bound by
+ * memory. The last rows come first: they are what the forward pass left in L2. dlogits may be the
+ * logits. */
+static __device__ __forceinline__ void ga__lp_fetch(const ga__lp_layout &L, const ga__lp_row &r,
+                                                    unsigned int w0, ga__lp_words q[GA_LP_U]) {
+  const unsigned int end = w0 + (GA_LP_U - 1) * blockDim.x;
+  if (GA_LP_CONTIG && w0 > 0 && end + 1 < r.nv) { /* neither the row's first nor its last vector */
+#pragma unroll
+    for (int u = 0; u < GA_LP_U; u++)
+      q[u] = *reinterpret_cast<const ga__lp_words *>(r.base + (size_t)(w0 + u * blockDim.x) * 16);
+    return;
+  }
+#pragma unroll
+  for (int u = 0; u < GA_LP_U; u++)
+    if (w0 + u * blockDim.x < r.nv) q[u] = ga__lp_load(L, r, w0 + u * blockDim.x);
+}
+
 extern "C" __global__ void __launch_bounds__(256)
 ga_lp_grad(const __grid_constant__ ga__lp_layout L, char *dlogits, const char *logits,
            const char *targets, const char *stats, const char *dlogp, const char *entropy,
            const char *dentropy, int *err) {
   ga__grid_dependency_sync();
-  const unsigned long long row = (unsigned long long)blockIdx.x * blockDim.y + threadIdx.y;
-  if (row >= L.rows) return;
+  const unsigned long long back = (unsigned long long)blockIdx.x * blockDim.y + threadIdx.y;
+  if (back >= L.rows) return;
+  const unsigned long long row = L.rows - 1 - back;
   const ga__lp_row r = ga__lp_open(L, logits, row);
-  const unsigned int w0 = blockIdx.y * blockDim.x * GA_LP_U + threadIdx.x;
+  unsigned int w0 = blockIdx.y * blockDim.x * GA_LP_U + threadIdx.x;
   if (w0 >= r.nv) return;
   char *g = dlogits + ga__lm_offset<GA_LP_ND>(row, L.dims, L.o_str[4]);
 
@@ -624,41 +669,44 @@ ga_lp_grad(const __grid_constant__ ga__lp_layout L, char *dlogits, const char *l
   const ga__f2 nm2 = ga__f2_of(-m, -m), c2 = ga__f2_of(c, c);
   const float l2 = -ls * GA_LP_LOG2E;
   const ga__f2 nl2 = ga__f2_of(l2, l2), k02 = ga__f2_of(k0, k0), k12 = ga__f2_of(k1, k1);
-  ga__lp_words q[GA_LP_U];
-  if (!none) {
+  const unsigned int step = gridDim.y * blockDim.x * GA_LP_U;
+  ga__lp_words next[GA_LP_U];
+  if (!none) ga__lp_fetch(L, r, w0, next);
+  for (; w0 < r.nv; w0 += step) {
+    ga__lp_words q[GA_LP_U];
 #pragma unroll
-    for (int u = 0; u < GA_LP_U; u++)
-      if (w0 + u * blockDim.x < r.nv) q[u] = ga__lp_load(L, r, w0 + u * blockDim.x);
-  }
+    for (int u = 0; u < GA_LP_U; u++) q[u] = next[u];
+    if (!none && w0 + step < r.nv) ga__lp_fetch(L, r, w0 + step, next);
 #pragma unroll
-  for (int u = 0; u < GA_LP_U; u++) {
-    const unsigned int w = w0 + u * blockDim.x;
-    if (w >= r.nv) break;
-    float x[2 * GA_LP_PAIRS];
-    if (none) {
+    for (int u = 0; u < GA_LP_U; u++) {
+      const unsigned int w = w0 + u * blockDim.x;
+      if (w >= r.nv) break;
+      float x[2 * GA_LP_PAIRS];
+      if (none) {
 #pragma unroll
-      for (int j = 0; j < 2 * GA_LP_PAIRS; j++) x[j] = 0.0f;
-    } else {
+        for (int j = 0; j < 2 * GA_LP_PAIRS; j++) x[j] = 0.0f;
+      } else {
 #pragma unroll
-      for (int k = 0; k < GA_LP_PAIRS; k++) {
-        float p, s;
-        ga__lp_pair(q[u], k, p, s);
-        ga__f2_to(ga__f2_fma(ga__f2_add(ga__f2_of(p, s), nm2), c2, nl2), p, s);
-        p = ga__max_nan(p, -200.0f);
-        s = ga__max_nan(s, -200.0f);
-        const ga__f2 y = ga__f2_of(p, s);
-        const ga__f2 e = ga__f2_of(ga__ex2(p), ga__ex2(s));
-        ga__f2_to(ga__f2_mul(e, ga__f2_fma(k12, y, k02)), x[2 * k], x[2 * k + 1]);
+        for (int k = 0; k < GA_LP_PAIRS; k++) {
+          float p, s;
+          ga__lp_pair(q[u], k, p, s);
+          ga__f2_to(ga__f2_fma(ga__f2_add(ga__f2_of(p, s), nm2), c2, nl2), p, s);
+          p = ga__max_nan(p, -200.0f);
+          s = ga__max_nan(s, -200.0f);
+          const ga__f2 y = ga__f2_of(p, s);
+          const ga__f2 e = ga__f2_of(ga__ex2(p), ga__ex2(s));
+          ga__f2_to(ga__f2_mul(e, ga__f2_fma(k12, y, k02)), x[2 * k], x[2 * k + 1]);
+        }
+        const unsigned int at = (unsigned int)target + r.skip - w * GA_LP_E;
+        if (target >= 0 && at < GA_LP_E) {
+#pragma unroll
+          for (int j = 0; j < GA_LP_E; j++)
+            if (at == j) x[j] += L.scale * a;
+        }
       }
-      const unsigned int at = (unsigned int)target + r.skip - w * GA_LP_E;
-      if (target >= 0 && at < GA_LP_E) {
-#pragma unroll
-        for (int j = 0; j < GA_LP_E; j++)
-          if (at == j) x[j] += L.scale * a;
-      }
+      const long long i = (long long)w * GA_LP_E - r.skip; /* below 0 where the row starts inside the vector */
+      ga__lp_store(g, L.o_col[4], i, i < 0 ? r.skip : 0, L.v, x, ga__lp_whole(L, r, w));
     }
-    const long long i = (long long)w * GA_LP_E - r.skip; /* below 0 where the row starts inside the vector */
-    ga__lp_store(g, L.o_col[4], i, i < 0 ? r.skip : 0, L.v, x, ga__lp_whole(L, r, w));
   }
 }
 #endif

@@ -170,7 +170,7 @@ def grad_tol(want, size, counts, dtype, f64):
 
 GRAD_CASES = [  # tokens, rows, width
     (1, 1, 1), (1, 5, 8), (2, 1, 3), (7, 3, 16), (40, 6, 5), (64, 64, 24), (100, 2, 9), (257, 30, 12), (300, 1, 4),
-    (512, 40, 33), (513, 3, 4), (2600, 600, 9), (5000, 511, 3), (700, 300000, 1),
+    (512, 40, 33), (513, 3, 4), (2600, 600, 9), (5000, 511, 3), (700, 300000, 1), (17000, 900, 2),
 ]
 
 

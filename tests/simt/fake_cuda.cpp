@@ -45,6 +45,13 @@ static std::string env(const char *name) {
   return v != NULL ? v : "";
 }
 
+/* CTAs of a cluster of the kernel: a C expression over the text's macros */
+static std::string cluster_of(const std::string &text, const char *kernel) {
+  if (strcmp(kernel, "ga_eg_sort_all") == 0) return "GA_EG_CLUSTER";
+  if (strcmp(kernel, "ga_lp_rows") == 0) return "GA_LP_CLUSTER";
+  return "1";
+}
+
 extern "C" {
 void fake_cuda_set_capturing(int on) { capturing = on; }
 
@@ -142,8 +149,12 @@ CUresult cuModuleGetFunction(CUfunction *f, CUmodule m, const char *name) {
       "template <class... A> static void simt_spread(void (*f)(A...), void **p) {\n"
       "  simt_call(f, p, std::index_sequence_for<A...>());\n}\n"
       "static void simt_body(void *p) { simt_spread(" + std::string(name) + ", (void **)p); }\n"
+      "namespace simt { void run_clusters(void (*)(void *), void *, simt_dim3, simt_dim3, unsigned); }\n"
       "extern \"C\" void simt_entry(void **p, const unsigned *g, const unsigned *b) {\n"
-      "  simt::run_grid(simt_body, p, simt_dim3{g[0], g[1], g[2]}, simt_dim3{b[0], b[1], b[2]});\n}\n";
+      "  const simt_dim3 grid{g[0], g[1], g[2]}, block{b[0], b[1], b[2]};\n"
+      "  const unsigned cluster = " + cluster_of(((fake_module *)m)->text, name) + ";\n"
+      "  if (cluster > 1) simt::run_clusters(simt_body, p, grid, block, cluster);\n"
+      "  else simt::run_grid(simt_body, p, grid, block);\n}\n";
   std::string all = text; /* the key covers every header that the text may include */
   const std::string dirs[2] = {env("SIMT_TEMPLATES"), env("SIMT_DIR") + "/include"};
   for (const std::string &dir : dirs) {
@@ -157,6 +168,7 @@ CUresult cuModuleGetFunction(CUfunction *f, CUmodule m, const char *name) {
     }
     for (const std::string &n : names) all += slurp(dir + "/" + n);
   }
+  all += slurp(env("SIMT_DIR") + "/simt_runtime.cpp") + slurp(env("SIMT_DIR") + "/simt_cluster.cpp");
   char key[40];
   snprintf(key, sizeof(key), "%016zx", std::hash<std::string>()(all));
   const std::string base = env("SIMT_BUILD") + "/lm_" + key, so = base + ".so";
@@ -171,7 +183,7 @@ CUresult cuModuleGetFunction(CUfunction *f, CUmodule m, const char *name) {
     fclose(o);
     const std::string cmd = "g++ -std=c++17 -O1 -shared -fPIC -w -include ga_lm_ptx.cuh -I" + env("SIMT_DIR") + "/include -I" +
                             env("SIMT_TEMPLATES") + " " + cpp + " " + env("SIMT_DIR") +
-                            "/simt_runtime.cpp -o " + tmp + " > " + log + " 2>&1";
+                            "/simt_runtime.cpp " + env("SIMT_DIR") + "/simt_cluster.cpp -o " + tmp + " > " + log + " 2>&1";
     if (system(cmd.c_str()) != 0) {
       fprintf(stderr, "%s\n%s\n", cmd.c_str(), slurp(log).substr(0, 4000).c_str());
       return CUDA_ERROR_INVALID_SOURCE;

@@ -1,7 +1,7 @@
 /* Host stand-in for templates/ga_lm_ptx.cuh under the SIMT emulator: the same
  * operations in plain C++, and the intrinsics the language-model templates use
- * beyond those of simt_emul.h. Thread-block clusters are not emulated (CTAs run
- * one after the other). */
+ * beyond those of simt_emul.h. The CTAs of a cluster run together
+ * (simt_cluster.cpp), each with shared memory of its own. */
 #ifndef GA_LM_PTX_CUH
 #define GA_LM_PTX_CUH
 #include "cluda.h"
@@ -83,6 +83,8 @@ static inline void ga__st32(char *p, const unsigned int w[8]) {
   if ((size_t)p % 32 != 0) abort();
   memcpy(p, w, 32);
 }
+static inline void ga__grid_dependency_wait() {}
+static inline void ga__grid_dependency_release() {}
 struct ga__f2 {
   float a, b;
 };
@@ -95,5 +97,25 @@ static inline ga__f2 ga__f2_add(ga__f2 x, ga__f2 y) { return ga__f2{x.a + y.a, x
 static inline ga__f2 ga__f2_mul(ga__f2 x, ga__f2 y) { return ga__f2{x.a * y.a, x.b * y.b}; }
 static inline ga__f2 ga__f2_fma(ga__f2 x, ga__f2 y, ga__f2 z) {
   return ga__f2{fmaf(x.a, y.a, z.a), fmaf(x.b, y.b, z.b)};
+}
+
+/* ---- shared memory and clusters ---- */
+namespace simt {
+extern unsigned cluster_rank;   /* of the running CTA */
+char *shared_of(unsigned rank); /* a CTA's shared memory */
+void cluster_arrive();
+void cluster_wait();
+}
+#define GA_LM_SHARED(type, name) type &name = *reinterpret_cast<type *>(simt::shared_of(simt::cluster_rank))
+#define GA_LM_SHARED_DYNAMIC(type, name) GA_LM_SHARED(type, name)
+#define __cluster_dims__(...)
+static inline unsigned int ga__cluster_rank() { return simt::cluster_rank; }
+static inline void ga__cluster_arrive() { simt::cluster_arrive(); }
+static inline void ga__cluster_wait() { simt::cluster_wait(); }
+template <typename T>
+static inline void ga__cluster_put(T *p, unsigned int rank, T v) {
+  const size_t at = (char *)p - simt::shared_of(simt::cluster_rank);
+  if (at >= 256 * 1024) abort(); /* not in this CTA's shared memory */
+  memcpy(simt::shared_of(rank) + at, &v, sizeof(T));
 }
 #endif
