@@ -223,7 +223,7 @@ int GpuLogProbs_call(GpuLogProbs *lp, GpuArray *logp, GpuArray *entropy, GpuArra
   /* Few rows: several CTAs share one, as long as the device holds them all and each has at least
    * one full step of loads. */
   if (v.group > 32)
-    while (v.cluster < (getenv("LPC") ? (unsigned)atoi(getenv("LPC")) : 8u) && L.rows * v.cluster * 2 * v.threads <= (unsigned long long)ctx->num_sms * 2048 &&
+    while (v.cluster < (getenv("LPC") ? (unsigned)atoi(getenv("LPC")) : 8u) && L.rows * v.cluster * 2 * v.threads <= (unsigned long long)ctx->num_sms * 2048 * (getenv("LPX") ? atoi(getenv("LPX")) : 1) &&
            row_vectors(&L, e) >= (unsigned long long)v.cluster * 2 * v.threads * 4)
       v.cluster *= 2;
   err = ga_lm_kernel(ctx, "ga_lp_rows", variant_key(&v), emit, &fn);

@@ -120,6 +120,36 @@ static __device__ __forceinline__ ga__lp_words ga__lp_load(const ga__lp_layout &
   return ga__lp_load_part(L, r, w);
 }
 
+/* A CTA's vectors [v0, v1) of a row: those in [f0, f1) are whole, or elements apart by themselves;
+ * the row's first or last one may be a part of a vector (GA_LP_NONE: it is not). The thread
+ * `lane` of `group` has f0 + lane, f0 + lane + group ...; thread 0 also p0, thread 1 also p1. */
+#define GA_LP_NONE 0xffffffffu
+struct ga__lp_share {
+  unsigned int v0, v1, f0, f1, p0, p1;
+};
+static __device__ __forceinline__ ga__lp_share ga__lp_split(const ga__lp_layout &L, const ga__lp_row &r,
+                                                            unsigned int part, unsigned int parts) {
+  ga__lp_share s;
+  const unsigned int each = (r.nv + parts - 1) / parts;
+  s.v0 = part * each < r.nv ? part * each : r.nv;
+  s.v1 = r.nv - s.v0 < each ? r.nv : s.v0 + each;
+  s.f0 = s.v0;
+  s.f1 = s.v1;
+  s.p0 = s.p1 = GA_LP_NONE;
+  if (s.v0 < s.v1 && s.v0 == 0 && r.skip > 0) s.p0 = s.f0++;
+  if (s.f0 < s.f1 && s.v1 == r.nv && r.nv * GA_LP_E - r.skip > L.v) s.p1 = --s.f1;
+  return s;
+}
+static __device__ __forceinline__ unsigned int ga__lp_extra(const ga__lp_share &s, unsigned int lane) {
+  return lane == 0 ? s.p0 : lane == 1 ? s.p1 : GA_LP_NONE;
+}
+/* one of [f0, f1) */
+static __device__ __forceinline__ ga__lp_words ga__lp_load_whole(const ga__lp_layout &L, const ga__lp_row &r,
+                                                                 unsigned int w) {
+  if (GA_LP_CONTIG) return *reinterpret_cast<const ga__lp_words *>(r.base + (size_t)w * 16);
+  return ga__lp_load_part(L, r, w);
+}
+
 static __device__ __forceinline__ float ga__lp_z(const char *p) {
 #if GA_LP_ZTYPE == 0
   return ga_half2float(*reinterpret_cast<const ga_half *>(p));
@@ -153,14 +183,21 @@ struct ga__lp_state {
   float m, s, t;
 };
 
-static __device__ __forceinline__ ga__lp_state ga__lp_merge(ga__lp_state a, ga__lp_state b, float c) {
-  ga__lp_state r;
-  r.m = fmaxf(a.m, b.m);
-  const float da = ga__max_nan((a.m - r.m) * c, GA_LP_YMIN), db = ga__max_nan((b.m - r.m) * c, GA_LP_YMIN);
-  const float fa = ga__ex2(da), fb = ga__ex2(db);
-  r.s = a.s * fa + b.s * fb;
-  r.t = (a.t + a.s * da) * fa + (b.t + b.s * db) * fb;
-  return r;
+/* The states of `width` lanes (a power of two) as one, the same bits in each of them. */
+static __device__ __forceinline__ ga__lp_state ga__lp_merge(ga__lp_state a, float c, int width) {
+  float m = a.m;
+#pragma unroll
+  for (int d = width / 2; d > 0; d /= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+  const float d = ga__max_nan((a.m - m) * c, GA_LP_YMIN), f = ga__ex2(d);
+  a.t = (a.t + a.s * d) * f;
+  a.s *= f;
+  a.m = m;
+#pragma unroll
+  for (int d = width / 2; d > 0; d /= 2) {
+    a.s += __shfl_xor_sync(0xffffffffu, a.s, d);
+    a.t += __shfl_xor_sync(0xffffffffu, a.t, d);
+  }
+  return a;
 }
 
 static __device__ __forceinline__ float ga__lp_max(const ga__lp_words &q) {
@@ -177,6 +214,47 @@ static __device__ __forceinline__ float ga__lp_max(const ga__lp_words &q) {
   for (int j = 1; j < GA_LP_W; j++) a = fmaxf(a, __uint_as_float(q.w[j]));
   return a;
 #endif
+}
+
+/* N vectors into a thread's state: the sums are kept in pairs beside it. */
+template <int N>
+static __device__ __forceinline__ void ga__lp_step(const ga__lp_words q[N], float c, ga__lp_state &st,
+                                                   ga__f2 &s2, ga__f2 &t2) {
+  float top = ga__lp_max(q[0]);
+#pragma unroll
+  for (int u = 1; u < N; u++) top = fmaxf(top, ga__lp_max(q[u]));
+  if (top > st.m) {
+    const float d = ga__max_nan((st.m - top) * c, GA_LP_YMIN), f = ga__ex2(d);
+    const ga__f2 f2 = ga__f2_of(f, f);
+#if GA_LP_ENT
+    t2 = ga__f2_mul(ga__f2_fma(s2, ga__f2_of(d, d), t2), f2);
+#endif
+    s2 = ga__f2_mul(s2, f2);
+    st.m = top;
+  }
+  const ga__f2 c2 = ga__f2_of(c, c);
+#pragma unroll
+  for (int u = 0; u < N; u++)
+#pragma unroll
+    for (int k = 0; k < GA_LP_PAIRS; k++) {
+      float a, b;
+#if GA_LP_ZTYPE == 0
+      ga__add_h2_f32(q[u].w[k], -st.m, a, b);
+      ga__f2_to(ga__f2_mul(ga__f2_of(a, b), c2), a, b);
+#else
+      ga__lp_pair(q[u], k, a, b);
+      ga__f2_to(ga__f2_mul(ga__f2_add(ga__f2_of(a, b), ga__f2_of(-st.m, -st.m)), c2), a, b);
+#endif
+#if GA_LP_ENT
+      a = ga__max_nan(a, GA_LP_YMIN); /* e y is 0 for a logit of -inf */
+      b = ga__max_nan(b, GA_LP_YMIN);
+#endif
+      const ga__f2 e2 = ga__f2_of(ga__ex2(a), ga__ex2(b));
+      s2 = ga__f2_add(s2, e2);
+#if GA_LP_ENT
+      t2 = ga__f2_fma(e2, ga__f2_of(a, b), t2);
+#endif
+    }
 }
 
 #if GA_LP_TOP
@@ -209,12 +287,24 @@ static __device__ __forceinline__ void ga__lp_keys(const ga__lp_layout &L, const
   }
 }
 
+/* The vector's largest key where it holds a value of m or more, else 0. */
+static __device__ __forceinline__ unsigned long long ga__lp_best(const ga__lp_layout &L, const ga__lp_row &r,
+                                                                 unsigned int w, float m) {
+  unsigned long long k[2 * GA_LP_PAIRS], best = 0;
+  if (!(ga__lp_max(ga__lp_load(L, r, w)) >= m)) return 0;
+  ga__lp_keys(L, r, w, k);
+#pragma unroll
+  for (int j = 0; j < 2 * GA_LP_PAIRS; j++) best = k[j] > best ? k[j] : best;
+  return best;
+}
+
 struct ga__lp_top_smem {
   unsigned long long cand[GA_LP_CAND];
   unsigned long long best[GA_LP_THREADS];
   unsigned long long out[GA_LP_CLUSTER * 32]; /* the CTAs' lists, in the first CTA of a cluster */
   unsigned int high[GA_LP_THREADS];
   unsigned int list[GA_LP_THREADS];
+  unsigned long long tau;
   unsigned int nlist, ncand, count;
 };
 
@@ -235,14 +325,18 @@ static __device__ __forceinline__ K ga__lp_nth(K mine, unsigned int top) {
 
 /* Appends the keys from `tau` on of the listed threads' vectors (or of all) to the candidates. */
 static __device__ __forceinline__ void ga__lp_collect(const ga__lp_layout &L, const ga__lp_row &r,
-                                                      unsigned int v0, unsigned int v1, int all,
+                                                      const ga__lp_share &sh, int all,
                                                       unsigned long long tau, ga__lp_top_smem &S) {
-  const unsigned int per = (v1 - v0 + GA_LP_THREADS - 1) / GA_LP_THREADS;
-  const unsigned int items = all ? v1 - v0 : S.nlist * per;
+  const unsigned int whole = (sh.f1 - sh.f0 + GA_LP_THREADS - 1) / GA_LP_THREADS;
+  const unsigned int items = all ? sh.v1 - sh.v0 : S.nlist * (whole + 1);
   for (unsigned int it = threadIdx.x; it < items; it += GA_LP_THREADS) {
     if (*(volatile unsigned int *)&S.ncand > GA_LP_CAND) break; /* too many: they are not used */
-    const unsigned int w = v0 + (all ? it : S.list[it / per] + (it % per) * GA_LP_THREADS);
-    if (w >= v1) continue;
+    unsigned int w = sh.v0 + it;
+    if (!all) {
+      const unsigned int t = S.list[it / (whole + 1)], j = it % (whole + 1);
+      w = j < whole ? sh.f0 + t + j * GA_LP_THREADS : ga__lp_extra(sh, t);
+      if (j < whole ? w >= sh.f1 : w == GA_LP_NONE) continue;
+    }
     unsigned long long k[2 * GA_LP_PAIRS];
     ga__lp_keys(L, r, w, k);
 #pragma unroll
@@ -255,7 +349,7 @@ static __device__ __forceinline__ void ga__lp_collect(const ga__lp_layout &L, co
   __syncthreads();
 }
 
-/* The `top` largest keys of vectors [v0, v1) of the row, into out[0..32) of this CTA's or the
+/* The `top` largest keys of a CTA's vectors of the row, into out[0..32) of this CTA's or the
  * cluster's first CTA's shared memory (0 where there are fewer). All threads of the CTA, after a
  * barrier behind which S.high has every thread's largest value and the counters are 0; m: this
  * thread's.
@@ -268,34 +362,36 @@ static __device__ __forceinline__ void ga__lp_collect(const ga__lp_layout &L, co
  * with keys that break ties by the index; where that is still too much (a row that hides its
  * largest elements in few threads' vectors) or NaNs are about (`odd`), tau is found by halving
  * over the row. */
-static __device__ void ga__lp_top(const ga__lp_layout &L, const ga__lp_row &r, unsigned int v0,
-                                  unsigned int v1, float m, int odd, ga__lp_top_smem &S) {
+static __device__ void ga__lp_top(const ga__lp_layout &L, const ga__lp_row &r, const ga__lp_share &sh,
+                                  float m, int odd, ga__lp_top_smem &S) {
   const unsigned int tid = threadIdx.x, lane = tid % 32;
   unsigned long long k[2 * GA_LP_PAIRS], tau = 0;
   if (!odd) {
-    unsigned int high = 0;
+    if (tid < 32) {
+      unsigned int high = 0;
 #pragma unroll
-    for (int j = 0; j < GA_LP_THREADS / 32; j++) {
-      const unsigned int b = S.high[j * 32 + lane];
-      high = b > high ? b : high;
+      for (int j = 0; j < GA_LP_THREADS / 32; j++) {
+        const unsigned int b = S.high[j * 32 + lane];
+        high = b > high ? b : high;
+      }
+      high = ga__lp_nth(high, L.top);
+      if (lane == 0) S.tau = (unsigned long long)high << 32;
     }
-    tau = (unsigned long long)ga__lp_nth(high, L.top) << 32;
+    __syncthreads();
+    tau = S.tau;
     const float minus_inf = __uint_as_float(0xff800000u);
     const int few = (tau >> 32) == (ga__lp_key(minus_inf, 0) >> 32); /* fewer above -inf than asked for */
     if (!few) {
-      if (v0 + tid < v1 && ga__lp_key(m, 0) >= tau) S.list[atomicAdd(&S.nlist, 1u)] = tid;
+      if (S.high[tid] > 0 && ga__lp_key(m, 0) >= tau) S.list[atomicAdd(&S.nlist, 1u)] = tid;
       __syncthreads();
-      ga__lp_collect(L, r, v0, v1, 0, tau, S);
+      ga__lp_collect(L, r, sh, 0, tau, S);
     }
     if (few || S.ncand > GA_LP_CAND) { /* the same in every thread */
       unsigned long long mine = 0;
-      for (unsigned int w = v0 + tid; w < v1; w += GA_LP_THREADS) /* its first place */
-        if (ga__lp_max(ga__lp_load(L, r, w)) >= m) {
-          ga__lp_keys(L, r, w, k);
-#pragma unroll
-          for (int j = 0; j < 2 * GA_LP_PAIRS; j++) mine = k[j] > mine ? k[j] : mine;
-          break;
-        }
+      /* its first place: p0 is before the whole vectors, p1 behind them */
+      if (tid == 0 && sh.p0 != GA_LP_NONE) mine = ga__lp_best(L, r, sh.p0, m);
+      for (unsigned int w = sh.f0 + tid; mine == 0 && w < sh.f1; w += GA_LP_THREADS) mine = ga__lp_best(L, r, w, m);
+      if (mine == 0 && tid == 1 && sh.p1 != GA_LP_NONE) mine = ga__lp_best(L, r, sh.p1, m);
       S.best[tid] = mine;
       __syncthreads();
       if (tid == 0) S.nlist = S.ncand = 0;
@@ -309,7 +405,7 @@ static __device__ void ga__lp_top(const ga__lp_layout &L, const ga__lp_row &r, u
       __syncthreads();
       if (mine >= tau) S.list[atomicAdd(&S.nlist, 1u)] = tid;
       __syncthreads();
-      ga__lp_collect(L, r, v0, v1, 0, tau, S);
+      ga__lp_collect(L, r, sh, 0, tau, S);
     }
   }
   if (odd || S.ncand > GA_LP_CAND) { /* the same in every thread */
@@ -322,7 +418,7 @@ static __device__ void ga__lp_top(const ga__lp_layout &L, const ga__lp_row &r, u
       __syncthreads();
       if (tid == 0) S.count = 0;
       __syncthreads();
-      for (unsigned int w = v0 + tid; w < v1; w += GA_LP_THREADS) {
+      for (unsigned int w = sh.v0 + tid; w < sh.v1; w += GA_LP_THREADS) {
         ga__lp_keys(L, r, w, k);
 #pragma unroll
         for (int j = 0; j < 2 * GA_LP_PAIRS; j++) c += k[j] >= mid;
@@ -338,7 +434,7 @@ static __device__ void ga__lp_top(const ga__lp_layout &L, const ga__lp_row &r, u
     tau = lo;
     if (tid == 0) S.ncand = 0;
     __syncthreads();
-    ga__lp_collect(L, r, v0, v1, 1, tau, S);
+    ga__lp_collect(L, r, sh, 1, tau, S);
   }
   /* a key's place is the number of larger ones */
   const unsigned int n = S.ncand < GA_LP_CAND ? S.ncand : GA_LP_CAND;
@@ -395,9 +491,7 @@ ga_lp_rows(const __grid_constant__ ga__lp_layout L, const char *logits, const ch
   ga__cluster_arrive(); /* waited for before the first store to another CTA's shared memory */
 #endif
   const ga__lp_row r = ga__lp_open(L, logits, row);
-  const unsigned int share = (r.nv + GA_LP_CLUSTER - 1) / GA_LP_CLUSTER;
-  const unsigned int v0 = part * share < r.nv ? part * share : r.nv;
-  const unsigned int v1 = r.nv - v0 < share ? r.nv : v0 + share;
+  const ga__lp_share my = ga__lp_split(L, r, part, GA_LP_CLUSTER);
   const float c = L.scale * GA_LP_LOG2E;
 
   /* the target's logit is fetched while the row streams */
@@ -411,53 +505,26 @@ ga_lp_rows(const __grid_constant__ ga__lp_layout L, const char *logits, const ch
 
   ga__lp_state st = {GA_LP_NOTHING, 0.0f, 0.0f};
   ga__f2 s2 = ga__f2_of(0.0f, 0.0f), t2 = s2;
-  const ga__f2 c2 = ga__f2_of(c, c);
-  for (unsigned int w = v0 + lane; w < v1; w += GA_LP_GROUP * GA_LP_U) {
+  const unsigned int extra = ga__lp_extra(my, lane);
+  unsigned int w = my.f0 + lane;
+  for (; w + (GA_LP_U - 1) * GA_LP_GROUP < my.f1; w += GA_LP_U * GA_LP_GROUP) {
     ga__lp_words q[GA_LP_U];
-    float top = GA_LP_NOTHING;
-    if (GA_LP_CONTIG && w > 0 && w + (GA_LP_U - 1) * GA_LP_GROUP < v1 &&
-        w + (GA_LP_U - 1) * GA_LP_GROUP + 1 < r.nv) { /* neither the row's first nor its last vector */
 #pragma unroll
-      for (int u = 0; u < GA_LP_U; u++)
-        q[u] = *reinterpret_cast<const ga__lp_words *>(r.base + (size_t)(w + u * GA_LP_GROUP) * 16);
-    } else {
+    for (int u = 0; u < GA_LP_U; u++) q[u] = ga__lp_load_whole(L, r, w + u * GA_LP_GROUP);
+    ga__lp_step<GA_LP_U>(q, c, st, s2, t2);
+  }
+  { /* fewer than GA_LP_U are left: all of them in flight, then one at a time */
+    ga__lp_words q[GA_LP_U];
 #pragma unroll
-      for (int u = 0; u < GA_LP_U; u++) {
-        if (w + u * GA_LP_GROUP < v1) q[u] = ga__lp_load(L, r, w + u * GA_LP_GROUP);
-        else {
+    for (int u = 0; u + 1 < GA_LP_U; u++)
+      if (w + u * GA_LP_GROUP < my.f1) q[u] = ga__lp_load_whole(L, r, w + u * GA_LP_GROUP);
+    if (extra != GA_LP_NONE) q[GA_LP_U - 1] = ga__lp_load_part(L, r, extra);
+#pragma unroll 1
+    for (int u = 0; u < GA_LP_U; u++) {
+      if (u + 1 < GA_LP_U ? w + u * GA_LP_GROUP < my.f1 : extra != GA_LP_NONE) ga__lp_step<1>(&q[0], c, st, s2, t2);
 #pragma unroll
-          for (int j = 0; j < GA_LP_W; j++)
-            q[u].w[j] = GA_LP_ZTYPE == 0 ? (GA_LP_MINUS_INF | GA_LP_MINUS_INF << 16) : GA_LP_MINUS_INF;
-        }
-      }
+      for (int i = 0; i + 1 < GA_LP_U; i++) q[i] = q[i + 1];
     }
-#pragma unroll
-    for (int u = 0; u < GA_LP_U; u++) top = fmaxf(top, ga__lp_max(q[u]));
-    if (top > st.m) {
-      const float d = ga__max_nan((st.m - top) * c, GA_LP_YMIN), f = ga__ex2(d);
-      const ga__f2 f2 = ga__f2_of(f, f);
-#if GA_LP_ENT
-      t2 = ga__f2_mul(ga__f2_fma(s2, ga__f2_of(d, d), t2), f2);
-#endif
-      s2 = ga__f2_mul(s2, f2);
-      st.m = top;
-    }
-    const ga__f2 nm2 = ga__f2_of(-st.m, -st.m);
-#pragma unroll
-    for (int u = 0; u < GA_LP_U; u++)
-#pragma unroll
-      for (int k = 0; k < GA_LP_PAIRS; k++) {
-        float a, b;
-        ga__lp_pair(q[u], k, a, b);
-        ga__f2_to(ga__f2_mul(ga__f2_add(ga__f2_of(a, b), nm2), c2), a, b);
-        a = ga__max_nan(a, GA_LP_YMIN);
-        b = ga__max_nan(b, GA_LP_YMIN);
-        const ga__f2 e2 = ga__f2_of(ga__ex2(a), ga__ex2(b));
-        s2 = ga__f2_add(s2, e2);
-#if GA_LP_ENT
-        t2 = ga__f2_fma(e2, ga__f2_of(a, b), t2);
-#endif
-      }
   }
   {
     float a, b;
@@ -470,39 +537,21 @@ ga_lp_rows(const __grid_constant__ ga__lp_layout L, const char *logits, const ch
 #if GA_LP_TOP
   ga__lp_top_smem &tops = sh.tops;
   const float most = st.s == 0.0f ? __uint_as_float(0xff800000u) : st.m; /* this thread's largest */
-  tops.high[threadIdx.x] = v0 + lane < v1 ? (unsigned int)(ga__lp_key(most, 0) >> 32) : 0;
+  tops.high[threadIdx.x] =
+      my.f0 + lane < my.f1 || extra != GA_LP_NONE ? (unsigned int)(ga__lp_key(most, 0) >> 32) : 0;
   if (threadIdx.x == 0) tops.nlist = tops.ncand = 0;
 #endif
-#pragma unroll
-  for (int d = 16; d > 0; d /= 2) {
-    ga__lp_state o;
-    o.m = __shfl_xor_sync(0xffffffffu, st.m, d);
-    o.s = __shfl_xor_sync(0xffffffffu, st.s, d);
-    o.t = __shfl_xor_sync(0xffffffffu, st.t, d);
-    st = ga__lp_merge(st, o, c);
-  }
+  st = ga__lp_merge(st, c, 32);
 #if GA_LP_GROUP > 32
   if (threadIdx.x % 32 == 0) sh.warps[threadIdx.x / 32] = st;
   __syncthreads();
-  /* every warp merges the warps' states in the same order: the same bits everywhere */
-  st = sh.warps[threadIdx.x % (GA_LP_THREADS / 32)];
-#pragma unroll
-  for (int d = GA_LP_THREADS / 64; d > 0; d /= 2) {
-    ga__lp_state o;
-    o.m = __shfl_xor_sync(0xffffffffu, st.m, d);
-    o.s = __shfl_xor_sync(0xffffffffu, st.s, d);
-    o.t = __shfl_xor_sync(0xffffffffu, st.t, d);
-    st = ga__lp_merge(st, o, c);
-  }
-  st.m = __shfl_sync(0xffffffffu, st.m, 0);
-  st.s = __shfl_sync(0xffffffffu, st.s, 0);
-  st.t = __shfl_sync(0xffffffffu, st.t, 0);
+  st = ga__lp_merge(sh.warps[threadIdx.x % (GA_LP_THREADS / 32)], c, GA_LP_THREADS / 32);
 #endif
 #if GA_LP_CLUSTER > 1
   ga__cluster_wait(); /* every CTA of the cluster runs */
 #endif
 #if GA_LP_TOP
-  ga__lp_top(L, r, v0, v1, most, !(st.s == st.s), tops);
+  ga__lp_top(L, r, my, most, !(st.s == st.s), tops);
 #endif
 #if GA_LP_CLUSTER > 1
   /* the CTAs' states and lists meet in the first one */
@@ -513,13 +562,12 @@ ga_lp_rows(const __grid_constant__ ga__lp_layout L, const char *logits, const ch
   ga__cluster_arrive();
   ga__cluster_wait();
   if (part != 0) return;
-#pragma unroll 1
-  for (int i = 0; i < GA_LP_CLUSTER; i++) {
-    ga__lp_state o;
-    o.m = __uint_as_float((unsigned int)(sh.parts[i][0] >> 32));
-    o.s = __uint_as_float((unsigned int)sh.parts[i][0]);
-    o.t = __uint_as_float((unsigned int)sh.parts[i][1]);
-    st = i == 0 ? o : ga__lp_merge(st, o, c);
+  {
+    const unsigned int i = threadIdx.x % GA_LP_CLUSTER;
+    st.m = __uint_as_float((unsigned int)(sh.parts[i][0] >> 32));
+    st.s = __uint_as_float((unsigned int)sh.parts[i][0]);
+    st.t = __uint_as_float((unsigned int)sh.parts[i][1]);
+    st = ga__lp_merge(st, c, GA_LP_CLUSTER);
   }
 #endif
   const int empty = st.s == 0.0f;

@@ -66,6 +66,11 @@ static inline void ga__unpack_h2(unsigned int w, float &lo, float &hi) {
   lo = ga_half2float(l);
   hi = ga_half2float(h);
 }
+static inline void ga__add_h2_f32(unsigned int w, float c, float &lo, float &hi) {
+  ga__unpack_h2(w, lo, hi);
+  lo += c;
+  hi += c;
+}
 static inline unsigned int ga__pack_h2(float lo, float hi) {
   return (unsigned int)ga_float2half(lo).data | (unsigned int)ga_float2half(hi).data << 16;
 }
