@@ -23,15 +23,17 @@ struct _GpuLogProbs {
 };
 
 typedef struct lp_variant {
-  int z_tc, i_tc, g_tc, grad, contig, ent, top;
+  int z_tc, i_tc, g_tc, grad, contig, ent, top, fold;
   unsigned threads, group, cluster, nd;
 } lp_variant;
+
+#define LP_U 4 /* vectors of a thread in one step: GA_LP_U of the template */
 
 static uint64_t variant_key(const lp_variant *v) {
   return (uint64_t)v->z_tc | (uint64_t)v->i_tc << 8 | (uint64_t)v->g_tc << 16 |
          (uint64_t)(v->threads / 32) << 24 | (uint64_t)(v->group / 32) << 32 |
          (uint64_t)v->cluster << 40 | (uint64_t)v->nd << 48 | (uint64_t)v->grad << 56 |
-         (uint64_t)v->contig << 57 | (uint64_t)v->ent << 58 | (uint64_t)v->top << 59;
+         (uint64_t)v->contig << 57 | (uint64_t)v->ent << 58 | (uint64_t)v->top << 59 | (uint64_t)v->fold << 60;
 }
 
 static void emit(ga_strb *sb, uint64_t key) {
@@ -49,9 +51,9 @@ static void emit(ga_strb *sb, uint64_t key) {
   else
     ga_strb_printf(sb,
                    "#define GA_LP_THREADS %u\n#define GA_LP_GROUP %u\n#define GA_LP_CLUSTER %u\n"
-                   "#define GA_LP_TOP %u\n",
+                   "#define GA_LP_TOP %u\n#define GA_LP_FOLD %u\n",
                    (unsigned)((key >> 24) & 0xff) * 32, (unsigned)((key >> 32) & 0xff) * 32,
-                   (unsigned)((key >> 40) & 0xff), (unsigned)((key >> 59) & 1));
+                   (unsigned)((key >> 40) & 0xff), (unsigned)((key >> 59) & 1), (unsigned)((key >> 60) & 1));
   ga_strb_puts(sb, "#include \"ga_logprobs.cuh\"\n");
 }
 
@@ -165,6 +167,32 @@ static unsigned long long row_vectors(const lp_layout *L, unsigned e) {
   return e == 1 ? L->v : ((unsigned long long)L->v + 2 * (e - 1)) / e;
 }
 
+/* Threads and CTAs for a row of nv vectors. Many short rows: a warp each, which has nothing to wait
+ * for but itself ((16384, 4000) halfs 33 us, with 5 alternatives 49; a CTA each 47 and 88). Many
+ * long rows: CTAs of 128 threads, 8 of them an SM, as more threads only make the last wave longer
+ * ((2047, 50021) halfs: 39 us with 128, 41 with 256). Fewer: 256 or 512, where the row gives each
+ * thread enough to do ((700, 131072) halfs: 35 us with 512, 39 with 256, 51 with 128), and 512
+ * where all rows are on the device at once; then up to 8 CTAs in a cluster, as long as the device
+ * holds them and each has a full step of loads (3 rows of 131072 halfs, 20 alternatives: 8.6 us;
+ * one CTA for a row 13.2). */
+static void choose_shape(lp_variant *v, unsigned long long rows, unsigned long long nv, unsigned num_sms) {
+  const unsigned long long device = (unsigned long long)num_sms * 1024; /* threads it holds at once */
+  v->threads = v->top ? 128 : 256; /* a warp's lists are 7 KiB of shared memory */
+  v->group = 32;
+  v->cluster = 1;
+  if (nv <= 64 || (nv <= (v->top ? 1024u : 2048u) && rows >= (unsigned long long)num_sms * 16)) return;
+  v->threads = 128;
+  if (rows <= (unsigned long long)num_sms * 8 && nv >= 256 * LP_U * 3) v->threads = 256;
+  if (rows <= (unsigned long long)num_sms * 8 && nv >= 512 * LP_U * 6) v->threads = 512;
+  if (rows * 512 <= device && nv >= 512 * LP_U) v->threads = 512;
+  while (v->cluster < 8 && rows * v->cluster * 2 * v->threads <= device &&
+         nv >= (unsigned long long)v->cluster * 2 * v->threads * LP_U)
+    v->cluster *= 2;
+  v->group = v->threads;
+}
+
+#define LP_FOLD_SCALE 64.0f /* halfs times this and log2 e stay below 2^23 */
+
 int GpuLogProbs_call(GpuLogProbs *lp, GpuArray *logp, GpuArray *entropy, GpuArray *stats,
                      GpuArray *top_logp, GpuArray *top_ids, const GpuArray *logits,
                      const GpuArray *targets, double scale, ssize_t ignore, int flags) {
@@ -216,16 +244,9 @@ int GpuLogProbs_call(GpuLogProbs *lp, GpuArray *logp, GpuArray *entropy, GpuArra
   if (L.v == 1) L.z_col = (long long)es;
   v.ent = entropy != NULL;
   v.top = top_logp != NULL || top_ids != NULL;
+  v.fold = lp->z_tc == GA_HALF && L.scale <= LP_FOLD_SCALE;
   e = v.contig ? 16 / (unsigned)es : 1;
-  v.threads = getenv("LPT") ? (unsigned)atoi(getenv("LPT")) : 256;
-  v.cluster = 1;
-  v.group = !v.top && row_vectors(&L, e) <= 512 ? 32 : v.threads;
-  /* Few rows: several CTAs share one, as long as the device holds them all and each has at least
-   * one full step of loads. */
-  if (v.group > 32)
-    while (v.cluster < (getenv("LPC") ? (unsigned)atoi(getenv("LPC")) : 8u) && L.rows * v.cluster * 2 * v.threads <= (unsigned long long)ctx->num_sms * 2048 * (getenv("LPX") ? atoi(getenv("LPX")) : 1) &&
-           row_vectors(&L, e) >= (unsigned long long)v.cluster * 2 * v.threads * 4)
-      v.cluster *= 2;
+  choose_shape(&v, L.rows, row_vectors(&L, e), ctx->num_sms);
   err = ga_lm_kernel(ctx, "ga_lp_rows", variant_key(&v), emit, &fn);
   if (err != GA_NO_ERROR) return err;
   block[0] = v.threads;
@@ -243,7 +264,6 @@ int GpuLogProbs_call(GpuLogProbs *lp, GpuArray *logp, GpuArray *entropy, GpuArra
 }
 
 #define LP_CTAS 16 /* of 256 threads, 4 of which an SM holds at once */
-#define LP_U 4 /* vectors of a thread in the gradient kernel: GA_LP_U of the template */
 
 int GpuLogProbs_grad(GpuLogProbs *lp, GpuArray *dlogits, const GpuArray *logits,
                      const GpuArray *targets, const GpuArray *stats, const GpuArray *dlogp,
@@ -303,7 +323,7 @@ int GpuLogProbs_grad(GpuLogProbs *lp, GpuArray *dlogits, const GpuArray *logits,
   grid[0] = (unsigned)((L.rows + block[1] - 1) / block[1]);
   /* A CTA takes as many steps along its row as leave LP_CTAS for every SM. */
   {
-    unsigned long long want = ((unsigned long long)ctx->num_sms * (getenv("LPG") ? (unsigned)atoi(getenv("LPG")) : LP_CTAS) + grid[0] - 1) / grid[0];
+    unsigned long long want = ((unsigned long long)ctx->num_sms * LP_CTAS + grid[0] - 1) / grid[0];
     if (grid[1] > want) grid[1] = (unsigned)want;
   }
   p[0] = at(dlogits);

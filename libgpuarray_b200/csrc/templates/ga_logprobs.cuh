@@ -18,7 +18,7 @@
  * GA_LP_ZTYPE (0 half, 1 float), GA_LP_G_T and GA_LP_GTYPE (dlogits),
  * GA_LP_I_T (token ids), GA_LP_ND (leading dimensions), GA_LP_CONTIG (elements
  * of a row adjacent), GA_LP_ENT (entropy wanted), and for the rows kernel
- * GA_LP_THREADS, GA_LP_GROUP (threads per row: 32 or GA_LP_THREADS),
+ * GA_LP_FOLD (see ga__lp_step), GA_LP_THREADS, GA_LP_GROUP (threads per row: 32 or GA_LP_THREADS),
  * GA_LP_CLUSTER (CTAs per row), GA_LP_TOP (alternatives wanted). */
 #include "ga_lm_common.cuh"
 
@@ -171,8 +171,8 @@ static __device__ __forceinline__ void ga__lp_pair(const ga__lp_words &q, int k,
 }
 
 #ifdef GA_LP_BUILD_ROWS
-#define GA_LP_U 4
-#define GA_LP_CAND 512
+#define GA_LP_U 4 /* vectors of a thread in one step, and as many fetched ahead */
+#define GA_LP_CAND (GA_LP_GROUP == 32 ? 256 : 512)
 /* below every logit that is not -inf: the maximum of nothing (a half is never so low; a float
  * logit of exactly this value gives the right S all the same) */
 #define GA_LP_NOTHING -3.402823466e38f
@@ -200,31 +200,40 @@ static __device__ __forceinline__ ga__lp_state ga__lp_merge(ga__lp_state a, floa
   return a;
 }
 
-static __device__ __forceinline__ float ga__lp_max(const ga__lp_words &q) {
+/* the largest element of N vectors, NaNs left out where there are numbers */
+template <int N>
+static __device__ __forceinline__ float ga__lp_max(const ga__lp_words q[N]) {
 #if GA_LP_ZTYPE == 0
-  unsigned int h = q.w[0];
+  unsigned int h = q[0].w[0];
 #pragma unroll
-  for (int j = 1; j < GA_LP_W; j++) h = ga__max_h2(h, q.w[j]);
+  for (int j = 1; j < N * GA_LP_W; j++) h = ga__max_h2(h, q[j / GA_LP_W].w[j % GA_LP_W]);
   float a, b;
   ga__unpack_h2(h, a, b);
   return fmaxf(a, b);
 #else
-  float a = __uint_as_float(q.w[0]);
+  float a = __uint_as_float(q[0].w[0]);
 #pragma unroll
-  for (int j = 1; j < GA_LP_W; j++) a = fmaxf(a, __uint_as_float(q.w[j]));
+  for (int j = 1; j < N * GA_LP_W; j++) a = fmaxf(a, __uint_as_float(q[j / GA_LP_W].w[j % GA_LP_W]));
   return a;
 #endif
 }
 
-/* N vectors into a thread's state: the sums are kept in pairs beside it. */
+/* N vectors into a thread's state: the sums are kept in pairs beside it. Returns their largest.
+ *
+ * GA_LP_FOLD (halfs, a scale of at most 64): y = z c - mc by one fused operation, mc = m c
+ * rounded (by itself, not inside another fused operation). All terms are then off by the same factor 2^d, d = m c - mc exactly, |d| < 1/2, which
+ * ga__lp_settle takes back once. Otherwise y = (z - m) c. */
 template <int N>
-static __device__ __forceinline__ void ga__lp_step(const ga__lp_words q[N], float c, ga__lp_state &st,
-                                                   ga__f2 &s2, ga__f2 &t2) {
-  float top = ga__lp_max(q[0]);
-#pragma unroll
-  for (int u = 1; u < N; u++) top = fmaxf(top, ga__lp_max(q[u]));
+static __device__ __forceinline__ float ga__lp_step(const ga__lp_words q[N], float c, ga__lp_state &st,
+                                                    ga__f2 &s2, ga__f2 &t2) {
+  const float top = ga__lp_max<N>(q);
   if (top > st.m) {
-    const float d = ga__max_nan((st.m - top) * c, GA_LP_YMIN), f = ga__ex2(d);
+#if GA_LP_FOLD
+    const float d = st.m == GA_LP_NOTHING ? GA_LP_YMIN : ga__max_nan(__fmul_rn(st.m, c) - __fmul_rn(top, c), GA_LP_YMIN);
+#else
+    const float d = ga__max_nan((st.m - top) * c, GA_LP_YMIN);
+#endif
+    const float f = ga__ex2(d);
     const ga__f2 f2 = ga__f2_of(f, f);
 #if GA_LP_ENT
     t2 = ga__f2_mul(ga__f2_fma(s2, ga__f2_of(d, d), t2), f2);
@@ -233,17 +242,22 @@ static __device__ __forceinline__ void ga__lp_step(const ga__lp_words q[N], floa
     st.m = top;
   }
   const ga__f2 c2 = ga__f2_of(c, c);
+#if GA_LP_FOLD
+  const float mc = st.m == GA_LP_NOTHING ? 0.0f : -__fmul_rn(st.m, c);
+  const ga__f2 mc2 = ga__f2_of(mc, mc);
+#else
+  const ga__f2 m2 = ga__f2_of(-st.m, -st.m);
+#endif
 #pragma unroll
   for (int u = 0; u < N; u++)
 #pragma unroll
     for (int k = 0; k < GA_LP_PAIRS; k++) {
       float a, b;
-#if GA_LP_ZTYPE == 0
-      ga__add_h2_f32(q[u].w[k], -st.m, a, b);
-      ga__f2_to(ga__f2_mul(ga__f2_of(a, b), c2), a, b);
-#else
       ga__lp_pair(q[u], k, a, b);
-      ga__f2_to(ga__f2_mul(ga__f2_add(ga__f2_of(a, b), ga__f2_of(-st.m, -st.m)), c2), a, b);
+#if GA_LP_FOLD
+      ga__f2_to(ga__f2_fma(ga__f2_of(a, b), c2, mc2), a, b);
+#else
+      ga__f2_to(ga__f2_mul(ga__f2_add(ga__f2_of(a, b), m2), c2), a, b);
 #endif
 #if GA_LP_ENT
       a = ga__max_nan(a, GA_LP_YMIN); /* e y is 0 for a logit of -inf */
@@ -255,6 +269,23 @@ static __device__ __forceinline__ void ga__lp_step(const ga__lp_words q[N], floa
       t2 = ga__f2_fma(e2, ga__f2_of(a, b), t2);
 #endif
     }
+  return top;
+}
+
+/* The thread's sums, relative to its m. */
+static __device__ __forceinline__ void ga__lp_settle(float c, ga__lp_state &st, ga__f2 s2, ga__f2 t2) {
+  float a, b;
+  ga__f2_to(s2, a, b);
+  st.s = a + b;
+  ga__f2_to(t2, a, b);
+  st.t = a + b;
+#if GA_LP_FOLD
+  if (st.m != GA_LP_NOTHING) {
+    const float mc = __fmul_rn(st.m, c), d = fmaf(st.m, c, -mc), f = ga__ex2(-d);
+    st.t = (st.t - st.s * d) * f;
+    st.s *= f;
+  }
+#endif
 }
 
 #if GA_LP_TOP
@@ -291,21 +322,43 @@ static __device__ __forceinline__ void ga__lp_keys(const ga__lp_layout &L, const
 static __device__ __forceinline__ unsigned long long ga__lp_best(const ga__lp_layout &L, const ga__lp_row &r,
                                                                  unsigned int w, float m) {
   unsigned long long k[2 * GA_LP_PAIRS], best = 0;
-  if (!(ga__lp_max(ga__lp_load(L, r, w)) >= m)) return 0;
+  const ga__lp_words q = ga__lp_load(L, r, w);
+  if (!(ga__lp_max<1>(&q) >= m)) return 0;
   ga__lp_keys(L, r, w, k);
 #pragma unroll
   for (int j = 0; j < 2 * GA_LP_PAIRS; j++) best = k[j] > best ? k[j] : best;
   return best;
 }
 
+/* the threads of a row meet */
+static __device__ __forceinline__ void ga__lp_sync() {
+  if (GA_LP_GROUP == 32) __syncwarp();
+  else __syncthreads();
+}
+
+/* A thread's vectors in pieces of so many steps of GA_LP_U, that GA_LP_PIECES hold them all; what
+ * is left over after its whole steps and the extra vector belong to the piece of the next step. */
+#define GA_LP_PIECES (GA_LP_GROUP == 32 ? 16 : 2048 / GA_LP_GROUP)
+static __device__ __forceinline__ unsigned int ga__lp_piece_steps(const ga__lp_share &s) {
+  const unsigned int steps = (s.f1 - s.f0) / (GA_LP_U * GA_LP_GROUP) + 2; /* of any thread, at most */
+  return (steps + GA_LP_PIECES - 1) / GA_LP_PIECES;
+}
+/* the last piece of thread t */
+static __device__ __forceinline__ unsigned int ga__lp_last_piece(const ga__lp_share &s, unsigned int t) {
+  const unsigned int mine = s.f0 + t < s.f1 ? (s.f1 - s.f0 - t + GA_LP_GROUP - 1) / GA_LP_GROUP : 0;
+  return mine / GA_LP_U / ga__lp_piece_steps(s);
+}
+
 struct ga__lp_top_smem {
   unsigned long long cand[GA_LP_CAND];
-  unsigned long long best[GA_LP_THREADS];
+  unsigned long long best[GA_LP_GROUP];
   unsigned long long out[GA_LP_CLUSTER * 32]; /* the CTAs' lists, in the first CTA of a cluster */
-  unsigned int high[GA_LP_THREADS];
-  unsigned int list[GA_LP_THREADS];
   unsigned long long tau;
-  unsigned int nlist, ncand, count;
+  unsigned int high[GA_LP_GROUP];
+  unsigned int piece[GA_LP_PIECES][GA_LP_GROUP]; /* largest values of the threads' pieces */
+  unsigned int list[GA_LP_CAND];                   /* piece * GA_LP_GROUP + thread */
+  unsigned int vec[GA_LP_CAND];
+  unsigned int nlist, nvec, ncand, count;
 };
 
 /* The top-th largest of the lanes' keys, at least 1 (0: no key); the same in every lane. */
@@ -323,40 +376,69 @@ static __device__ __forceinline__ K ga__lp_nth(K mine, unsigned int top) {
   return t > 0 ? t : 1;
 }
 
-/* Appends the keys from `tau` on of the listed threads' vectors (or of all) to the candidates. */
+static __device__ __forceinline__ void ga__lp_list(unsigned int piece, ga__lp_top_smem &S) {
+  const unsigned int at = atomicAdd(&S.nlist, 1u);
+  if (at < GA_LP_CAND) S.list[at] = piece * GA_LP_GROUP + threadIdx.x % GA_LP_GROUP;
+}
+static __device__ __forceinline__ void ga__lp_append(unsigned long long key, ga__lp_top_smem &S) {
+  const unsigned int at = atomicAdd(&S.ncand, 1u);
+  if (at < GA_LP_CAND) S.cand[at] = key;
+}
+
+/* Appends the keys from `tau` on of the listed pieces' vectors to the candidates: first the vectors
+ * that hold one, by their largest element, then an element for each thread. */
 static __device__ __forceinline__ void ga__lp_collect(const ga__lp_layout &L, const ga__lp_row &r,
-                                                      const ga__lp_share &sh, int all,
-                                                      unsigned long long tau, ga__lp_top_smem &S) {
-  const unsigned int whole = (sh.f1 - sh.f0 + GA_LP_THREADS - 1) / GA_LP_THREADS;
-  const unsigned int items = all ? sh.v1 - sh.v0 : S.nlist * (whole + 1);
-  for (unsigned int it = threadIdx.x; it < items; it += GA_LP_THREADS) {
-    if (*(volatile unsigned int *)&S.ncand > GA_LP_CAND) break; /* too many: they are not used */
-    unsigned int w = sh.v0 + it;
-    if (!all) {
-      const unsigned int t = S.list[it / (whole + 1)], j = it % (whole + 1);
-      w = j < whole ? sh.f0 + t + j * GA_LP_THREADS : ga__lp_extra(sh, t);
-      if (j < whole ? w >= sh.f1 : w == GA_LP_NONE) continue;
+                                                      const ga__lp_share &sh, unsigned long long tau,
+                                                      ga__lp_top_smem &S) {
+  const unsigned int steps = ga__lp_piece_steps(sh);
+  const unsigned int per = steps * GA_LP_U + 1; /* and the extra vector */
+  const unsigned int items = (S.nlist < GA_LP_CAND ? S.nlist : GA_LP_CAND) * per;
+  const float inv = 1.0f / (float)per; /* exact quotients below 2^20 */
+  const unsigned int tid = threadIdx.x % GA_LP_GROUP;
+  if (tid == 0 && S.nlist > GA_LP_CAND) S.nvec = GA_LP_CAND + 1;
+  for (unsigned int it = tid; it < items && S.nlist <= GA_LP_CAND; it += GA_LP_GROUP) {
+    if (*(volatile unsigned int *)&S.nvec > GA_LP_CAND) break; /* too many: they are not used */
+    const unsigned int l = items < (1u << 20) ? (unsigned int)(((float)it + 0.5f) * inv) : it / per;
+    const unsigned int t = S.list[l] % GA_LP_GROUP, p = S.list[l] / GA_LP_GROUP, j = it - l * per;
+    unsigned int w;
+    if (j + 1 < per) {
+      w = sh.f0 + t + (p * steps * GA_LP_U + j) * GA_LP_GROUP;
+      if (w >= sh.f1) continue;
+    } else { /* the extra vector is in the last piece of its thread that there is */
+      w = ga__lp_extra(sh, t);
+      if (w == GA_LP_NONE || p != ga__lp_last_piece(sh, t)) continue;
     }
-    unsigned long long k[2 * GA_LP_PAIRS];
-    ga__lp_keys(L, r, w, k);
-#pragma unroll
-    for (int j = 0; j < 2 * GA_LP_PAIRS; j++)
-      if (k[j] >= tau) {
-        const unsigned int at = atomicAdd(&S.ncand, 1u);
-        if (at < GA_LP_CAND) S.cand[at] = k[j];
-      }
+    const ga__lp_words q = ga__lp_load(L, r, w);
+    /* no element's key is above that of the largest value at the vector's first place */
+    const unsigned int i0 = w * GA_LP_E < r.skip ? 0 : w * GA_LP_E - r.skip;
+    if (ga__lp_key(ga__lp_max<1>(&q), i0) >= tau) {
+      const unsigned int at = atomicAdd(&S.nvec, 1u);
+      if (at < GA_LP_CAND) S.vec[at] = w;
+    }
   }
-  __syncthreads();
+  ga__lp_sync();
+  if (S.nvec > GA_LP_CAND) { /* the same in every thread */
+    if (tid == 0) S.ncand = GA_LP_CAND + 1;
+  } else {
+    const unsigned int elements = S.nvec * GA_LP_E;
+    for (unsigned int it = tid; it < elements; it += GA_LP_GROUP) {
+      const unsigned int i = S.vec[it / GA_LP_E] * GA_LP_E + it % GA_LP_E - r.skip;
+      if (i >= L.v) continue;
+      const unsigned long long k = ga__lp_key(ga__lp_z(r.z + (long long)i * L.z_col), i);
+      if (k >= tau) ga__lp_append(k, S);
+    }
+  }
+  ga__lp_sync();
 }
 
 /* The `top` largest keys of a CTA's vectors of the row, into out[0..32) of this CTA's or the
- * cluster's first CTA's shared memory (0 where there are fewer). All threads of the CTA, after a
+ * cluster's first CTA's shared memory (0 where there are fewer). All threads of the group, after a
  * barrier behind which S.high has every thread's largest value and the counters are 0; m: this
  * thread's.
  *
  * The largest values of 32 disjoint groups of threads are values of 32 elements, so the top-th
  * largest of them, tau, is a lower bound for the top-th largest of all, and every element that
- * reaches it belongs to a thread whose largest does: only those threads' vectors are read again.
+ * reaches it belongs to a piece of a thread whose largest does: only those pieces are read again.
  * (For 20 alternatives of 256 threads they are about 30.) Where more elements reach tau than can
  * be held (equal values: rows with fewer numbers than alternatives, constants), the same is done
  * with keys that break ties by the index; where that is still too much (a row that hides its
@@ -364,48 +446,52 @@ static __device__ __forceinline__ void ga__lp_collect(const ga__lp_layout &L, co
  * over the row. */
 static __device__ void ga__lp_top(const ga__lp_layout &L, const ga__lp_row &r, const ga__lp_share &sh,
                                   float m, int odd, ga__lp_top_smem &S) {
-  const unsigned int tid = threadIdx.x, lane = tid % 32;
+  const unsigned int tid = threadIdx.x % GA_LP_GROUP, lane = tid % 32;
+  const unsigned int last = ga__lp_last_piece(sh, tid);
   unsigned long long k[2 * GA_LP_PAIRS], tau = 0;
   if (!odd) {
     if (tid < 32) {
       unsigned int high = 0;
 #pragma unroll
-      for (int j = 0; j < GA_LP_THREADS / 32; j++) {
+      for (int j = 0; j < GA_LP_GROUP / 32; j++) {
         const unsigned int b = S.high[j * 32 + lane];
         high = b > high ? b : high;
       }
       high = ga__lp_nth(high, L.top);
       if (lane == 0) S.tau = (unsigned long long)high << 32;
     }
-    __syncthreads();
+    ga__lp_sync();
     tau = S.tau;
     const float minus_inf = __uint_as_float(0xff800000u);
     const int few = (tau >> 32) == (ga__lp_key(minus_inf, 0) >> 32); /* fewer above -inf than asked for */
     if (!few) {
-      if (S.high[tid] > 0 && ga__lp_key(m, 0) >= tau) S.list[atomicAdd(&S.nlist, 1u)] = tid;
-      __syncthreads();
-      ga__lp_collect(L, r, sh, 0, tau, S);
+      if (S.high[tid] > 0 && ga__lp_key(m, 0) >= tau)
+        for (unsigned int p = 0; p <= last; p++)
+          if ((unsigned long long)S.piece[p][tid] << 32 >= tau) ga__lp_list(p, S);
+      ga__lp_sync();
+      ga__lp_collect(L, r, sh, tau, S);
     }
     if (few || S.ncand > GA_LP_CAND) { /* the same in every thread */
       unsigned long long mine = 0;
       /* its first place: p0 is before the whole vectors, p1 behind them */
       if (tid == 0 && sh.p0 != GA_LP_NONE) mine = ga__lp_best(L, r, sh.p0, m);
-      for (unsigned int w = sh.f0 + tid; mine == 0 && w < sh.f1; w += GA_LP_THREADS) mine = ga__lp_best(L, r, w, m);
+      for (unsigned int w = sh.f0 + tid; mine == 0 && w < sh.f1; w += GA_LP_GROUP) mine = ga__lp_best(L, r, w, m);
       if (mine == 0 && tid == 1 && sh.p1 != GA_LP_NONE) mine = ga__lp_best(L, r, sh.p1, m);
       S.best[tid] = mine;
-      __syncthreads();
-      if (tid == 0) S.nlist = S.ncand = 0;
+      ga__lp_sync();
+      if (tid == 0) S.nlist = S.nvec = S.ncand = 0;
       unsigned long long most = 0;
 #pragma unroll
-      for (int j = 0; j < GA_LP_THREADS / 32; j++) {
+      for (int j = 0; j < GA_LP_GROUP / 32; j++) {
         const unsigned long long b = S.best[j * 32 + lane];
         most = b > most ? b : most;
       }
       tau = ga__lp_nth(most, L.top);
-      __syncthreads();
-      if (mine >= tau) S.list[atomicAdd(&S.nlist, 1u)] = tid;
-      __syncthreads();
-      ga__lp_collect(L, r, sh, 0, tau, S);
+      ga__lp_sync();
+      if (mine >= tau)
+        for (unsigned int p = 0; p <= last; p++) ga__lp_list(p, S);
+      ga__lp_sync();
+      ga__lp_collect(L, r, sh, tau, S);
     }
   }
   if (odd || S.ncand > GA_LP_CAND) { /* the same in every thread */
@@ -415,17 +501,17 @@ static __device__ void ga__lp_top(const ga__lp_layout &L, const ga__lp_row &r, c
     for (int step = 0; step < 66; step++) {
       const unsigned long long mid = step == 0 ? 1 : lo + (hi - lo) / 2;
       unsigned int c = 0;
-      __syncthreads();
+      ga__lp_sync();
       if (tid == 0) S.count = 0;
-      __syncthreads();
-      for (unsigned int w = sh.v0 + tid; w < sh.v1; w += GA_LP_THREADS) {
+      ga__lp_sync();
+      for (unsigned int w = sh.v0 + tid; w < sh.v1; w += GA_LP_GROUP) {
         ga__lp_keys(L, r, w, k);
 #pragma unroll
         for (int j = 0; j < 2 * GA_LP_PAIRS; j++) c += k[j] >= mid;
       }
       c = ga__warp_sum_u32(c);
       if (lane == 0) atomicAdd(&S.count, c);
-      __syncthreads();
+      ga__lp_sync();
       c = S.count;
       if (c >= L.top || step == 0) lo = mid;
       else hi = mid;
@@ -433,18 +519,24 @@ static __device__ void ga__lp_top(const ga__lp_layout &L, const ga__lp_row &r, c
     }
     tau = lo;
     if (tid == 0) S.ncand = 0;
-    __syncthreads();
-    ga__lp_collect(L, r, sh, 1, tau, S);
+    ga__lp_sync();
+    for (unsigned int w = sh.v0 + tid; w < sh.v1; w += GA_LP_GROUP) {
+      ga__lp_keys(L, r, w, k);
+#pragma unroll
+      for (int j = 0; j < 2 * GA_LP_PAIRS; j++)
+        if (k[j] >= tau) ga__lp_append(k[j], S);
+    }
+    ga__lp_sync();
   }
   /* a key's place is the number of larger ones */
   const unsigned int n = S.ncand < GA_LP_CAND ? S.ncand : GA_LP_CAND;
 #if GA_LP_CLUSTER > 1
   const unsigned int slot = ga__cluster_rank() * 32;
-  for (unsigned int i = tid + n; i < L.top; i += GA_LP_THREADS) ga__cluster_put(&S.out[slot + i], 0, 0ULL);
+  for (unsigned int i = tid + n; i < L.top; i += GA_LP_GROUP) ga__cluster_put(&S.out[slot + i], 0, 0ULL);
 #else
-  for (unsigned int i = tid + n; i < L.top; i += GA_LP_THREADS) S.out[i] = 0;
+  for (unsigned int i = tid + n; i < L.top; i += GA_LP_GROUP) S.out[i] = 0;
 #endif
-  for (unsigned int i = tid; i < n; i += GA_LP_THREADS) {
+  for (unsigned int i = tid; i < n; i += GA_LP_GROUP) {
     const unsigned long long key = S.cand[i];
     unsigned int place = 0;
 #pragma unroll 4
@@ -462,13 +554,13 @@ static __device__ void ga__lp_top(const ga__lp_layout &L, const ga__lp_row &r, c
 
 struct ga__lp_shared {
 #if GA_LP_TOP
-  ga__lp_top_smem tops;
+  ga__lp_top_smem tops[GA_LP_THREADS / GA_LP_GROUP];
 #endif
   unsigned long long parts[GA_LP_CLUSTER][2]; /* the CTAs' states, in the first CTA of a cluster */
   ga__lp_state warps[GA_LP_THREADS / 32];
 };
 
-extern "C" __global__ void __launch_bounds__(GA_LP_THREADS)
+extern "C" __global__ void __launch_bounds__(GA_LP_THREADS, 1024 / GA_LP_THREADS)
 #if GA_LP_CLUSTER > 1
     __cluster_dims__(GA_LP_CLUSTER, 1, 1)
 #endif
@@ -507,11 +599,39 @@ ga_lp_rows(const __grid_constant__ ga__lp_layout L, const char *logits, const ch
   ga__f2 s2 = ga__f2_of(0.0f, 0.0f), t2 = s2;
   const unsigned int extra = ga__lp_extra(my, lane);
   unsigned int w = my.f0 + lane;
-  for (; w + (GA_LP_U - 1) * GA_LP_GROUP < my.f1; w += GA_LP_U * GA_LP_GROUP) {
+  GA_LM_SHARED(ga__lp_shared, sh);
+#if GA_LP_TOP
+  ga__lp_top_smem &tops = sh.tops[threadIdx.x / GA_LP_GROUP];
+  const unsigned int steps = ga__lp_piece_steps(my);
+  unsigned int left = steps, piece = 0;
+  float largest = __uint_as_float(0xff800000u); /* of the piece */
+#endif
+  /* the next vectors are fetched before the present ones are worked on */
+  ga__lp_words next[GA_LP_U];
+  int more = w + (GA_LP_U - 1) * GA_LP_GROUP < my.f1;
+  if (more) {
+#pragma unroll
+    for (int u = 0; u < GA_LP_U; u++) next[u] = ga__lp_load_whole(L, r, w + u * GA_LP_GROUP);
+  }
+  while (more) {
     ga__lp_words q[GA_LP_U];
 #pragma unroll
-    for (int u = 0; u < GA_LP_U; u++) q[u] = ga__lp_load_whole(L, r, w + u * GA_LP_GROUP);
-    ga__lp_step<GA_LP_U>(q, c, st, s2, t2);
+    for (int u = 0; u < GA_LP_U; u++) q[u] = next[u];
+    w += GA_LP_U * GA_LP_GROUP;
+    more = w + (GA_LP_U - 1) * GA_LP_GROUP < my.f1;
+    if (more) {
+#pragma unroll
+      for (int u = 0; u < GA_LP_U; u++) next[u] = ga__lp_load_whole(L, r, w + u * GA_LP_GROUP);
+    }
+    const float top = ga__lp_step<GA_LP_U>(q, c, st, s2, t2);
+#if GA_LP_TOP
+    largest = fmaxf(largest, top);
+    if (--left == 0) {
+      tops.piece[piece++][lane] = (unsigned int)(ga__lp_key(largest, 0) >> 32);
+      largest = __uint_as_float(0xff800000u);
+      left = steps;
+    }
+#endif
   }
   { /* fewer than GA_LP_U are left: all of them in flight, then one at a time */
     ga__lp_words q[GA_LP_U];
@@ -521,31 +641,33 @@ ga_lp_rows(const __grid_constant__ ga__lp_layout L, const char *logits, const ch
     if (extra != GA_LP_NONE) q[GA_LP_U - 1] = ga__lp_load_part(L, r, extra);
 #pragma unroll 1
     for (int u = 0; u < GA_LP_U; u++) {
-      if (u + 1 < GA_LP_U ? w + u * GA_LP_GROUP < my.f1 : extra != GA_LP_NONE) ga__lp_step<1>(&q[0], c, st, s2, t2);
+      if (u + 1 < GA_LP_U ? w + u * GA_LP_GROUP < my.f1 : extra != GA_LP_NONE) {
+        const float top = ga__lp_step<1>(&q[0], c, st, s2, t2);
+#if GA_LP_TOP
+        largest = fmaxf(largest, top);
+#endif
+      }
 #pragma unroll
       for (int i = 0; i + 1 < GA_LP_U; i++) q[i] = q[i + 1];
     }
   }
-  {
-    float a, b;
-    ga__f2_to(s2, a, b);
-    st.s = a + b;
-    ga__f2_to(t2, a, b);
-    st.t = a + b;
-  }
-  GA_LM_SHARED(ga__lp_shared, sh);
 #if GA_LP_TOP
-  ga__lp_top_smem &tops = sh.tops;
+  tops.piece[piece][lane] = (unsigned int)(ga__lp_key(largest, 0) >> 32);
+#endif
+  ga__lp_settle(c, st, s2, t2);
+#if GA_LP_TOP
   const float most = st.s == 0.0f ? __uint_as_float(0xff800000u) : st.m; /* this thread's largest */
-  tops.high[threadIdx.x] =
+  tops.high[lane] =
       my.f0 + lane < my.f1 || extra != GA_LP_NONE ? (unsigned int)(ga__lp_key(most, 0) >> 32) : 0;
-  if (threadIdx.x == 0) tops.nlist = tops.ncand = 0;
+  if (lane == 0) tops.nlist = tops.nvec = tops.ncand = 0;
 #endif
   st = ga__lp_merge(st, c, 32);
 #if GA_LP_GROUP > 32
   if (threadIdx.x % 32 == 0) sh.warps[threadIdx.x / 32] = st;
   __syncthreads();
   st = ga__lp_merge(sh.warps[threadIdx.x % (GA_LP_THREADS / 32)], c, GA_LP_THREADS / 32);
+#elif GA_LP_TOP
+  __syncwarp();
 #endif
 #if GA_LP_CLUSTER > 1
   ga__cluster_wait(); /* every CTA of the cluster runs */
@@ -600,10 +722,10 @@ ga_lp_rows(const __grid_constant__ ga__lp_layout L, const char *logits, const ch
 #if GA_LP_CLUSTER > 1
   const unsigned int n = GA_LP_CLUSTER * 32;
 #else
-  __syncthreads();
+  ga__lp_sync();
   const unsigned int n = L.top;
 #endif
-  for (unsigned int i = threadIdx.x; i < n; i += GA_LP_THREADS) {
+  for (unsigned int i = lane; i < n; i += GA_LP_GROUP) {
 #if GA_LP_CLUSTER > 1
     if (i % 32 >= L.top) continue;
 #endif

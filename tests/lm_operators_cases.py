@@ -273,6 +273,7 @@ def lp_formula(z, targets, scale, ignore=None):
         p = e / s
         ent = -np.where(p > 0, p * np.where(p > 0, logs, 0), np.where(np.isnan(p), p, 0)).sum(-1)
     bad = np.isnan(s[..., 0])
+    logs[logs < np.finfo(np.float32).min] = -INF        # results are floats: a scaled lowest value can lie below them
     logs[bad] = np.nan
     logs[empty] = -INF
     p[empty] = 0
@@ -340,17 +341,17 @@ def check_top(api, z, k, values, ids, logs, tol, empty):
         close(values[r], logs[r][order], tol[r], "row %d" % r)
 
 
-SHAPES = [(1, 1), (3, 2), (4, 7), (5, 33), (3, 256), (3, 1000), (2, 2049), (2, 4500), (1, 9001)]
+SHAPES = [(1, 1), (3, 2), (4, 7), (5, 33), (3, 256), (3, 1000), (40, 150), (34, 1111), (2, 2049), (2, 4500), (1, 9001)]
 
 
 @pytest.mark.parametrize("dtype", ["f2", "f4"])
 @pytest.mark.parametrize("kind", ["plain", "masked", "lowest", "ties", "large"])
 @pytest.mark.parametrize("rows,V", SHAPES)
 def test_logprobs(api, ctx, rng, dtype, kind, rows, V):
-    top = min(V, [0, 1, 5, 20, 32][(rows + V) % 5])
+    top = min(V, [0, 1, 5, 20, 32, 32][(rows + V) % 6])
     z = rows_of_logits(rng, rows, V, dtype, kind)
     targets = rng.integers(0, V, rows).astype(np.int64)
-    scale = [1.0, 0.7, 1.3][V % 3]
+    scale = [1.0, 0.7, 1.3, 100.0][V % 4]
     op = api.GpuLogProbs(ctx, dtype, np.int64, top=top)
     lead = (rows,)
     d = {n: api.GpuArray.empty(ctx, s, t) for n, s, t in (

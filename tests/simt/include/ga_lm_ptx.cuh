@@ -44,6 +44,7 @@ static inline unsigned int __match_any_sync(unsigned, unsigned int v) {
   simt::warp_barrier(w, n);
   return r;
 }
+static inline float __fmul_rn(float a, float b) { return a * b; }
 static inline int __popc(unsigned int v) { return __builtin_popcount(v); }
 static inline int __ffs(unsigned int v) { return __builtin_ffs((int)v); }
 static inline unsigned int ga__warp_sum_u32(unsigned int v) {
