@@ -167,18 +167,19 @@ def lib():
         ctypes.c_char_p, ci, cu, ctypes.POINTER(_ElemwiseArg), ci)
     sig("GpuMapReduction_free", None, vp)
     sig("GpuMapReduction_call", ci, vp, A, ctypes.POINTER(vp), cu, ctypes.POINTER(ci), ci)
-    cd, pA = ctypes.c_double, ctypes.POINTER(A)
-    sig("GpuArray_embed", ci, A, A, A, cd, ctypes.c_ssize_t, ci)
+    # arrays go in as addresses (GpuArray.at): a conversion for each costs as much as the checks
+    cd = ctypes.c_double
+    sig("GpuArray_embed", ci, vp, vp, vp, cd, ctypes.c_ssize_t, ci)
     sig("GpuEmbedGrad_new", ci, ctypes.POINTER(vp), vp)
     sig("GpuEmbedGrad_free", None, vp)
-    sig("GpuEmbedGrad_call", ci, vp, A, A, A, cd, ctypes.c_ssize_t, ci)
+    sig("GpuEmbedGrad_call", ci, vp, vp, vp, vp, cd, ctypes.c_ssize_t, ci)
     sig("GpuLogProbs_new", ci, ctypes.POINTER(vp), vp, ci, ci, cu)
     sig("GpuLogProbs_free", None, vp)
-    sig("GpuLogProbs_call", ci, vp, A, A, A, A, A, A, A, cd, ctypes.c_ssize_t, ci)
-    sig("GpuLogProbs_grad", ci, vp, A, A, A, A, A, A, A, cd, ctypes.c_ssize_t, ci)
+    sig("GpuLogProbs_call", ci, vp, vp, vp, vp, vp, vp, vp, vp, cd, ctypes.c_ssize_t, ci)
+    sig("GpuLogProbs_grad", ci, vp, vp, vp, vp, vp, vp, vp, vp, cd, ctypes.c_ssize_t, ci)
     sig("GpuClipNorm_new", ci, ctypes.POINTER(vp), vp)
     sig("GpuClipNorm_free", None, vp)
-    sig("GpuClipNorm_call", ci, vp, A, pA, pA, cu, cd, cd)
+    sig("GpuClipNorm_call", ci, vp, vp, vp, vp, cu, cd, cd)
     for name in ("gpucomm_new", "gpucomm_free", "gpucomm_gen_clique_id", "gpucomm_all_reduce",
                  "gpucomm_get_count", "gpucomm_get_rank"):
         if not hasattr(L, name):
@@ -289,6 +290,7 @@ class GpuArray:
     def __init__(self, ctx):
         self.ctx = ctx
         self.ga = _GpuArrayStruct()
+        self.at = ctypes.addressof(self.ga)     # GpuArray * of the C interface
         self._live = False
 
     # ---- construction ----
@@ -660,17 +662,13 @@ def maxandargmax(dst_max, dst_argmax, src, axes):
                                                     ctypes.byref(src.ga), len(axes), ax))
 
 
-def _ref(a):
-    """The C struct of an array, or NULL for None."""
-    return None if a is None else ctypes.byref(a.ga)
-
-
 def embed(out, table, ids, scale=1.0, pad=None, check=False):
     """GpuArray_embed (include/gpuarray/embedding.h): out[t, :] = scale * table[ids[t], :],
     rows of zeros where ids[t] == pad. check=True waits and raises for an id
     outside the table."""
-    flags = (0 if pad is None else GA_EMBED_PAD) | (GA_EMBED_CHECK if check else 0)
-    err = lib().GpuArray_embed(_ref(out), _ref(table), _ref(ids), scale, pad or 0, flags)
+    err = lib().GpuArray_embed(out.at, table.at if table is not None else None,
+                               ids.at if ids is not None else None, scale, pad or 0,
+                               (pad is not None) * GA_EMBED_PAD | check * GA_EMBED_CHECK)
     if err:
         _check(out.ctx.ptr, err)
 
@@ -712,10 +710,10 @@ class GpuEmbedGrad(_Operator):
         self._made(ctx, "GpuEmbedGrad_new")
 
     def __call__(self, dtable, dout, ids, scale=1.0, pad=None, accumulate=False, check=False):
-        flags = ((0 if pad is None else GA_EMBED_PAD) | (GA_EMBED_CHECK if check else 0) |
-                 (GA_EMBED_ACCUMULATE if accumulate else 0))
-        err = lib().GpuEmbedGrad_call(self.ptr, _ref(dtable), _ref(dout), _ref(ids), scale,
-                                      pad or 0, flags)
+        err = lib().GpuEmbedGrad_call(
+            self.ptr, dtable.at if dtable is not None else None, dout.at if dout is not None else None,
+            ids.at if ids is not None else None, scale, pad or 0,
+            (pad is not None) * GA_EMBED_PAD | check * GA_EMBED_CHECK | accumulate * GA_EMBED_ACCUMULATE)
         if err:
             _check(self.ctx.ptr, err)
 
@@ -738,10 +736,12 @@ class GpuLogProbs(_Operator):
 
     def __call__(self, logits, targets=None, logp=None, entropy=None, stats=None, top_logp=None,
                  top_ids=None, scale=1.0, ignore=None, check=False):
-        flags = (0 if ignore is None else GA_LOGPROBS_IGNORE) | (GA_LOGPROBS_CHECK if check else 0)
-        err = lib().GpuLogProbs_call(self.ptr, _ref(logp), _ref(entropy), _ref(stats), _ref(top_logp),
-                                     _ref(top_ids), _ref(logits), _ref(targets), scale, ignore or 0,
-                                     flags)
+        err = lib().GpuLogProbs_call(
+            self.ptr, logp.at if logp is not None else None, entropy.at if entropy is not None else None,
+            stats.at if stats is not None else None, top_logp.at if top_logp is not None else None,
+            top_ids.at if top_ids is not None else None, logits.at if logits is not None else None,
+            targets.at if targets is not None else None, scale, ignore or 0,
+            (ignore is not None) * GA_LOGPROBS_IGNORE | check * GA_LOGPROBS_CHECK)
         if err:
             _check(self.ctx.ptr, err)
 
@@ -749,10 +749,12 @@ class GpuLogProbs(_Operator):
              ignore=None, check=False):
         """dlogits from the gradients arriving at logp and (with the entropy that the
         forward pass wrote) at the entropy; dlogits may be the logits."""
-        flags = (0 if ignore is None else GA_LOGPROBS_IGNORE) | (GA_LOGPROBS_CHECK if check else 0)
-        err = lib().GpuLogProbs_grad(self.ptr, _ref(dlogits), _ref(logits), _ref(targets),
-                                     _ref(stats), _ref(dlogp), _ref(entropy), _ref(dentropy), scale,
-                                     ignore or 0, flags)
+        err = lib().GpuLogProbs_grad(
+            self.ptr, dlogits.at if dlogits is not None else None,
+            logits.at if logits is not None else None, targets.at if targets is not None else None,
+            stats.at if stats is not None else None, dlogp.at if dlogp is not None else None,
+            entropy.at if entropy is not None else None, dentropy.at if dentropy is not None else None,
+            scale, ignore or 0, (ignore is not None) * GA_LOGPROBS_IGNORE | check * GA_LOGPROBS_CHECK)
         if err:
             _check(self.ctx.ptr, err)
 
@@ -763,8 +765,8 @@ class GpuArrayList:
 
     def __init__(self, arrays):
         self.arrays = list(arrays)
-        self.ptrs = (ctypes.POINTER(_GpuArrayStruct) * max(len(self.arrays), 1))(
-            *[ctypes.pointer(a.ga) for a in self.arrays])
+        self.ptrs = (ctypes.c_void_p * max(len(self.arrays), 1))(*[a.at for a in self.arrays])
+        self.at = ctypes.addressof(self.ptrs)
 
     def __len__(self):
         return len(self.arrays)
@@ -788,10 +790,11 @@ class GpuClipNorm(_Operator):
             dsts = srcs if same else dsts
         if dsts is not None and not isinstance(dsts, GpuArrayList):
             dsts = GpuArrayList(dsts)
-        if dsts is not None and len(dsts) != len(srcs):
-            raise ValueError("%d destinations for %d arrays" % (len(dsts), len(srcs)))
-        err = lib().GpuClipNorm_call(self.ptr, _ref(norm), None if dsts is None else dsts.ptrs,
-                                     srcs.ptrs, len(srcs), scale, limit)
+        n = len(srcs.arrays)
+        if dsts is not None and len(dsts.arrays) != n:
+            raise ValueError("%d destinations for %d arrays" % (len(dsts.arrays), n))
+        err = lib().GpuClipNorm_call(self.ptr, norm.at if norm is not None else None,
+                                     None if dsts is None else dsts.at, srcs.at, n, scale, limit)
         if err:
             _check(self.ctx.ptr, err)
 

@@ -142,18 +142,24 @@ static int check_overlap(GpuClipNorm *cn, GpuArray *const *dst, const GpuArray *
   return GA_NO_ERROR;
 }
 
+/* ga_lm_check, the array's place in the list named only where there is something to say */
+static int check_listed(gpucontext *ctx, const GpuArray *a, const char *list, unsigned int i, int dest) {
+  char why[GA_ERR_MSGLEN];
+  const int err = ga_lm_check(ctx, a, "the array", dest);
+  if (err == GA_NO_ERROR) return err;
+  memcpy(why, ctx->err->msg, sizeof(why));
+  return ga_err_fmt(ctx->err, err, "%s[%u]: %.900s", list, i, why);
+}
+
 static int check_one(gpucontext *ctx, const GpuArray *s, const GpuArray *d, unsigned int i) {
-  char name[32];
   int err, f = GA_C_CONTIGUOUS | GA_F_CONTIGUOUS;
-  snprintf(name, sizeof(name), "src[%u]", i);
-  if ((err = ga_lm_check(ctx, s, name, 0)) != GA_NO_ERROR) return err;
+  if ((err = check_listed(ctx, s, "src", i, 0)) != GA_NO_ERROR) return err;
   if (type_index(s->typecode) < 0)
     return ga_err_fmt(ctx->err, GA_UNSUPPORTED_ERROR, "src[%u] must be half, float or double", i);
   if (!(s->flags & f))
     return ga_err_fmt(ctx->err, GA_INVALID_ERROR, "src[%u] is not one segment of memory", i);
-  if (d == NULL) return GA_NO_ERROR;
-  snprintf(name, sizeof(name), "dst[%u]", i);
-  if ((err = ga_lm_check(ctx, d, name, 1)) != GA_NO_ERROR) return err;
+  if (d == NULL || d == s) return d == NULL ? GA_NO_ERROR : check_listed(ctx, d, "dst", i, 1);
+  if ((err = check_listed(ctx, d, "dst", i, 1)) != GA_NO_ERROR) return err;
   if (d->typecode != s->typecode && !(s->typecode == GA_HALF && d->typecode == GA_FLOAT))
     return ga_err_fmt(ctx->err, GA_VALUE_ERROR, "dst[%u] must have the type of src[%u], or be float for half",
                       i, i);

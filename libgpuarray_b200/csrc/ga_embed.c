@@ -333,7 +333,7 @@ int GpuEmbedGrad_call(GpuEmbedGrad *eg, GpuArray *dtable, const GpuArray *dout, 
   grid[1] = ny;
   /* Chunks: threads for half the device, which with EG_STEP loads of a thread in flight keep the
    * memory busy; more and shorter ones only leave more parts to join. None shorter than one step. */
-  groups = (unsigned long long)ctx->num_sms * (getenv("EGT") ? (unsigned)atoi(getenv("EGT")) : EG_GROUP_THREADS) / ((unsigned long long)block[0] * ny);
+  groups = (unsigned long long)ctx->num_sms * EG_GROUP_THREADS / ((unsigned long long)block[0] * ny);
   if (groups == 0) groups = 1;
   L.chunk = (unsigned)((L.n + groups - 1) / groups);
   L.chunk = (L.chunk + EG_STEP - 1) / EG_STEP * EG_STEP;

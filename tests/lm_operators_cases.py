@@ -10,9 +10,6 @@ Tolerances. u = 2^-24 is half a step of float, 2^-11 of half. A result rounded
 once to half may be off by 2^-11 relative (2^-25 absolute near zero, half a
 step of the smallest halfs) beyond what float arithmetic leaves.
 """
-import ctypes
-import mmap
-
 import numpy as np
 import pytest
 
@@ -766,8 +763,8 @@ def test_embed_refusals(api, ctx):
     refused(api, api.GA_UNALIGNED_ERROR, lambda: api.GpuClipNorm(ctx)(e(ctx, (), np.float32), [odd], [odd], 1.0))
     refused(api, api.GA_INVALID_ERROR, lambda: api.embed(out, None, ids))
     L = api.lib()
-    assert L.GpuArray_embed(ctypes.byref(out.ga), ctypes.byref(table.ga), ctypes.byref(ids.ga), 1.0, 0, 64) == api.GA_INVALID_ERROR
-    assert L.GpuArray_embed(None, ctypes.byref(table.ga), ctypes.byref(ids.ga), 1.0, 0, 0) == api.GA_INVALID_ERROR
+    assert L.GpuArray_embed(out.at, table.at, ids.at, 1.0, 0, 64) == api.GA_INVALID_ERROR
+    assert L.GpuArray_embed(None, table.at, ids.at, 1.0, 0, 0) == api.GA_INVALID_ERROR
 
 
 def test_logprobs_refusals(api, ctx):
