@@ -17,7 +17,8 @@
  *    an infinite norm, zeros for finite elements and NaN for infinite ones
  *    (limit infinite: nothing is clipped).
  *  - dst[i] may be src[i] (nothing is written where the factor is 1); no other
- *    two arrays may overlap where one of them is a destination (GA_VALUE_ERROR). */
+ *    two arrays may overlap where one of them is a destination, the norm among
+ *    them (GA_VALUE_ERROR). */
 #ifndef GPUARRAY_CLIPNORM_H
 #define GPUARRAY_CLIPNORM_H
 

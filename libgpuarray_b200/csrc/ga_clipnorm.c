@@ -98,18 +98,19 @@ static int by_start(const void *a, const void *b) {
   return x->at < y->at ? -1 : x->at > y->at;
 }
 
-/* Sources may overlap each other; a destination may overlap nothing but be its own source. */
-static int check_overlap(GpuClipNorm *cn, GpuArray *const *dst, const GpuArray *const *src,
-                         unsigned int n) {
+/* Sources may overlap each other; a destination (the norm too, as array n) may overlap nothing but
+ * be its own source. */
+static int check_overlap(GpuClipNorm *cn, const GpuArray *norm, GpuArray *const *dst,
+                         const GpuArray *const *src, unsigned int n) {
   unsigned int i, k = 0;
   int sorted = 1;
   unsigned long long reach_dst = 0, reach_any = 0; /* ends of what came before */
   unsigned int who_any = 0, who_dst = 0;
-  if (2 * (size_t)n > cn->nspan) {
-    cn_span *s = realloc(cn->span, 2 * (size_t)n * sizeof(*s));
+  if (2 * (size_t)n + 1 > cn->nspan) {
+    cn_span *s = realloc(cn->span, (2 * (size_t)n + 1) * sizeof(*s));
     if (s == NULL) return ga_err_sys(cn->ctx->err, "realloc");
     cn->span = s;
-    cn->nspan = 2 * n;
+    cn->nspan = 2 * n + 1;
   }
   for (i = 0; i < n; i++) {
     const unsigned long long cnt = elements(src[i]);
@@ -127,6 +128,11 @@ static int check_overlap(GpuClipNorm *cn, GpuArray *const *dst, const GpuArray *
     if (s < d) sorted = 0;
     k++;
   }
+  cn->span[k].lo = norm->data->ptr + norm->offset;
+  cn->span[k].hi = cn->span[k].lo + gpuarray_get_elsize(norm->typecode);
+  cn->span[k].at = 2 * n + 1;
+  if (k > 0 && cn->span[k].lo < cn->span[k - 1].lo) sorted = 0;
+  k++;
   if (!sorted) qsort(cn->span, k, sizeof(*cn->span), by_start);
   for (i = 0; i < k; i++) {
     const cn_span *p = &cn->span[i];
@@ -224,7 +230,7 @@ int GpuClipNorm_call(GpuClipNorm *cn, GpuArray *norm, GpuArray *const *dst,
     err = check_one(ctx, src[i], dst != NULL ? dst[i] : NULL, i);
     if (err != GA_NO_ERROR) return err;
   }
-  if (dst != NULL && (err = check_overlap(cn, dst, src, n)) != GA_NO_ERROR) return err;
+  if (dst != NULL && (err = check_overlap(cn, norm, dst, src, n)) != GA_NO_ERROR) return err;
 
   /* the smallest table that holds the list: what a launch carries is copied with it */
   cap = n <= 32 ? 32 : n <= 128 ? 128 : CN_MAX_CAP;

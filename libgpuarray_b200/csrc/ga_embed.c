@@ -130,7 +130,7 @@ static int check_call(gpucontext *ctx, const GpuArray *by_row, double scale, int
 
 #define EM_TOKENS 256 /* GA_EM_TOKENS of the template */
 #define EM_MOST 64
-#define EM_CTAS 6     /* CTAs of 256 threads for every SM */
+#define EM_CTAS 12    /* CTAs of 256 threads for every SM, 5 of which it holds at once */
 
 int GpuArray_embed(GpuArray *out, const GpuArray *table, const GpuArray *ids, double scale,
                    ssize_t pad, int flags) {

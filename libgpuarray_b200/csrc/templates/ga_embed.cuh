@@ -102,7 +102,8 @@ static __device__ __forceinline__ V ga__em_zero() {
 }
 
 #ifdef GA_EM_BUILD_LOOKUP
-#define GA_EM_U 8        /* loads of a thread in flight */
+/* loads of a thread in flight (4 x 4095 tokens of 4096 halfs: 34 us with 4, 35 with 8, 42 with 16) */
+#define GA_EM_U 4
 #define GA_EM_TOKENS 256 /* of a CTA's groups at most */
 #define GA_EM_NOWHERE (-0x7fffffffffffffffLL) /* no offset of an array */
 /* A group of threads (blockIdx.x, threadIdx.y) owns L.chunk tokens and one slice of their rows, a
@@ -471,10 +472,11 @@ ga_eg_sort_all(const __grid_constant__ ga__em_layout L, const __grid_constant__ 
 }
 
 /* ---- summing ---- */
-/* tokens whose rows a thread has in flight, 16 bytes of each. Four of 4 CTAs an SM: 8 of 2 CTAs
- * are as many bytes, but fewer warps to go on while a run's end is written (two parts of 8190 rows
- * of 1021 floats: 114 against 134 us). */
-#define GA_EG_U 4
+/* tokens whose rows a thread has in flight, 16 bytes of each, in 4 CTAs an SM. Twice as many in half
+ * as many CTAs are as many bytes, but fewer warps to go on while a run's end is written; rows moved
+ * in several narrow vectors take more registers (two parts of 8190 rows of 1021 floats: 100 us with
+ * 2, 107 with 4, 125 with 4 in 2 CTAs; 32760 rows of 2048 halfs: 126 with 2, 119 with 4). */
+#define GA_EG_U (GA_EM_C > 1 ? 2 : 4)
 #define GA_EG_J 4 /* parts a thread has in flight */
 
 static __device__ __forceinline__ void ga__eg_park(GA_EM_F_T *p, const GA_EM_F_T acc[GA_EM_N]) {
@@ -500,7 +502,7 @@ static __device__ __forceinline__ void ga__eg_chunk(const ga__em_layout &L, char
   for (int j = 0; j < GA_EM_N; j++) acc[j] = 0;
   ga__em_out old; /* of row `cur` */
   for (unsigned int i = lo; i < hi && cur != none; i += GA_EG_U) {
-    struct alignas(16) {
+    struct alignas(4 * GA_EG_U) { /* i is a multiple of GA_EG_U */
       unsigned int v[GA_EG_U];
     } k;
     struct alignas(16) {

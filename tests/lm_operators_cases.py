@@ -167,7 +167,12 @@ def grad_tol(want, size, counts, dtype, f64):
 
 GRAD_CASES = [  # tokens, rows, width
     (1, 1, 1), (1, 5, 8), (2, 1, 3), (7, 3, 16), (40, 6, 5), (64, 64, 24), (100, 2, 9), (257, 30, 12), (300, 1, 4),
-    (512, 40, 33), (513, 3, 4), (2600, 600, 9), (5000, 511, 3), (700, 300000, 1), (17000, 900, 2),
+    (512, 40, 33),
+]
+SORTED_CASES = [  # more tokens than one launch of the direct kernel takes; one to three passes, runs across many chunks
+    (513, 3, 4, "f2", "f2", True), (2600, 600, 9, "f4", "f4", True), (2600, 600, 24, "f2", "f4", False),
+    (5000, 511, 3, "f4", "f4", False), (700, 300000, 1, "f4", "f4", True), (17000, 900, 2, "f2", "f2", False),
+    (1500, 2, 130, "f8", "f8", True),
 ]
 
 
@@ -175,6 +180,15 @@ GRAD_CASES = [  # tokens, rows, width
 @pytest.mark.parametrize("dout_dtype,out_dtype", [("f2", "f2"), ("f4", "f4"), ("f2", "f4"), ("f8", "f8")])
 @pytest.mark.parametrize("accumulate", [False, True])
 def test_embed_gradient(api, ctx, rng, tokens, rows, width, dout_dtype, out_dtype, accumulate):
+    embed_gradient_case(api, ctx, rng, tokens, rows, width, dout_dtype, out_dtype, accumulate)
+
+
+@pytest.mark.parametrize("case", SORTED_CASES, ids=str)
+def test_embed_gradient_of_sorted_tokens(api, ctx, rng, case):
+    embed_gradient_case(api, ctx, rng, *case)
+
+
+def embed_gradient_case(api, ctx, rng, tokens, rows, width, dout_dtype, out_dtype, accumulate):
     dout = rng.standard_normal((tokens, width)).astype(dout_dtype)
     ids = np.minimum(rng.geometric(0.3, tokens) - 1, rows - 1).astype(np.int32)   # few rows, often
     base = rng.standard_normal((rows, width)).astype(out_dtype)
@@ -242,6 +256,26 @@ def test_embed_gradient_strides_and_growing_calls(api, ctx, rng):
     op(dt, put(api, ctx, dout.T.copy()).transpose(), spread(api, ctx, ids))
     want, size, counts = grad_formula(3, dout, ids, 1.0, None)
     close(dt.to_numpy(), want, grad_tol(want, size, counts, "f4", False))
+
+
+def test_embed_gradient_of_a_broadcast_upstream(api, ctx, rng):
+    """one upstream row, and one upstream number, for all tokens (strides of 0); one id for all"""
+    rows, width, tokens = 7, 8, 600
+    ids = rng.integers(0, rows, tokens).astype(np.int64)
+    counts = np.bincount(ids, minlength=rows)
+    row = put(api, ctx, rng.integers(-4, 4, width).astype(np.float32))
+    op = api.GpuEmbedGrad(ctx)
+    dt = api.GpuArray.empty(ctx, (rows, width), np.float32)
+    for strides, each in (((0, 4), row.to_numpy()), ((0, 0), np.full(width, row.to_numpy()[0]))):
+        up = api.GpuArray.from_pointer(ctx, row.devptr, (tokens, width), np.float32, strides=strides, nbytes=4 * width)
+        op(dt, up, put(api, ctx, ids))
+        assert (dt.to_numpy() == counts[:, None] * each).all()          # small whole numbers: exact
+    one = put(api, ctx, ids[:1])
+    every = api.GpuArray.from_pointer(ctx, one.devptr, (tokens,), np.int64, strides=(0,), nbytes=8)
+    op(dt, up, every)
+    want = np.zeros((rows, width))
+    want[ids[0]] = tokens * row.to_numpy()[0]
+    assert (dt.to_numpy() == want).all()
 
 
 def test_embed_gradient_is_the_adjoint(api, ctx, rng):
@@ -463,6 +497,32 @@ def test_logprobs_ignored_and_bad_targets(api, ctx, rng):
     op(put(api, ctx, z[:1]), put(api, ctx, targets[:1]), logp=api.GpuArray.empty(ctx, (1,), np.float32), check=True)
 
 
+@pytest.mark.parametrize("dtype", ["f2", "f4"])
+def test_logprobs_of_one_row_and_of_repeated_rows(api, ctx, rng, dtype):
+    """a 1-d array of logits with 0-d results; the same row for every target (a stride of 0)"""
+    V = 300
+    z = rows_of_logits(rng, 1, V, dtype, "plain")
+    op = api.GpuLogProbs(ctx, dtype, np.int64, top=2)
+    e = api.GpuArray.empty
+    gz = put(api, ctx, z[0])
+    lp, tv, ti, st = e(ctx, (), "f4"), e(ctx, (2,), "f4"), e(ctx, (2,), "i8"), e(ctx, (2,), "f4")
+    op(gz, api.GpuArray.from_numpy(ctx, np.array(7, np.int64)), logp=lp, top_logp=tv, top_ids=ti, stats=st, check=True)
+    want, _, logs, p, _ = lp_formula(z, np.array([7]), 1.0)
+    tol = lp_tols(z, 1.0, p)[0] + 1e-5
+    close(lp.to_numpy(), want[0], tol[0])
+    assert (ti.to_numpy() == np.argsort(-z[0].astype(np.float64), kind="stable")[:2]).all()
+    dz = e(ctx, (V,), dtype)
+    op.grad(dz, gz, api.GpuArray.from_numpy(ctx, np.array(7, np.int64)), st, api.GpuArray.from_numpy(ctx, np.array(2, np.float32)))
+    g, p, logs, h = lp_grad_formula(z, np.array([7]), 1.0, np.array([2.0]), None)
+    t = lp_grad_tol(z, 1.0, p, logs, h, np.array([2.0]), None, dtype)
+    close(dz.to_numpy(), g[0], (t + U[np.dtype(dtype)] * (np.abs(g) + t) + TINY[np.dtype(dtype)])[0])
+    many = api.GpuArray.from_pointer(ctx, gz.devptr, (50, V), dtype, strides=(0, gz.dtype.itemsize), nbytes=V * gz.dtype.itemsize)
+    targets = rng.integers(0, V, 50)
+    out = e(ctx, (50,), "f4")
+    op(many, put(api, ctx, targets.astype(np.int64)), logp=out)
+    close(out.to_numpy(), lp_formula(np.repeat(z, 50, 0), targets, 1.0)[0], tol)
+
+
 def lp_grad_formula(z, targets, scale, a, b, ignore=None):
     logp, ent, logs, p, empty = lp_formula(z, targets, scale, ignore)
     t = targets.astype(np.int64)
@@ -521,6 +581,24 @@ def test_logprobs_gradient(api, ctx, rng, dtype, out_dtype, kind, rows, V, with_
     if dtype == out_dtype:                              # in place
         op.grad(gz, gz, gt, stats, put(api, ctx, a), scale=scale, ignore=-1, **more)
         assert (gz.to_numpy() == dz.to_numpy()).all()
+
+
+@pytest.mark.parametrize("dtype", ["f2", "f4"])
+def test_logprobs_gradient_of_rows_with_nans_and_infinities(api, ctx, rng, dtype):
+    """NaN throughout, but 0 in an ignored row whatever it holds"""
+    z = rows_of_logits(rng, 5, 40, dtype, "plain")
+    z[0, 3] = np.nan
+    z[1, 4] = INF
+    z[2] = np.nan
+    z[3, ::2] = INF
+    targets = np.array([1, 4, -1, -1, 6], np.int32)
+    op = api.GpuLogProbs(ctx, dtype, np.int32)
+    gz, gt = put(api, ctx, z), put(api, ctx, targets)
+    lp, stats = api.GpuArray.empty(ctx, (5,), np.float32), api.GpuArray.empty(ctx, (5, 2), np.float32)
+    op(gz, gt, logp=lp, stats=stats, ignore=-1)
+    op.grad(gz, gz, gt, stats, put(api, ctx, np.ones(5, np.float32)), ignore=-1)
+    g = gz.to_numpy()
+    assert np.isnan(g[:2]).all() and (g[2:4] == 0).all() and np.isfinite(g[4]).all()
 
 
 @pytest.mark.parametrize("dtype", ["f2", "f4"])
@@ -828,6 +906,9 @@ def test_clip_refusals(api, ctx):
     refused(api, V, lambda: op(norm, [a[:6], a[5:]], [a[:6], a[5:]], 1.0))
     refused(api, V, lambda: op(norm, [b, a], [a, b], 1.0))
     refused(api, V, lambda: op(norm, [a[:8]], [a[2:]], 1.0))
+    inside = api.GpuArray.from_pointer(ctx, a.devptr + 8, (), f, nbytes=4)
+    refused(api, V, lambda: op(inside, [a], [a], 1.0))
+    refused(api, V, lambda: op(inside, [b], [a], 1.0))
     op(norm, [a[:5], a[5:]], [a[:5], a[5:]], 1.0)
     with pytest.raises(ValueError):
         op(norm, [b], [a, b], 1.0)

@@ -107,7 +107,7 @@ def test_training_steps_replay_from_a_graph(api, ctx, rng):
     torch = pytest.importorskip("torch")
     stream = torch.cuda.ExternalStream(ctx.stream, device=0)
     steps = []
-    for V, B, S in ((200, 4, 33), (90, 2, 70)):
+    for V, B, S in ((200, 4, 300), (90, 2, 70)):   # sorted tokens, and few
         table, tokens, ops, buf = bigram_setup(api, ctx, rng, V, B, S, 0.05)
         gt, gk = put(api, ctx, table), put(api, ctx, tokens)
         bigram_step(api, ctx, gt, gk, ops, buf, 0.5, 0.05)
