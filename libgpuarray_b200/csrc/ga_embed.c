@@ -26,19 +26,19 @@ struct _GpuEmbedGrad {
 static int is_real(int tc) { return tc == GA_HALF || tc == GA_FLOAT || tc == GA_DOUBLE; }
 
 /* key: A type | O type << 8 | id type << 16 | E << 24 | ND << 32 | gradient << 40 |
- * accumulate << 41 | C << 48 | rounds of the one-launch sort << 56 */
+ * accumulate << 41 | C << 48 | rounds of the one-launch sort << 56 | its CTAs << 60 */
 static void emit(ga_strb *sb, uint64_t key) {
   const int a = (int)(key & 0xff), o = (int)((key >> 8) & 0xff), i = (int)((key >> 16) & 0xff);
   ga_strb_printf(sb,
                  "#include \"cluda.h\"\n#define %s\n#define GA_EM_A_T %s\n#define GA_EM_O_T %s\n"
                  "#define GA_EM_I_T %s\n#define GA_EM_F_T %s\n#define GA_EM_E %u\n"
                  "#define GA_EM_ND %u\n#define GA_EM_ACCUMULATE %u\n#define GA_EM_C %u\n"
-                 "#define GA_EG_ROUNDS %u\n#include \"ga_embed.cuh\"\n",
+                 "#define GA_EG_ROUNDS %u\n#define GA_EG_CLUSTER %u\n#include \"ga_embed.cuh\"\n",
                  (key >> 40) & 1 ? "GA_EM_BUILD_GRAD" : "GA_EM_BUILD_LOOKUP", ga_ctype(a), ga_ctype(o),
                  ga_ctype(i), a == GA_DOUBLE || o == GA_DOUBLE ? "ga_double" : "ga_float",
                  (unsigned)((key >> 24) & 0xff), (unsigned)((key >> 32) & 0xff),
                  (unsigned)((key >> 41) & 1), (unsigned)((key >> 48) & 0xff),
-                 (key >> 56) ? (unsigned)(key >> 56) : 1u);
+                 (key >> 56) ? (unsigned)((key >> 56) & 15) : 1u, (key >> 60) ? (unsigned)(key >> 60) : 1u);
 }
 
 static int check_types(gpucontext *ctx, const GpuArray *a, const GpuArray *o, const GpuArray *ids) {
@@ -212,14 +212,17 @@ void GpuEmbedGrad_free(GpuEmbedGrad *eg) {
 /* constants of the template */
 #define EG_STEP 8        /* a multiple of GA_EG_U */
 #define EG_X 64          /* threads along the rows: four or more share the joining of a run */
-#define EG_FEW 512       /* GA_EG_FEW */
+#define EG_FEW 1024      /* GA_EG_FEW */
 #define EG_TX 32         /* GA_EG_TX */
 #define EG_BITS 9        /* GA_EG_BITS */
 #define EG_THREADS 512   /* GA_EG_THREADS */
 #define EG_ROUND 2048    /* GA_EG_ROUND */
 #define EG_GROUP_THREADS 1024
-#define EG_CLUSTER 8     /* GA_EG_CLUSTER */
-#define EG_MAX_ROUNDS 4  /* of EG_ROUND tokens for each CTA of the cluster */
+#define EG_CHUNKS 16 /* chunks for every SM at most, where each takes a CTA to join */
+#define EG_CLUSTER 8     /* CTAs of the one-launch sort: one where EG_ALONE rounds are enough */
+#define EG_ALONE 2
+#define EG_MAX_ROUNDS 2  /* of EG_ROUND tokens for each CTA of the cluster; more tokens are sorted
+                            sooner by all SMs in several launches (65000: 29 us, one cluster 39) */
 #define EG_SHARED (16 * 512 * 4 + 8 * 512 * 4 + 512 * 4 + 16 * 4) /* ga__eg_shared without `keys` */
 #define EG_MAX_TILES 128 /* every sorting CTA reads all tiles' counts: 256 KiB at most */
 
@@ -334,6 +337,8 @@ int GpuEmbedGrad_call(GpuEmbedGrad *eg, GpuArray *dtable, const GpuArray *dout, 
   /* Chunks: threads for half the device, which with EG_STEP loads of a thread in flight keep the
    * memory busy; more and shorter ones only leave more parts to join. None shorter than one step. */
   groups = (unsigned long long)ctx->num_sms * EG_GROUP_THREADS / ((unsigned long long)block[0] * ny);
+  if (groups > (unsigned long long)ctx->num_sms * EG_CHUNKS && block[0] >= 32)
+    groups = (unsigned long long)ctx->num_sms * EG_CHUNKS;
   if (groups == 0) groups = 1;
   L.chunk = (unsigned)((L.n + groups - 1) / groups);
   L.chunk = (L.chunk + EG_STEP - 1) / EG_STEP * EG_STEP;
@@ -345,8 +350,8 @@ int GpuEmbedGrad_call(GpuEmbedGrad *eg, GpuArray *dtable, const GpuArray *dout, 
   S.pass = 0;
   one = L.n <= (unsigned long long)EG_CLUSTER * EG_ROUND * EG_MAX_ROUNDS;
   if (one) {
-    S.tiles = EG_CLUSTER;
-    for (rounds = 1; (unsigned long long)EG_CLUSTER * EG_ROUND * rounds < L.n; rounds *= 2) {}
+    S.tiles = L.n <= EG_ROUND * EG_ALONE ? 1 : EG_CLUSTER;
+    for (rounds = 1; (unsigned long long)S.tiles * EG_ROUND * rounds < L.n; rounds *= 2) {}
     S.tile = EG_ROUND * rounds;
   } else {
     S.tiles = (unsigned)((L.n + EG_ROUND - 1) / EG_ROUND);
@@ -357,7 +362,7 @@ int GpuEmbedGrad_call(GpuEmbedGrad *eg, GpuArray *dtable, const GpuArray *dout, 
 
   fsize = dout->typecode == GA_DOUBLE || dtable->typecode == GA_DOUBLE ? 8 : 4;
   list = ((size_t)(L.n + EG_STEP) * 4 + 511) / 512 * 512;
-  cbytes = one ? 0 : (size_t)S.passes * EG_THREADS * S.tiles * 4;
+  cbytes = one ? 0 : (size_t)EG_THREADS * S.tiles * 4;
   /* the sorted keys and offsets; for many tokens the counts and the lists between the passes */
   err = ga_workspace_need(ctx, &eg->ws, 3 * list + (one ? 0 : cbytes + 3 * list) +
                                             2 * (size_t)L.chunks * ny * block[0] * c * e * fsize);
@@ -377,7 +382,8 @@ int GpuEmbedGrad_call(GpuEmbedGrad *eg, GpuArray *dtable, const GpuArray *dout, 
   params[1] = &S;
   g1[0] = S.tiles;
   if (one) {
-    if ((err = ga_lm_kernel(ctx, "ga_eg_sort_all", key | (uint64_t)rounds << 56, emit, &sort)) != GA_NO_ERROR)
+    if ((err = ga_lm_kernel(ctx, "ga_eg_sort_all", key | (uint64_t)rounds << 56 | (uint64_t)S.tiles << 60, emit,
+                            &sort)) != GA_NO_ERROR)
       return err;
     params[2] = &p_ids;
     params[3] = &p_key[0];
@@ -389,13 +395,14 @@ int GpuEmbedGrad_call(GpuEmbedGrad *eg, GpuArray *dtable, const GpuArray *dout, 
     if ((err = ga_lm_kernel(ctx, "ga_eg_count", key, emit, &count)) != GA_NO_ERROR ||
         (err = ga_lm_kernel(ctx, "ga_eg_scatter", key, emit, &scatter)) != GA_NO_ERROR)
       return err;
+    last = (S.passes - 1) % 2;
     params[2] = &p_counts;
     params[3] = &p_ids;
-    params[4] = &p_err;
-    err = ga_launch(ctx, count, g1, flat, 0, params);
-    last = (S.passes - 1) % 2;
     for (; S.pass < S.passes && err == GA_NO_ERROR; S.pass++) {
       params[4] = &p_key[1 - S.pass % 2];
+      params[5] = &p_err;
+      err = ga_launch(ctx, count, g1, flat, 0, params);
+      if (err != GA_NO_ERROR) break;
       params[5] = &p_order[1 - S.pass % 2];
       params[6] = &p_key[S.pass % 2];
       params[7] = &p_order[S.pass % 2];
@@ -417,7 +424,7 @@ int GpuEmbedGrad_call(GpuEmbedGrad *eg, GpuArray *dtable, const GpuArray *dout, 
   if (err == GA_NO_ERROR && L.chunks > 1) {
     params[2] = &p_key[last];
     params[3] = &p_part;
-    grid[0] = L.chunks - 1;
+    grid[0] = block[0] < 32 ? (L.chunks + 6) / 8 : L.chunks - 1;
     err = ga_launch(ctx, join, grid, block, 0, params);
   }
   if (err == GA_NO_ERROR && ISSET(flags, GA_EMBED_CHECK))

@@ -159,8 +159,9 @@ ga_embed(const __grid_constant__ ga__em_layout L, char *out, const char *table, 
 #endif
 
 #ifdef GA_EM_BUILD_GRAD
-#ifndef GA_EG_ROUNDS
+#ifndef GA_EG_ROUNDS /* of the one-launch sort, and its CTAs */
 #define GA_EG_ROUNDS 1
+#define GA_EG_CLUSTER 1
 #endif
 /* The gradient is a sum over SORTED tokens, in launches that depend on nothing
  * but the ids' values, so that the result is the same bits every time.
@@ -170,9 +171,9 @@ ga_embed(const __grid_constant__ ga__em_layout L, char *out, const char *table, 
  * writes zeros and sums.
  *
  * More tokens: they are sorted by row and, within a row, by token (a radix sort
- * of GA_EG_BITS bits a pass), up to 65536 of them by one cluster in one launch
- * (ga_eg_sort_all), beyond by ga_eg_count and a ga_eg_scatter for each pass,
- * which also counts for the next. Tokens that contribute nothing get the key V
+ * of GA_EG_BITS bits a pass), up to 32768 of them by one CTA or cluster in one
+ * launch (ga_eg_sort_all), beyond by a ga_eg_count and a ga_eg_scatter for each
+ * pass. Tokens that contribute nothing get the key V
  * and go last. ga_eg_zero writes zeros to all rows beside the sort.
  * Then ga_eg_sum: the sorted tokens are cut into equal chunks; a group of
  * threads sums a chunk's rows, one vector position per thread. A run of equal
@@ -259,11 +260,18 @@ static __device__ __forceinline__ unsigned int ga__eg_key(const ga__em_layout &L
   return r < 0 ? (unsigned int)L.v : (unsigned int)r;
 }
 
-/* counts[pass][digit][tile]: how many keys of a tile have the digit. The first pass's are counted
- * here, the others' are set to zero for ga_eg_scatter to add to. */
+/* Key i of a pass: the first pass makes them from the ids. */
+static __device__ __forceinline__ unsigned int ga__eg_key_of(const ga__em_layout &L, const ga__eg_sort &S,
+                                                             const char *ids, const unsigned int *key_in,
+                                                             unsigned int i, int *err) {
+  return S.pass == 0 ? ga__eg_key(L, ids, i, err) : key_in[i];
+}
+
+/* counts[digit][tile]: how many keys of a tile have the digit. (Counting for the next pass where
+ * keys are scattered takes an atomic for each, thousands of them on the counts of a frequent id.) */
 extern "C" __global__ void __launch_bounds__(GA_EG_THREADS)
 ga_eg_count(const __grid_constant__ ga__em_layout L, const __grid_constant__ ga__eg_sort S,
-            unsigned int *counts, const char *ids, int *err) {
+            unsigned int *counts, const char *ids, const unsigned int *key_in, int *err) {
   ga__grid_dependency_sync();
   __shared__ unsigned int hist[GA_EG_DIGITS];
   const unsigned int d = threadIdx.x, tile = blockIdx.x;
@@ -271,11 +279,9 @@ ga_eg_count(const __grid_constant__ ga__em_layout L, const __grid_constant__ ga_
   __syncthreads();
   const unsigned int lo = tile * S.tile, hi = S.n - lo < S.tile ? S.n : lo + S.tile;
   for (unsigned int i = lo + threadIdx.x; i < hi; i += GA_EG_THREADS)
-    atomicAdd(&hist[ga__eg_key(L, ids, i, err) & (GA_EG_DIGITS - 1)], 1u);
+    atomicAdd(&hist[(ga__eg_key_of(L, S, ids, key_in, i, err) >> (S.pass * GA_EG_BITS)) & (GA_EG_DIGITS - 1)], 1u);
   __syncthreads();
   counts[d * S.tiles + tile] = hist[d];
-  for (unsigned int p = 1; p < S.passes; p++)
-    counts[(p * GA_EG_DIGITS + d) * S.tiles + tile] = 0;
 }
 
 /* The exclusive prefix of x over the CTA's GA_EG_THREADS threads. */
@@ -303,22 +309,38 @@ static __device__ __forceinline__ void ga__eg_places(const unsigned int digit[GA
                                                      const int live[GA_EG_KEYS], unsigned int &base,
                                                      ga__eg_table &cnt, unsigned int at[GA_EG_KEYS]) {
   const unsigned int d = threadIdx.x, lane = d % 32, warp = d / 32;
+#pragma unroll
   for (int w = 0; w < GA_EG_WARPS; w++) cnt[w][d] = 0;
+  /* the lanes with a key's digit, from a vote for each of its bits (one match instruction takes
+   * longer the more digits there are: a round 4 us, so 1.5) */
+  unsigned int same[GA_EG_KEYS];
+#pragma unroll
+  for (int j = 0; j < GA_EG_KEYS; j++) {
+    same[j] = __ballot_sync(0xffffffffu, live[j]);
+#pragma unroll
+    for (int b = 0; b < GA_EG_BITS; b++) {
+      const int bit = (digit[j] >> b) & 1;
+      const unsigned int set = __ballot_sync(0xffffffffu, bit);
+      same[j] &= bit ? set : ~set;
+    }
+  }
   __syncthreads();
 #pragma unroll
   for (int j = 0; j < GA_EG_KEYS; j++) {
-    const unsigned int same = __match_any_sync(0xffffffffu, live[j] ? digit[j] : GA_EG_DIGITS);
     const unsigned int seen = live[j] ? cnt[warp][digit[j]] : 0;
-    at[j] = seen + __popc(same & ((1u << lane) - 1));
+    at[j] = seen + __popc(same[j] & ((1u << lane) - 1));
     __syncwarp();
-    if (live[j] && __ffs(same) - 1 == (int)lane) cnt[warp][digit[j]] = seen + __popc(same);
+    if (live[j] && __ffs(same[j]) - 1 == (int)lane) cnt[warp][digit[j]] = seen + __popc(same[j]);
     __syncwarp();
   }
   __syncthreads();
+  unsigned int x[GA_EG_WARPS];
+#pragma unroll
+  for (int w = 0; w < GA_EG_WARPS; w++) x[w] = cnt[w][d];
+#pragma unroll
   for (int w = 0; w < GA_EG_WARPS; w++) { /* the digit's place for each warp */
-    const unsigned int x = cnt[w][d];
     cnt[w][d] = base;
-    base += x;
+    base += x[w];
   }
   __syncthreads();
 #pragma unroll
@@ -330,7 +352,7 @@ static __device__ __forceinline__ void ga__eg_places(const unsigned int digit[GA
  * of the tokens' rows of dout, so that the sums need no division. */
 extern "C" __global__ void __launch_bounds__(GA_EG_THREADS)
 ga_eg_scatter(const __grid_constant__ ga__em_layout L, const __grid_constant__ ga__eg_sort S,
-              unsigned int *counts, const char *ids,
+              const unsigned int *counts, const char *ids,
               const unsigned int *key_in, const unsigned int *order_in, unsigned int *key,
               unsigned int *order, long long *off) {
   ga__grid_dependency_sync();
@@ -340,7 +362,7 @@ ga_eg_scatter(const __grid_constant__ ga__em_layout L, const __grid_constant__ g
   const unsigned int shift = S.pass * GA_EG_BITS;
 
   /* where the digit's keys of this tile begin */
-  const unsigned int *c = counts + (S.pass * GA_EG_DIGITS + d) * S.tiles;
+  const unsigned int *c = counts + d * S.tiles;
   unsigned int total = 0, before = 0;
   for (unsigned int t = 0; t < S.tiles; t++) {
     const unsigned int x = c[t];
@@ -359,7 +381,7 @@ ga_eg_scatter(const __grid_constant__ ga__em_layout L, const __grid_constant__ g
       k[j] = o[j] = 0;
       live[j] = i < hi;
       if (live[j]) {
-        k[j] = S.pass == 0 ? ga__eg_key(L, ids, i, nullptr) : key_in[i];
+        k[j] = ga__eg_key_of(L, S, ids, key_in, i, nullptr);
         o[j] = S.pass == 0 ? i : order_in[i];
       }
       digit[j] = (k[j] >> shift) & (GA_EG_DIGITS - 1);
@@ -369,22 +391,16 @@ ga_eg_scatter(const __grid_constant__ ga__em_layout L, const __grid_constant__ g
     for (int j = 0; j < GA_EG_KEYS; j++) {
       if (!live[j]) continue;
       key[at[j]] = k[j];
-      if (S.pass + 1 == S.passes) {
-        off[at[j]] = ga__lm_offset<GA_EM_ND>(o[j], L.dims, L.t_str);
-      } else {
-        const unsigned int next = (k[j] >> (shift + GA_EG_BITS)) & (GA_EG_DIGITS - 1);
-        order[at[j]] = o[j];
-        atomicAdd(&counts[((S.pass + 1) * GA_EG_DIGITS + next) * S.tiles + at[j] / S.tile], 1u);
-      }
+      if (S.pass + 1 == S.passes) off[at[j]] = ga__lm_offset<GA_EM_ND>(o[j], L.dims, L.t_str);
+      else order[at[j]] = o[j];
     }
     __syncthreads();
   }
 }
 
-/* All passes in one launch, for as many tokens as the shared memory of one cluster holds: CTA r of
- * the cluster has the tokens, then the sorted keys, from r * GA_EG_TILE on. A pass counts
+/* All passes in one launch, for as many tokens as the shared memory of a CTA or of one cluster
+ * holds: CTA r of the cluster has the tokens, then the sorted keys, from r * GA_EG_TILE on. A pass counts
  * its digits, gives the counts to all CTAs, and sends every key to its place. */
-#define GA_EG_CLUSTER 8
 #define GA_EG_TILE (GA_EG_ROUND * GA_EG_ROUNDS)
 struct ga__eg_shared {
   ga__eg_table cnt;
@@ -394,12 +410,35 @@ struct ga__eg_shared {
   unsigned long long keys[GA_EG_TILE]; /* key << 32 | token */
 };
 
-extern "C" __global__ void __cluster_dims__(GA_EG_CLUSTER, 1, 1) __launch_bounds__(GA_EG_THREADS)
+/* all CTAs of the sort meet */
+static __device__ __forceinline__ void ga__eg_meet() {
+#if GA_EG_CLUSTER > 1
+  ga__cluster_arrive();
+  ga__cluster_wait();
+#else
+  __syncthreads();
+#endif
+}
+template <typename T>
+static __device__ __forceinline__ void ga__eg_put(T *p, unsigned int rank, T v) {
+#if GA_EG_CLUSTER > 1
+  ga__cluster_put(p, rank, v);
+#else
+  *p = v;
+#endif
+}
+
+extern "C" __global__ void __launch_bounds__(GA_EG_THREADS)
+#if GA_EG_CLUSTER > 1
+    __cluster_dims__(GA_EG_CLUSTER, 1, 1)
+#endif
 ga_eg_sort_all(const __grid_constant__ ga__em_layout L, const __grid_constant__ ga__eg_sort S,
                const char *ids, unsigned int *key, long long *off, int *err) {
   ga__grid_dependency_sync();
   GA_LM_SHARED_DYNAMIC(ga__eg_shared, sh);
+#if GA_EG_CLUSTER > 1
   ga__cluster_arrive(); /* waited for before the first store to another CTA's shared memory */
+#endif
   const unsigned int d = threadIdx.x, lane = d % 32, warp = d / 32, r = blockIdx.x;
   unsigned int k[GA_EG_ROUNDS][GA_EG_KEYS], o[GA_EG_ROUNDS][GA_EG_KEYS];
 #pragma unroll
@@ -410,7 +449,9 @@ ga_eg_sort_all(const __grid_constant__ ga__em_layout L, const __grid_constant__ 
       o[g][j] = i;
       k[g][j] = i < S.n ? ga__eg_key(L, ids, i, err) : 0;
     }
+#if GA_EG_CLUSTER > 1
   ga__cluster_wait();
+#endif
   for (unsigned int pass = 0; pass < S.passes; pass++) {
     const unsigned int shift = pass * GA_EG_BITS;
     sh.hist[d] = 0;
@@ -422,10 +463,9 @@ ga_eg_sort_all(const __grid_constant__ ga__em_layout L, const __grid_constant__ 
         if (r * GA_EG_TILE + g * GA_EG_ROUND + (warp * GA_EG_KEYS + j) * 32 + lane < S.n)
           atomicAdd(&sh.hist[(k[g][j] >> shift) & (GA_EG_DIGITS - 1)], 1u);
     __syncthreads();
-    for (unsigned int t = 0; t < GA_EG_CLUSTER; t++) ga__cluster_put(&sh.tab[r][d], t, sh.hist[d]);
+    for (unsigned int t = 0; t < GA_EG_CLUSTER; t++) ga__eg_put(&sh.tab[r][d], t, sh.hist[d]);
     /* behind this everybody has the counts, and has taken its keys out of `keys` */
-    ga__cluster_arrive();
-    ga__cluster_wait();
+    ga__eg_meet();
     unsigned int total = 0, before = 0;
 #pragma unroll
     for (unsigned int t = 0; t < GA_EG_CLUSTER; t++) {
@@ -447,19 +487,19 @@ ga_eg_sort_all(const __grid_constant__ ga__em_layout L, const __grid_constant__ 
 #pragma unroll
       for (int j = 0; j < GA_EG_KEYS; j++) {
         if (!live[j]) continue;
-        if (pass + 1 == S.passes) {
+        if (GA_EG_CLUSTER > 1 && pass + 1 == S.passes) {
           key[at[j]] = k[g][j];
           off[at[j]] = ga__lm_offset<GA_EM_ND>(o[g][j], L.dims, L.t_str);
         } else {
-          ga__cluster_put(&sh.keys[at[j] % GA_EG_TILE], at[j] / GA_EG_TILE,
-                          (unsigned long long)k[g][j] << 32 | o[g][j]);
+          ga__eg_put(&sh.keys[at[j] % GA_EG_TILE], at[j] / GA_EG_TILE,
+                     (unsigned long long)k[g][j] << 32 | o[g][j]);
         }
       }
       __syncthreads();
     }
-    if (pass + 1 == S.passes) return;
-    ga__cluster_arrive(); /* every key has arrived */
-    ga__cluster_wait();
+    if (GA_EG_CLUSTER > 1 && pass + 1 == S.passes) return;
+    ga__eg_meet(); /* every key has arrived */
+    if (pass + 1 == S.passes) break;
 #pragma unroll
     for (int g = 0; g < GA_EG_ROUNDS; g++)
 #pragma unroll
@@ -468,6 +508,13 @@ ga_eg_sort_all(const __grid_constant__ ga__em_layout L, const __grid_constant__ 
         k[g][j] = (unsigned int)(x >> 32);
         o[g][j] = (unsigned int)x;
       }
+  }
+  /* One CTA's lists leave in order: its scattered stores would take a cycle for each key (4096
+   * tokens 15.6 us, so 12.5). A cluster's have as many SMs to leave from. */
+  for (unsigned int i = d; i < GA_EG_TILE && r * GA_EG_TILE + i < S.n; i += GA_EG_THREADS) {
+    const unsigned long long x = sh.keys[i];
+    key[r * GA_EG_TILE + i] = (unsigned int)(x >> 32);
+    off[r * GA_EG_TILE + i] = ga__lm_offset<GA_EM_ND>((unsigned int)x, L.dims, L.t_str);
   }
 }
 
@@ -565,8 +612,8 @@ static __device__ __forceinline__ void ga__eg_chunk(const ga__em_layout &L, char
 
 /* Joins the run that starts in chunk c (tokens c * size ...) and goes on in the next, if there is
  * one: of the `ny` threads at a vector position thread y takes every ny-th part, then the first
- * adds their sums, always in the same order; with ny > 1 all threads of the CTA are here for the
- * same c. part: the chunks' parked rows at this thread's vectors, heads and tails in turn, `step`
+ * adds their sums, always in the same order; with ny > 1 all threads of a warp, or of the CTA where
+ * there are 32 or more along the row, are here for the same c. part: the chunks' parked rows at this thread's vectors, heads and tails in turn, `step`
  * elements apart. sum: with ny > 1, 256 * GA_EM_N entries of shared memory. */
 static __device__ __forceinline__ void ga__eg_join_run(const ga__em_layout &L, char *dtable,
                                                        const unsigned int *key, unsigned int c,
@@ -614,13 +661,16 @@ static __device__ __forceinline__ void ga__eg_join_run(const ga__em_layout &L, c
         for (int j = 0; j < GA_EM_N; j++) acc[j] += x[u][j];
       }
     }
-    if (y > 0) ga__eg_park(sum + (y * blockDim.x + threadIdx.x) * GA_EM_N, acc);
+    if (y > 0) ga__eg_park(sum + (threadIdx.y * blockDim.x + threadIdx.x) * GA_EM_N, acc);
   }
-  if (ny > 1) __syncthreads();
+  if (ny > 1) {
+    if (blockDim.x < 32) __syncwarp();
+    else __syncthreads();
+  }
   if (!inside || y > 0) return;
   for (unsigned int i = 1; i < ny; i++)
 #pragma unroll
-    for (int j = 0; j < GA_EM_N; j++) acc[j] += sum[(i * blockDim.x + threadIdx.x) * GA_EM_N + j];
+    for (int j = 0; j < GA_EM_N; j++) acc[j] += sum[((threadIdx.y + i) * blockDim.x + threadIdx.x) * GA_EM_N + j];
   ga__eg_write(L, dtable, cur, pos, acc, old);
 }
 
@@ -639,19 +689,22 @@ ga_eg_sum(const __grid_constant__ ga__em_layout L, char *dtable, const char *dou
 }
 
 /* A CTA for each chunk but the last (blockIdx.x) and slice of the rows, with as many threads along
- * them as in ga_eg_sum; most find nothing to join. */
+ * them as in ga_eg_sum; a warp where these are fewer than 32. Most find nothing to join. */
 extern "C" __global__ void __launch_bounds__(256)
 ga_eg_join(const __grid_constant__ ga__em_layout L, char *dtable, const unsigned int *key,
            const GA_EM_F_T *part) {
   ga__grid_dependency_sync();
   __shared__ GA_EM_F_T sum[256 * GA_EM_N];
-  ga__eg_join_run(L, dtable, key, blockIdx.x, L.chunk, L.chunks, ga__em_here(L),
+  const unsigned int narrow = blockDim.x < 32, ny = narrow ? 32 / blockDim.x : blockDim.y;
+  const unsigned int c = narrow ? blockIdx.x * 8 + threadIdx.y / ny : blockIdx.x;
+  if (c + 1 >= L.chunks) return; /* whole warps */
+  ga__eg_join_run(L, dtable, key, c, L.chunk, L.chunks, ga__em_here(L),
                   part + (size_t)(blockIdx.y * blockDim.x + threadIdx.x) * GA_EM_N,
-                  (size_t)gridDim.y * blockDim.x * GA_EM_N, threadIdx.y, blockDim.y, sum);
+                  (size_t)gridDim.y * blockDim.x * GA_EM_N, threadIdx.y % ny, ny, sum);
 }
 
 /* ---- few tokens ---- */
-#define GA_EG_FEW 512 /* tokens at most */
+#define GA_EG_FEW 1024 /* tokens at most */
 #define GA_EG_FEW_WARPS 8
 #define GA_EG_TX 32   /* vector positions of a CTA at most; blockDim.x * blockDim.y is 256 */
 
@@ -660,10 +713,13 @@ extern "C" __global__ void __launch_bounds__(256)
 ga_eg_direct(const __grid_constant__ ga__em_layout L, char *dtable, const char *dout,
              const char *ids, int *err) {
   ga__grid_dependency_sync();
-  __shared__ unsigned int row[GA_EG_FEW], token[GA_EG_FEW], key[GA_EG_FEW + GA_EG_U];
+  __shared__ unsigned int key[GA_EG_FEW + GA_EG_U], found[GA_EG_FEW_WARPS];
   __shared__ long long off[GA_EG_FEW + GA_EG_U];
-  __shared__ unsigned int found[GA_EG_FEW_WARPS];
-  __shared__ GA_EM_F_T part[256 * 2 * GA_EM_N];
+  /* the rows and numbers of the CTA's tokens; when these are sorted, the parts of runs */
+  alignas(16) __shared__ char both[sizeof(GA_EM_F_T) * 256 * 2 * GA_EM_N > 8 * GA_EG_FEW
+                                       ? sizeof(GA_EM_F_T) * 256 * 2 * GA_EM_N : 8 * GA_EG_FEW];
+  unsigned int *row = reinterpret_cast<unsigned int *>(both), *token = row + GA_EG_FEW;
+  GA_EM_F_T *part = reinterpret_cast<GA_EM_F_T *>(both);
   const unsigned int tid = threadIdx.y * blockDim.x + threadIdx.x, lane = tid % 32, warp = tid / 32;
   const unsigned int n = (unsigned int)L.n;
   const unsigned long long r0 = (unsigned long long)blockIdx.x * L.chunk;
@@ -693,7 +749,10 @@ ga_eg_direct(const __grid_constant__ ga__em_layout L, char *dtable, const char *
   for (unsigned int i = tid; i < m; i += 256) {
     const unsigned int k = row[i];
     unsigned int at = 0;
-    for (unsigned int j = 0; j < m; j++) at += row[j] < k || (row[j] == k && j < i);
+    if (r1 - r0 == 1) at = i; /* one row: in order already */
+    else
+#pragma unroll 4
+      for (unsigned int j = 0; j < m; j++) at += row[j] < k + (j < i);
     key[at] = k;
     off[at] = ga__lm_offset<GA_EM_ND>(token[i], L.dims, L.t_str);
   }

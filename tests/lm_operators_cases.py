@@ -167,12 +167,12 @@ def grad_tol(want, size, counts, dtype, f64):
 
 GRAD_CASES = [  # tokens, rows, width
     (1, 1, 1), (1, 5, 8), (2, 1, 3), (7, 3, 16), (40, 6, 5), (64, 64, 24), (100, 2, 9), (257, 30, 12), (300, 1, 4),
-    (512, 40, 33),
+    (512, 40, 33), (1024, 9, 6),
 ]
 SORTED_CASES = [  # more tokens than one launch of the direct kernel takes; one to three passes, runs across many chunks
-    (513, 3, 4, "f2", "f2", True), (2600, 600, 9, "f4", "f4", True), (2600, 600, 24, "f2", "f4", False),
-    (5000, 511, 3, "f4", "f4", False), (700, 300000, 1, "f4", "f4", True), (17000, 900, 2, "f2", "f2", False),
-    (1500, 2, 130, "f8", "f8", True),
+    (1025, 3, 4, "f2", "f2", True), (2600, 600, 9, "f4", "f4", True), (2600, 600, 24, "f2", "f4", False),
+    (5000, 511, 3, "f4", "f4", False), (1100, 300000, 1, "f4", "f4", True), (17000, 900, 2, "f2", "f2", False),
+    (1500, 2, 130, "f8", "f8", True), (33000, 700, 2, "f4", "f4", True),
 ]
 
 
@@ -260,7 +260,7 @@ def test_embed_gradient_strides_and_growing_calls(api, ctx, rng):
 
 def test_embed_gradient_of_a_broadcast_upstream(api, ctx, rng):
     """one upstream row, and one upstream number, for all tokens (strides of 0); one id for all"""
-    rows, width, tokens = 7, 8, 600
+    rows, width, tokens = 7, 8, 1200
     ids = rng.integers(0, rows, tokens).astype(np.int64)
     counts = np.bincount(ids, minlength=rows)
     row = put(api, ctx, rng.integers(-4, 4, width).astype(np.float32))

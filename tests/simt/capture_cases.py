@@ -32,9 +32,9 @@ def test_captured_calls(api, ctx, rng, capturing):
         lp(out, t, logp=logp, stats=stats, check=check)
         lp.grad(out, out, t, stats, dl, check=check)
     every(False)
-    eg(table, long[:600], more[:600])                  # sorted tokens: the workspace is made
+    eg(table, long[:1100], more[:1100])                  # sorted tokens: the workspace is made
     capturing(1)
-    eg(table, long[:600], more[:600])
+    eg(table, long[:1100], more[:1100])
     every(False)                                       # a repeated call needs nothing new
     for call in (lambda: api.embed(out, table, ids, check=True), lambda: eg(table, out, ids, check=True),
                  lambda: lp(out, t, logp=logp, check=True), lambda: lp.grad(out, out, t, stats, dl, check=True),
