@@ -43,29 +43,29 @@ template <>
 struct ga__lm_type<ga_half> {
   template <int N, typename F>
   static __device__ __forceinline__ void get(F x[N], const ga__lm_raw<2 * N> &q) {
-    if (N == 1) {
+    if constexpr (N == 1) {
       ga_half h;
       h.data = (ga_ushort)q.w[0];
       x[0] = (F)ga_half2float(h);
-      return;
-    }
+    } else {
 #pragma unroll
-    for (int j = 0; j < N / 2; j++) {
-      float a, b;
-      ga__unpack_h2(q.w[j], a, b);
-      x[2 * j] = (F)a;
-      x[2 * j + 1] = (F)b;
+      for (int j = 0; j < N / 2; j++) {
+        float a, b;
+        ga__unpack_h2(q.w[j], a, b);
+        x[2 * j] = (F)a;
+        x[2 * j + 1] = (F)b;
+      }
     }
   }
   /* a double narrows to half through float: two roundings, each to nearest */
   template <int N, typename F>
   static __device__ __forceinline__ void put(ga__lm_raw<2 * N> &q, const F x[N]) {
-    if (N == 1) {
+    if constexpr (N == 1) {
       q.w[0] = ga_float2half((float)x[0]).data;
-      return;
-    }
+    } else {
 #pragma unroll
-    for (int j = 0; j < N / 2; j++) q.w[j] = ga__pack_h2((float)x[2 * j], (float)x[2 * j + 1]);
+      for (int j = 0; j < N / 2; j++) q.w[j] = ga__pack_h2((float)x[2 * j], (float)x[2 * j + 1]);
+    }
   }
 };
 template <>
