@@ -724,12 +724,26 @@ ga_eg_direct(const __grid_constant__ ga__em_layout L, char *dtable, const char *
   const unsigned int n = (unsigned int)L.n;
   const unsigned long long r0 = (unsigned long long)blockIdx.x * L.chunk;
   const unsigned long long r1 = L.v - r0 < L.chunk ? L.v : r0 + L.chunk;
+  /* all keys are on their way, and the zeros, before the first is looked at (1024 halfs on (32000,
+   * 1024): 18.5 us; keys 256 at a time with zeros after the sort: 19.8; 20 tokens: 4.0 and 3.9) */
+  unsigned int all_keys[GA_EG_FEW / 256];
+#pragma unroll
+  for (int j = 0; j < GA_EG_FEW / 256; j++) {
+    const unsigned int i = j * 256 + tid;
+    all_keys[j] = i < n ? ga__eg_key(L, ids, i, blockIdx.x == 0 && blockIdx.y == 0 ? err : nullptr) : (unsigned int)L.v;
+  }
+  const ga__em_pos pos = ga__em_here(L);
+#if !GA_EM_ACCUMULATE
+  if (pos.v < L.nv)
+    for (unsigned long long r = r0 + threadIdx.y; r < r1; r += blockDim.y)
+      ga__em_write(dtable + (long long)r * L.v_row, L.v_col, pos, ga__em_zero<ga__em_out>());
+#endif
   /* the tokens of these rows, in their order */
   unsigned int m = 0;
-  for (unsigned int i0 = 0; i0 < n; i0 += 256) {
-    const unsigned int i = i0 + tid;
-    unsigned long long r = L.v;
-    if (i < n) r = ga__eg_key(L, ids, i, blockIdx.x == 0 && blockIdx.y == 0 ? err : nullptr);
+#pragma unroll
+  for (int j = 0; j < GA_EG_FEW / 256; j++) {
+    if (j * 256 >= n) break;
+    const unsigned int r = all_keys[j];
     const int mine = r >= r0 && r < r1;
     const unsigned int all = __ballot_sync(0xffffffffu, mine);
     if (lane == 0) found[warp] = __popc(all);
@@ -740,8 +754,8 @@ ga_eg_direct(const __grid_constant__ ga__em_layout L, char *dtable, const char *
       m += found[w];
     }
     if (mine) {
-      row[at] = (unsigned int)r;
-      token[at] = i;
+      row[at] = r;
+      token[at] = j * 256 + tid;
     }
     __syncthreads();
   }
@@ -756,12 +770,6 @@ ga_eg_direct(const __grid_constant__ ga__em_layout L, char *dtable, const char *
     key[at] = k;
     off[at] = ga__lm_offset<GA_EM_ND>(token[i], L.dims, L.t_str);
   }
-  const ga__em_pos pos = ga__em_here(L);
-#if !GA_EM_ACCUMULATE
-  if (pos.v < L.nv)
-    for (unsigned long long r = r0 + threadIdx.y; r < r1; r += blockDim.y)
-      ga__em_write(dtable + (long long)r * L.v_row, L.v_col, pos, ga__em_zero<ga__em_out>());
-#endif
   __syncthreads();
   if (m == 0) return;
   const unsigned int size = (m + blockDim.y - 1) / blockDim.y, chunks = (m + size - 1) / size;
