@@ -172,7 +172,7 @@ GRAD_CASES = [  # tokens, rows, width
 SORTED_CASES = [  # more tokens than one launch of the direct kernel takes; one to three passes, runs across many chunks
     (1025, 3, 4, "f2", "f2", True), (2600, 600, 9, "f4", "f4", True), (2600, 600, 24, "f2", "f4", False),
     (5000, 511, 3, "f4", "f4", False), (1100, 300000, 1, "f4", "f4", True), (17000, 900, 2, "f2", "f2", False),
-    (1500, 2, 130, "f8", "f8", True), (33000, 700, 2, "f4", "f4", True),
+    (1500, 2, 130, "f8", "f8", True), (4096, 90, 3, "f4", "f4", True), (4097, 90, 3, "f2", "f4", False), (33000, 700, 2, "f4", "f4", True),
 ]
 
 

@@ -153,3 +153,23 @@ def test_clip_many_and_large(api, ctx, rng):
         want = np.sqrt((flat.astype(np.float64) ** 2).sum())
         assert abs(float(norm.to_numpy()) - want) <= 1e-12 * want
         close(to.to_numpy(), flat * (2.0 / want), np.abs(flat) * (2.0 / want) * 4 * 2.0 ** -24)
+
+
+def test_two_contexts_side_by_side(api, ctx, rng):
+    """the operators on two contexts (two streams) of one device, their calls interleaved and
+    nothing waited for in between"""
+    other = api.Context(0, kernel_cache=None)
+    work = []
+    for c, V, B, S in ((ctx, 150, 3, 500), (other, 60, 5, 700)):
+        table, tokens, ops, buf = bigram_setup(api, c, rng, V, B, S, 0.05)
+        work.append((c, table, tokens, ops, buf, put(api, c, table), put(api, c, tokens)))
+    for _ in range(5):
+        for c, table, tokens, ops, buf, gt, gk in work:
+            bigram_step(api, c, gt, gk, ops, buf, 0.5, 0.05)
+    for c, table, tokens, ops, buf, gt, gk in work:
+        logp, ent, dt, norm = bigram_formula(table, tokens, 0.05, 0.5)
+        close(buf["logp"].to_numpy(), logp, 1e-4)
+        close(buf["norm"].to_numpy(), norm, 1e-4 * norm)
+        close(buf["dtable"].to_numpy(), dt, 1e-4)
+    del work, c, ops, buf, gt, gk
+    other.close()
