@@ -310,7 +310,8 @@ int GpuEmbedGrad_call(GpuEmbedGrad *eg, GpuArray *dtable, const GpuArray *dout, 
   if (err != GA_NO_ERROR) return err;
   if (L.n > 0x7fffffffULL)
     return ga_err_set(ctx->err, GA_XLARGE_ERROR, "More than 2^31 - 1 tokens in one call");
-  if (L.nv == 0 || (L.n == 0 && accumulate)) return GA_NO_ERROR;
+  /* without tokens there are zeros to write at most, for rows that there are */
+  if (L.nv == 0 || (L.n == 0 && (accumulate || L.v == 0))) return GA_NO_ERROR;
 
   key = (uint64_t)dout->typecode | (uint64_t)dtable->typecode << 8 | (uint64_t)ids->typecode << 16 |
         (uint64_t)e << 24 | (uint64_t)lead.nd << 32 | (uint64_t)1 << 40 | (uint64_t)accumulate << 41 |

@@ -222,6 +222,23 @@ def test_embed_gradient_ranks_padding_and_bad_ids(api, ctx, rng, shape, id_dtype
         assert e.value.code == api.GA_VALUE_ERROR
 
 
+@pytest.mark.parametrize("tokens", [0, 5, 1500])
+@pytest.mark.parametrize("accumulate", [False, True])
+def test_embed_gradient_of_an_empty_table(api, ctx, accumulate, tokens):
+    """no rows to write: nothing happens, and every id is outside the table"""
+    op = api.GpuEmbedGrad(ctx)
+    dt, dout = api.GpuArray.empty(ctx, (0, 8), np.float32), api.GpuArray.empty(ctx, (tokens, 8), np.float32)
+    ids = api.GpuArray.from_numpy(ctx, np.zeros(tokens, np.int64))
+    op(dt, dout, ids, accumulate=accumulate)
+    op(dt, dout, ids, accumulate=accumulate, pad=0, check=True)
+    if tokens:
+        with pytest.raises(api.GpuArrayException) as e:
+            op(dt, dout, ids, accumulate=accumulate, check=True)
+        assert e.value.code == api.GA_VALUE_ERROR
+    else:
+        op(dt, dout, ids, accumulate=accumulate, check=True)
+
+
 def test_embed_gradient_negative_ids_and_all_padding(api, ctx, rng):
     dout = rng.standard_normal((6, 4)).astype(np.float32)
     ids = np.array([-1, 3, -4, 0, 3, -5], np.int64)
