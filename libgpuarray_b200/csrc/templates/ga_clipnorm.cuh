@@ -187,9 +187,14 @@ ga_cn_norm(const __grid_constant__ ga__cn_layout L, double *part, ga__cn_result 
   }
 }
 
+/* Arithmetic in F. The factor's product with a float is one in double where no normal float holds the
+ * factor, as that of large gradients and a small limit: elements and results may be ordinary floats
+ * all the same. */
 template <typename T, typename D, typename F>
-static __device__ __forceinline__ void ga__cn_scale(const ga__cn_item &t, unsigned int b, F factor) {
+static __device__ __forceinline__ void ga__cn_scale(const ga__cn_item &t, unsigned int b, double factor) {
   const int E = 16 / (int)sizeof(T);
+  const F f = (F)factor;
+  const int wide = sizeof(F) == 4 && (fabs(factor) < 1.1754943508222875e-38 || fabs(factor) > 3.4028234663852886e38);
   typedef ga__lm_vec<D, E> vec;
   const ga__cn_at a = ga__cn_open<(int)sizeof(T)>(t, b);
   char *base = t.dst - a.skip * sizeof(D);
@@ -202,7 +207,7 @@ static __device__ __forceinline__ void ga__cn_scale(const ga__cn_item &t, unsign
     F x[E];
     ga__lm_get<T, E>(x, q[u]);
 #pragma unroll
-    for (int j = 0; j < E; j++) x[j] *= factor;
+    for (int j = 0; j < E; j++) x[j] = wide ? (F)((double)x[j] * factor) : x[j] * f;
     if (aligned && (a.inner || (w * E >= a.skip && i + E <= t.n))) {
       vec o;
       ga__lm_put<D, E>(o, x);
@@ -224,16 +229,15 @@ extern "C" __global__ void __launch_bounds__(GA_CN_THREADS)
 ga_cn_scale(const __grid_constant__ ga__cn_layout L, const ga__cn_result *res) {
   ga__grid_dependency_sync();
   const double factor = __ldcg(&res->factor);
-  const float f = (float)factor;
   const unsigned int b = L.blocks - 1 - blockIdx.x;
   const ga__cn_item &t = L.item[ga__cn_find(L, b)];
   /* an array that stays where it is and is multiplied by one is what it was */
   if (t.dst == t.src && t.stype == t.dtype && factor == 1.0) return;
   if (t.stype == 0) {
-    if (t.dtype == 0) ga__cn_scale<ga_half, ga_half, float>(t, b, f);
-    else ga__cn_scale<ga_half, ga_float, float>(t, b, f);
+    if (t.dtype == 0) ga__cn_scale<ga_half, ga_half, float>(t, b, factor);
+    else ga__cn_scale<ga_half, ga_float, float>(t, b, factor);
   } else if (t.stype == 1) {
-    ga__cn_scale<ga_float, ga_float, float>(t, b, f);
+    ga__cn_scale<ga_float, ga_float, float>(t, b, factor);
   } else {
     ga__cn_scale<ga_double, ga_double, double>(t, b, factor);
   }

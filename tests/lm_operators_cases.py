@@ -755,6 +755,34 @@ def test_clip_infinities_nans_and_the_range_of_float(api, ctx, rng):
         clip_check(api, norm.to_numpy(), [dst.to_numpy()], [a], 1.0, limit, ["f4"])
 
 
+@pytest.mark.parametrize("values,times,limit,scale", [
+    ([1e38], 4, 1e-3, 1.0), ([1e38], 4, 1e-6, 1.0), ([1e38], 4, 1e-9, 1.0), ([3e38, -1e38, 2e30], 700, 1e-6, 1.0),
+    ([3e38, 1.0], 1, INF, 1e-40), ([1e-38, -3e-39], 1, INF, 1e39), ([1e-44, 0.0], 1, 1e-3, 1e45)])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_clip_factors_outside_the_range_of_float(api, ctx, values, times, limit, scale, in_place):
+    """a factor that no normal float holds, between inputs and results that are floats. Its product
+    is taken in double: the norm's error, one rounding to double and one to float are left"""
+    a = np.array(values * times, np.float32)
+    src, norm = put(api, ctx, a), api.GpuArray.empty(ctx, (), np.float64)
+    dst = src if in_place else api.GpuArray.empty(ctx, a.shape, np.float32)
+    api.GpuClipNorm(ctx)(norm, [dst], [src], limit, scale=scale)
+    want_norm, f, want = clip_formula([a], scale, limit)
+    assert np.isfinite(want[0]).all() and want[0].any() and not 2.0 ** -126 <= abs(f) < 2.0 ** 128
+    close(norm.to_numpy(), want_norm, 1e-13 * want_norm, "norm")
+    close(dst.to_numpy(), want[0], 1.01 * 2.0 ** -24 * np.abs(want[0]) + 2.0 ** -150)
+
+
+def test_clip_of_halfs_by_a_factor_below_the_floats(api, ctx):
+    """halfs into floats: results are floats although the factor is not a normal one"""
+    a = np.array([60000.0, -0.25, 6e-8, 1000.0] * 3, np.float16)
+    dst, norm = api.GpuArray.empty(ctx, a.shape, np.float32), api.GpuArray.empty(ctx, (), np.float64)
+    api.GpuClipNorm(ctx)(norm, [dst], [put(api, ctx, a)], 1e-35)
+    want_norm, f, want = clip_formula([a], 1.0, 1e-35)
+    # squares of 8 halfs are summed in float: at most 8 half steps of the sum, half of that in the norm
+    close(norm.to_numpy(), want_norm, 1.01 * 4 * 2.0 ** -24 * want_norm, "norm")
+    close(dst.to_numpy(), want[0], 1.01 * 5 * 2.0 ** -24 * np.abs(want[0]) + 2.0 ** -150)
+
+
 def test_clip_leaves_what_need_not_change(api, ctx, rng):
     """in place below the limit: the same bits; between arrays: untouched"""
     a = rng.standard_normal(1000).astype(np.float32)
