@@ -12,7 +12,9 @@
  *    that their type has; anything else is GA_INVALID_ERROR. Arrays without
  *    elements are allowed.
  *  - Squares are summed in double in an order that the sizes alone decide:
- *    equal calls give equal bits, and no finite float overflows.
+ *    equal calls give equal bits, and no finite float overflows (doubles beyond
+ *    1e154 do: an infinite norm). Products with the factor are rounded to the
+ *    type of dst whatever the factor's size.
  *  - A NaN anywhere gives a NaN norm and NaN in every dst; an infinity gives
  *    an infinite norm, zeros for finite elements and NaN for infinite ones
  *    (limit infinite: nothing is clipped).

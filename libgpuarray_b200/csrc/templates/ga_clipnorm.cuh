@@ -179,9 +179,10 @@ ga_cn_norm(const __grid_constant__ ga__cn_layout L, double *part, ga__cn_result 
   if (threadIdx.x == 0) {
     s = 0.0;
     for (int i = 0; i < GA_CN_THREADS / 32; i++) s += warps[i];
-    const double v = sqrt(s) * fabs(L.scale);
+    const double size = sqrt(s), v = size * fabs(L.scale);
     res->ticket = 0;
-    res->factor = v != v ? v : (v > L.limit ? L.scale * (L.limit / v) : L.scale);
+    /* scale * limit / v without the scale, whose product with the size need not be a double */
+    res->factor = v != v ? v : (v > L.limit ? copysign(L.limit / size, L.scale) : L.scale);
     if (norm_is_double) *reinterpret_cast<double *>(norm) = v;
     else *reinterpret_cast<float *>(norm) = (float)v;
   }

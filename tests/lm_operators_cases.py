@@ -783,6 +783,17 @@ def test_clip_of_halfs_by_a_factor_below_the_floats(api, ctx):
     close(dst.to_numpy(), want[0], 1.01 * 5 * 2.0 ** -24 * np.abs(want[0]) + 2.0 ** -150)
 
 
+def test_clip_where_scale_and_norm_leave_the_doubles(api, ctx):
+    """|scale| times the norm, or the limit over it, may be no double: dst is +-limit / |src| all the same"""
+    op, norm = api.GpuClipNorm(ctx), api.GpuArray.empty(ctx, (), np.float64)
+    for scale, limit in ((1e300, 1e-200), (-1e300, 2.0), (1e300, 1e300)):
+        a = np.array([3.0, 4e20], np.float64)
+        dst = api.GpuArray.empty(ctx, a.shape, np.float64)
+        op(norm, [dst], [put(api, ctx, a)], limit, scale=scale)
+        want = np.sign(scale) * a / np.sqrt((a * a).sum()) * limit
+        close(dst.to_numpy(), want, 8 * 2.0 ** -53 * np.abs(want))
+
+
 def test_clip_leaves_what_need_not_change(api, ctx, rng):
     """in place below the limit: the same bits; between arrays: untouched"""
     a = rng.standard_normal(1000).astype(np.float32)
