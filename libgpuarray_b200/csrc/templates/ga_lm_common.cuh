@@ -123,7 +123,9 @@ static __device__ __forceinline__ long long ga__lm_offset(unsigned long long i,
                                                           const long long *strs) {
   if (ND <= 1) return (long long)i * strs[0];
   long long p = 0;
-  if (i <= 0xffffffffULL) { /* quotients of 32-bit numbers are several times cheaper */
+  /* Quotients of 32-bit numbers are several times cheaper; i is below the number that stands for a
+   * longer dimension. */
+  if (i < 0xffffffffULL) {
     unsigned int r = (unsigned int)i;
 #pragma unroll
     for (int d = ND - 1; d > 0; d--) {
