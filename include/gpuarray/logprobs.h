@@ -15,7 +15,10 @@
  *  - Logits are GA_HALF or GA_FLOAT; the last axis is the vocabulary (1 to
  *    2^28 - 1 entries), the others are the rows. Tokens are GA_INT, GA_UINT,
  *    GA_LONG or GA_ULONG. All other results and inputs are GA_FLOAT; dlogits is
- *    GA_FLOAT or the logits' type. Arithmetic is in float.
+ *    GA_FLOAT or the logits' type. Arithmetic is in float. scale is positive
+ *    and at most 2.358e38, so that scale * log2 e is a float (GA_VALUE_ERROR).
+ *    Differences of logits are taken before it: where two finite logits are
+ *    further apart than the largest float, the lower one has probability 0.
  *  - Offsets and strides are honoured; inputs of the gradient may have strides
  *    of 0 (one dlogp for all rows). Adjacent logits are fastest; rows may start
  *    at any element. dlogits may be the logits themselves; other overlaps of a

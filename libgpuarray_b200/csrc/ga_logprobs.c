@@ -27,6 +27,7 @@ typedef struct lp_variant {
   unsigned threads, group, cluster, nd;
 } lp_variant;
 
+#define LP_LOG2E 1.4426950408889634f /* GA_LP_LOG2E of the template */
 #define LP_U 4 /* vectors of a thread in one step: GA_LP_U of the template */
 
 static uint64_t variant_key(const lp_variant *v) {
@@ -114,8 +115,8 @@ static int check_common(GpuLogProbs *lp, const GpuArray *logits, double scale, i
     return ga_err_set(ctx->err, GA_VALUE_ERROR, "logits has no vocabulary axis");
   if (logits->dimensions[logits->nd - 1] >= (1UL << 28))
     return ga_err_set(ctx->err, GA_XLARGE_ERROR, "The vocabulary has 2^28 entries or more");
-  if (!(scale > 0) || isinf((float)scale) || (float)scale == 0)
-    return ga_err_set(ctx->err, GA_VALUE_ERROR, "scale must be positive and finite");
+  if (!(scale > 0) || isinf((float)scale * LP_LOG2E) || (float)scale == 0) /* the kernels' exponents */
+    return ga_err_set(ctx->err, GA_VALUE_ERROR, "scale must be positive, and finite as a float times log2 e");
   if (flags & ~(GA_LOGPROBS_IGNORE | GA_LOGPROBS_CHECK))
     return ga_err_fmt(ctx->err, GA_INVALID_ERROR, "Unknown flags 0x%x", flags);
   if (ISSET(flags, GA_LOGPROBS_CHECK) && ga_lm_capturing(ctx))

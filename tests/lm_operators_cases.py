@@ -515,6 +515,27 @@ def test_logprobs_ignored_and_bad_targets(api, ctx, rng):
 
 
 @pytest.mark.parametrize("dtype", ["f2", "f4"])
+def test_logprobs_scales_near_the_largest_float(api, ctx, dtype):
+    """refused where scale log2(e) is no float, and right below that"""
+    V = api.GA_VALUE_ERROR
+    z, t = put(api, ctx, np.array([[1, 1, 0.5, 1], [0, -0.25, -1, -2]], dtype)), put(api, ctx, np.array([1, 0], np.int64))
+    e = api.GpuArray.empty
+    op, lp, en, st = api.GpuLogProbs(ctx, dtype, np.int64), e(ctx, (2,), "f4"), e(ctx, (2,), "f4"), e(ctx, (2, 2), "f4")
+    largest = float(np.finfo(np.float32).max) / np.log2(np.e)
+    for bad in (largest * 1.0001, 2.4e38, 3e38, 3.4028235e38):
+        refused(api, V, lambda: op(z, t, logp=lp, entropy=en, stats=st, scale=bad))
+        refused(api, V, lambda: op.grad(z, z, t, st, lp, scale=bad))
+    op(z, t, logp=lp, entropy=en, stats=st, scale=largest * 0.9999, check=True)
+    # equal logits share the mass, the others have none; two roundings of a logarithm and its part
+    close(lp.to_numpy(), [-np.log(3), 0], 8 * 2.0 ** -24)
+    close(en.to_numpy(), [np.log(3), 0], 8 * 2.0 ** -24)
+    dz = put(api, ctx, np.full((2, 4), 7, np.float32))
+    op.grad(dz, z, t, st, put(api, ctx, np.full(2, 1e-38, np.float32)), scale=largest * 0.9999)
+    a = np.float32(1e-38).astype(np.float64) * largest * 0.9999
+    close(dz.to_numpy(), [[-a / 3, a * 2 / 3, 0, -a / 3], [0, 0, 0, 0]], 16 * 2.0 ** -24 * a)
+
+
+@pytest.mark.parametrize("dtype", ["f2", "f4"])
 def test_logprobs_of_one_row_and_of_repeated_rows(api, ctx, rng, dtype):
     """a 1-d array of logits with 0-d results; the same row for every target (a stride of 0)"""
     V = 300
