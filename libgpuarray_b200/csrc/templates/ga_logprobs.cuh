@@ -714,7 +714,8 @@ ga_lp_rows(const __grid_constant__ ga__lp_layout L, const char *logits, const ch
 #endif
     if (stats != nullptr) {
       char *p = stats + ga__lm_offset<GA_LP_ND>(row, L.dims, L.o_str[2]);
-      *reinterpret_cast<float *>(p) = empty ? minus_inf : st.m;
+      /* m leaves NaNs out: the sum tells */
+      *reinterpret_cast<float *>(p) = empty ? minus_inf : st.s == st.s ? st.m : st.s;
       *reinterpret_cast<float *>(p + L.o_col[2]) = ls;
     }
   }

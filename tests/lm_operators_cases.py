@@ -536,6 +536,26 @@ def test_logprobs_scales_near_the_largest_float(api, ctx, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["f2", "f4"])
+@pytest.mark.parametrize("V", [1, 40, 5000])
+def test_logprobs_stats_of_rows_with_nans_and_infinities(api, ctx, rng, dtype, V):
+    """both numbers are NaN, and -inf in a row of -inf; the others are what they are alone"""
+    z = rows_of_logits(rng, 6, V, dtype, "plain")
+    z[0, V // 2] = np.nan
+    z[1, V - 1] = INF
+    z[2] = np.nan
+    z[3, ::2] = INF
+    z[4] = -INF
+    st, one = api.GpuArray.empty(ctx, (6, 2), np.float32), api.GpuArray.empty(ctx, (1, 2), np.float32)
+    op = api.GpuLogProbs(ctx, dtype, np.int32)
+    op(put(api, ctx, z), stats=st)
+    op(put(api, ctx, z[5:]), stats=one)
+    got = st.to_numpy()
+    assert np.isnan(got[:4]).all(), got
+    assert (got[4] == -INF).all()
+    assert got[5, 0] == one.to_numpy()[0, 0] == z[5].max() and abs(got[5, 1] - one.to_numpy()[0, 1]) <= 2 * lp_tols(z[5:], 1.0, lp_formula(z[5:], None, 1.0)[3])[0]
+
+
+@pytest.mark.parametrize("dtype", ["f2", "f4"])
 def test_logprobs_of_one_row_and_of_repeated_rows(api, ctx, rng, dtype):
     """a 1-d array of logits with 0-d results; the same row for every target (a stride of 0)"""
     V = 300
