@@ -816,13 +816,14 @@ ga_lp_grad(const __grid_constant__ ga__lp_layout L, char *dlogits, const char *l
   const float m = *reinterpret_cast<const float *>(sp);
   const float ls = *reinterpret_cast<const float *>(sp + L.o_col[0]);
   float a = *reinterpret_cast<const float *>(dlogp + ga__lm_offset<GA_LP_ND>(row, L.dims, L.o_str[1]));
-  int none = 0;
+  int none = 0; /* the row's gradient is `fill` throughout */
+  float fill = 0.0f;
   if (L.has_ignore && target == L.ignore) {
     a = 0.0f;
     target = -1;
     none = !GA_LP_ENT;
   } else if (target < 0 || target >= (long long)L.v) {
-    a = __uint_as_float(0x7fffffffu);
+    a = fill = __uint_as_float(0x7fffffffu);
     if (w0 == 0 && err != nullptr) *err = -1;
   }
   if (m == __uint_as_float(0xff800000u)) none = 1; /* nothing above -inf in the row */
@@ -855,7 +856,7 @@ ga_lp_grad(const __grid_constant__ ga__lp_layout L, char *dlogits, const char *l
       float x[2 * GA_LP_PAIRS];
       if (none) {
 #pragma unroll
-        for (int j = 0; j < 2 * GA_LP_PAIRS; j++) x[j] = 0.0f;
+        for (int j = 0; j < 2 * GA_LP_PAIRS; j++) x[j] = fill;
       } else {
 #pragma unroll
         for (int k = 0; k < GA_LP_PAIRS; k++) {

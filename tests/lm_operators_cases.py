@@ -660,6 +660,27 @@ def test_logprobs_gradient_of_rows_with_nans_and_infinities(api, ctx, rng, dtype
 
 
 @pytest.mark.parametrize("dtype", ["f2", "f4"])
+@pytest.mark.parametrize("with_entropy", [False, True])
+def test_logprobs_gradient_of_bad_targets_in_empty_rows(api, ctx, dtype, with_entropy):
+    """a target outside the vocabulary gives a logp and a gradient row of NaN, in a row without a
+    logit above -inf too; 0 there for any other target"""
+    V = 70
+    z = np.full((5, V), -INF, dtype)
+    z[4] = 0.5
+    t = np.array([V, -1, 3, -7, 1000], np.int64)         # outside, ignored, inside, outside, outside
+    op = api.GpuLogProbs(ctx, dtype, np.int64)
+    gz, gt = put(api, ctx, z), put(api, ctx, t)
+    e = api.GpuArray.empty
+    lp, en, st = e(ctx, (5,), "f4"), e(ctx, (5,), "f4"), e(ctx, (5, 2), "f4")
+    op(gz, gt, logp=lp, entropy=en, stats=st, ignore=-1)
+    assert (np.isnan(lp.to_numpy()) == [True, False, False, True, True]).all()
+    dz, one = put(api, ctx, np.full((5, V), 7, dtype)), put(api, ctx, np.ones(5, np.float32))
+    op.grad(dz, gz, gt, st, one, ignore=-1, **(dict(entropy=en, dentropy=one) if with_entropy else {}))
+    got = dz.to_numpy()
+    assert np.isnan(got[[0, 3, 4]]).all() and (got[1:3] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", ["f2", "f4"])
 def test_logprobs_gradient_strides_and_broadcast_inputs(api, ctx, rng, dtype):
     V = 53
     z = rows_of_logits(rng, 6, V, dtype, "plain").reshape(2, 3, V)
