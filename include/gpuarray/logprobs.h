@@ -29,8 +29,9 @@
  *  - GA_LOGPROBS_IGNORE: rows whose target equals `ignore` have logp 0, which has
  *    no gradient: the dlogp term is dropped whatever the row holds.
  *  - Any other target outside [0, V) gives a logp and a gradient row of NaN,
- *    whatever the row holds; with GA_LOGPROBS_CHECK the call also waits for the result and returns
- *    GA_VALUE_ERROR (not while a CUDA graph is captured: GA_UNSUPPORTED_ERROR). */
+ *    whatever the row holds; with GA_LOGPROBS_CHECK the call also waits for the
+ *    result and returns GA_VALUE_ERROR (not while a CUDA graph is captured:
+ *    GA_UNSUPPORTED_ERROR). */
 #ifndef GPUARRAY_LOGPROBS_H
 #define GPUARRAY_LOGPROBS_H
 

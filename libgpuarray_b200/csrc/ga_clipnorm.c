@@ -148,6 +148,18 @@ static int check_overlap(GpuClipNorm *cn, const GpuArray *norm, GpuArray *const 
   return GA_NO_ERROR;
 }
 
+/* The same where the norm is the only destination. */
+static int check_norm_overlap(gpucontext *ctx, const GpuArray *norm, const GpuArray *const *src, unsigned int n) {
+  const unsigned long long lo = norm->data->ptr + norm->offset, hi = lo + gpuarray_get_elsize(norm->typecode);
+  unsigned int i;
+  for (i = 0; i < n; i++) {
+    const unsigned long long cnt = elements(src[i]), s = src[i]->data->ptr + src[i]->offset;
+    if (cnt > 0 && s < hi && lo < s + cnt * gpuarray_get_elsize(src[i]->typecode))
+      return ga_err_fmt(ctx->err, GA_VALUE_ERROR, "The norm overlaps src[%u]", i);
+  }
+  return GA_NO_ERROR;
+}
+
 /* ga_lm_check, the array's place in the list named only where there is something to say */
 static int check_listed(gpucontext *ctx, const GpuArray *a, const char *list, unsigned int i, int dest) {
   char why[GA_ERR_MSGLEN];
@@ -230,7 +242,8 @@ int GpuClipNorm_call(GpuClipNorm *cn, GpuArray *norm, GpuArray *const *dst,
     err = check_one(ctx, src[i], dst != NULL ? dst[i] : NULL, i);
     if (err != GA_NO_ERROR) return err;
   }
-  if (dst != NULL && (err = check_overlap(cn, norm, dst, src, n)) != GA_NO_ERROR) return err;
+  err = dst != NULL ? check_overlap(cn, norm, dst, src, n) : check_norm_overlap(ctx, norm, src, n);
+  if (err != GA_NO_ERROR) return err;
 
   /* the smallest table that holds the list: what a launch carries is copied with it */
   cap = n <= 32 ? 32 : n <= 128 ? 128 : CN_MAX_CAP;

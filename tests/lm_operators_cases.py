@@ -1032,6 +1032,25 @@ def test_clip_refusals(api, ctx):
         op(norm, [b], [a, b], 1.0)
 
 
+def test_clip_refuses_a_norm_inside_a_source_without_destinations(api, ctx):
+    e = api.GpuArray.empty
+    f = np.float32
+    op, a, b = api.GpuClipNorm(ctx), put(api, ctx, np.ones(10, f)), put(api, ctx, np.ones(3, f))
+    for k in (0, 2, 9):
+        inside = api.GpuArray.from_pointer(ctx, a.devptr + 4 * k, (), f, nbytes=4)
+        for src in ([a], [b, a], [a, b, a], [a[k:], b]):
+            refused(api, api.GA_VALUE_ERROR, lambda: op(inside, None, src, 1.0))
+        op(inside, None, [b, a[:k], a[k + 1:]], 1.0)       # beside the sources, and one of no elements
+        assert float(inside.to_numpy()) == np.sqrt(f(12))
+        a.write(np.ones(10, f))
+    wide = api.GpuArray.from_pointer(ctx, a.devptr + 24, (), np.float64, nbytes=8)
+    refused(api, api.GA_VALUE_ERROR, lambda: op(wide, None, [a[7:]], 1.0))
+    op(wide, None, [a[7:7], b[:0]], 1.0)                   # arrays without elements overlap nothing
+    assert float(wide.to_numpy()) == 0
+    a.write(np.ones(10, f))
+    assert (a.to_numpy() == 1).all()
+
+
 def test_arrays_of_another_context_are_refused(api, ctx):
     other = api.Context(0)
     f = np.float32
