@@ -57,10 +57,16 @@ struct ga__lm_type<ga_half> {
       }
     }
   }
-  /* a double narrows to half through float: two roundings, each to nearest */
+  /* one rounding: a double does not go by way of float */
   template <int N, typename F>
   static __device__ __forceinline__ void put(ga__lm_raw<2 * N> &q, const F x[N]) {
-    if constexpr (N == 1) {
+    if constexpr (sizeof(F) == 8) {
+#pragma unroll
+      for (int j = 0; j < (N + 1) / 2; j++) {
+        q.w[j] = ga__half_bits((double)x[2 * j]);
+        if constexpr (N > 1) q.w[j] |= (unsigned int)ga__half_bits((double)x[2 * j + 1]) << 16;
+      }
+    } else if constexpr (N == 1) {
       q.w[0] = ga_float2half((float)x[0]).data;
     } else {
 #pragma unroll

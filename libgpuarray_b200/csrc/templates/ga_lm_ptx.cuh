@@ -38,6 +38,12 @@ static __device__ __forceinline__ unsigned int ga__pack_h2(float lo, float hi) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(hi), "f"(lo));
   return w;
 }
+/* a double as half, with one rounding */
+static __device__ __forceinline__ unsigned short ga__half_bits(double x) {
+  unsigned short w;
+  asm("cvt.rn.f16.f64 %0, %1;" : "=h"(w) : "d"(x));
+  return w;
+}
 
 /* Two floats handled by one instruction (sm_100: packed add, multiply, fused multiply-add) */
 struct ga__f2 {

@@ -88,6 +88,36 @@ def test_embed_types_and_widths(api, ctx, rng, width, table_dtype, out_dtype):
     close(out.to_numpy(), want, embed_tol(want, out_dtype, "f8" in (table_dtype, out_dtype)))
 
 
+@pytest.mark.parametrize("width", [1, 8, 11])
+def test_embed_and_gradient_round_doubles_to_halfs_once(api, ctx, width):
+    """doubles next to the middle between two halfs: by way of float they would come to lie on it,
+    and go to the even one"""
+    step = 2.0 ** -10
+    k = np.arange(23 * width).reshape(23, width)
+    middle = (1 + step / 2 + step * (k % 1000)) * 2.0 ** (k % 9 - 4) * (-1.0) ** k
+    v = middle * (1 + 2.0 ** -40 * (1 - 2 * (k // 2 % 2)))
+    v[0, 0], v[1, 0], v[2, 0] = 2.0 ** -24 * (0.5 + 2.0 ** -40), 65520 * (1 - 2.0 ** -40), 1e300     # smallest, largest, infinite
+    with np.errstate(over="ignore"):
+        want = v.astype(np.float16)                        # one rounding to nearest
+        assert (want != v.astype(np.float32).astype(np.float16)).any()
+    ids = np.arange(23)[::-1].astype(np.int64)
+    out = api.GpuArray.empty(ctx, (23, width), np.float16)
+    api.embed(out, put(api, ctx, v), put(api, ctx, ids), check=True)
+    assert (out.to_numpy() == want[ids]).all()
+    op = api.GpuEmbedGrad(ctx)
+    op(out, put(api, ctx, v), put(api, ctx, ids), check=True)
+    assert (out.to_numpy() == want[ids]).all()
+    # sorted tokens: six times the row more for the first three, in parts of 2^-6; a sum's few roundings
+    # to double are far below its distance of 2^-40 to a middle
+    many = np.concatenate([ids, np.repeat(ids[:3], 64 * 6)])
+    up = np.concatenate([v, np.repeat(v[:3] / 64, 64 * 6, 0)])
+    op(out, put(api, ctx, up), put(api, ctx, many), check=True)
+    sums = v.copy()
+    sums[:3] *= 7
+    with np.errstate(over="ignore"):
+        assert (out.to_numpy() == sums.astype(np.float16)[ids]).all()
+
+
 @pytest.mark.parametrize("id_dtype", ["i4", "u4", "i8", "u8"])
 @pytest.mark.parametrize("shape", [(), (1,), (5,), (2, 3), (2, 3, 2), (0,), (3, 0)])
 def test_embed_ids_of_any_rank_and_type(api, ctx, rng, id_dtype, shape):

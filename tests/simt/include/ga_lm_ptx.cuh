@@ -75,6 +75,12 @@ static inline void ga__add_h2_f32(unsigned int w, float c, float &lo, float &hi)
 static inline unsigned int ga__pack_h2(float lo, float hi) {
   return (unsigned int)ga_float2half(lo).data | (unsigned int)ga_float2half(hi).data << 16;
 }
+static inline unsigned short ga__half_bits(double x) {
+  const _Float16 v = (_Float16)x; /* one rounding to nearest even */
+  unsigned short w;
+  memcpy(&w, &v, 2);
+  return w;
+}
 static inline unsigned int ga__max_h2(unsigned int a, unsigned int b) {
   float al, ah, bl, bh;
   ga__unpack_h2(a, al, ah);
