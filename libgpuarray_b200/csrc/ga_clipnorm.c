@@ -5,7 +5,7 @@
 
 #define CN_MAX_CAP 960     /* entries of the largest table: a parameter block holds 32764 bytes */
 #define CN_VECS 2048       /* GA_CN_VECS of the template */
-#define CN_CTAS_PER_SM 8   /* 256 threads each: all that fit */
+#define CN_CTAS_PER_SM 8   /* 256 threads each; an SM holds 5 of them at once (48 registers a thread) */
 
 typedef struct cn_item { /* the template's ga__cn_item */
   CUdeviceptr src, dst;

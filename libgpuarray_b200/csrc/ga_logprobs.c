@@ -264,7 +264,8 @@ int GpuLogProbs_call(GpuLogProbs *lp, GpuArray *logp, GpuArray *entropy, GpuArra
   return err;
 }
 
-#define LP_CTAS 16 /* of 256 threads, 4 of which an SM holds at once */
+#define LP_CTAS 16 /* of 256 threads, 3 of which an SM holds at once where logits are adjacent (80 registers
+                      a thread; one word of it spilled for halfs without entropy and one leading dimension) */
 
 int GpuLogProbs_grad(GpuLogProbs *lp, GpuArray *dlogits, const GpuArray *logits,
                      const GpuArray *targets, const GpuArray *stats, const GpuArray *dlogp,
