@@ -129,14 +129,11 @@ static __device__ __forceinline__ long long ga__lm_offset(unsigned long long i,
                                                           const long long *strs) {
   if (ND <= 1) return (long long)i * strs[0];
   long long p = 0;
-  /* Quotients of 32-bit numbers are several times cheaper; i is below the number that stands for a
-   * longer dimension. */
-  if (i < 0xffffffffULL) {
+  if (i <= 0xffffffffULL) { /* quotients of 32-bit numbers are several times cheaper */
     unsigned int r = (unsigned int)i;
 #pragma unroll
     for (int d = ND - 1; d > 0; d--) {
-      const unsigned int n = dims[d] > 0xffffffffULL ? 0xffffffffu : (unsigned int)dims[d];
-      const unsigned int q = r / n;
+      const unsigned int n = (unsigned int)dims[d], q = dims[d] > 0xffffffffULL ? 0 : r / n;
       p += (long long)(r - q * n) * strs[d];
       r = q;
     }
