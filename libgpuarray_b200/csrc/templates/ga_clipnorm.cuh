@@ -188,14 +188,27 @@ ga_cn_norm(const __grid_constant__ ga__cn_layout L, double *part, ga__cn_result 
   }
 }
 
-/* Arithmetic in F. The factor's product with a float is one in double where no normal float holds the
- * factor, as that of large gradients and a small limit: elements and results may be ordinary floats
- * all the same. */
+/* Halfs and floats times a factor that no normal float holds, as that of large gradients and a small
+ * limit: elements and results may be ordinary floats all the same, so products are taken in double.
+ * An element at a time, apart from the loops below, which it would make slower (0.7 % on 295 M halfs). */
+static __device__ __forceinline__ void ga__cn_scale_wide(const ga__cn_item &t, unsigned int b, double factor) {
+  const unsigned int E = t.stype == 0 ? 8 : 4, es = 16 / E, skip = (unsigned int)((size_t)t.src & 15) / es;
+  const unsigned long long first = (unsigned long long)(b - t.first) * GA_CN_VECS * E;
+  for (unsigned int k = threadIdx.x; k < GA_CN_VECS * E; k += GA_CN_THREADS) {
+    const unsigned long long i = first + k - skip; /* wraps below the start */
+    if (i >= t.n) continue;
+    float x;
+    if (t.stype == 0) x = ga_half2float(*reinterpret_cast<const ga_half *>(t.src + i * 2));
+    else x = *reinterpret_cast<const float *>(t.src + i * 4);
+    const double y = (double)x * factor;
+    if (t.dtype == 0) *reinterpret_cast<unsigned short *>(t.dst + i * 2) = ga__half_bits(y);
+    else *reinterpret_cast<float *>(t.dst + i * 4) = (float)y;
+  }
+}
+
 template <typename T, typename D, typename F>
-static __device__ __forceinline__ void ga__cn_scale(const ga__cn_item &t, unsigned int b, double factor) {
+static __device__ __forceinline__ void ga__cn_scale(const ga__cn_item &t, unsigned int b, F factor) {
   const int E = 16 / (int)sizeof(T);
-  const F f = (F)factor;
-  const int wide = sizeof(F) == 4 && (fabs(factor) < 1.1754943508222875e-38 || fabs(factor) > 3.4028234663852886e38);
   typedef ga__lm_vec<D, E> vec;
   const ga__cn_at a = ga__cn_open<(int)sizeof(T)>(t, b);
   char *base = t.dst - a.skip * sizeof(D);
@@ -208,7 +221,7 @@ static __device__ __forceinline__ void ga__cn_scale(const ga__cn_item &t, unsign
     F x[E];
     ga__lm_get<T, E>(x, q[u]);
 #pragma unroll
-    for (int j = 0; j < E; j++) x[j] = wide ? (F)((double)x[j] * factor) : x[j] * f;
+    for (int j = 0; j < E; j++) x[j] *= factor;
     if (aligned && (a.inner || (w * E >= a.skip && i + E <= t.n))) {
       vec o;
       ga__lm_put<D, E>(o, x);
@@ -230,15 +243,19 @@ extern "C" __global__ void __launch_bounds__(GA_CN_THREADS)
 ga_cn_scale(const __grid_constant__ ga__cn_layout L, const ga__cn_result *res) {
   ga__grid_dependency_sync();
   const double factor = __ldcg(&res->factor);
+  const float f = (float)factor;
   const unsigned int b = L.blocks - 1 - blockIdx.x;
   const ga__cn_item &t = L.item[ga__cn_find(L, b)];
   /* an array that stays where it is and is multiplied by one is what it was */
   if (t.dst == t.src && t.stype == t.dtype && factor == 1.0) return;
+  const double size = fabs(factor); /* zero, after an infinite norm or for a limit of 0, is a float */
+  if (t.stype != 2 && size != 0.0 && (size < 1.1754943508222875e-38 || size > 3.4028234663852886e38))
+    return ga__cn_scale_wide(t, b, factor);
   if (t.stype == 0) {
-    if (t.dtype == 0) ga__cn_scale<ga_half, ga_half, float>(t, b, factor);
-    else ga__cn_scale<ga_half, ga_float, float>(t, b, factor);
+    if (t.dtype == 0) ga__cn_scale<ga_half, ga_half, float>(t, b, f);
+    else ga__cn_scale<ga_half, ga_float, float>(t, b, f);
   } else if (t.stype == 1) {
-    ga__cn_scale<ga_float, ga_float, float>(t, b, factor);
+    ga__cn_scale<ga_float, ga_float, float>(t, b, f);
   } else {
     ga__cn_scale<ga_double, ga_double, double>(t, b, factor);
   }
