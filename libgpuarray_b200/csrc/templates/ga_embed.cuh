@@ -28,9 +28,10 @@ struct ga__em_layout {
   long long t_col, v_row, v_col; /* its element stride; the table's (dtable's) row and element stride */
 };
 
-/* Table row of token i's id, or -1 for the padding id, -2 for an id outside the table. */
-static __device__ __forceinline__ long long ga__em_row(const ga__em_layout &L, const char *ids,
-                                                       unsigned long long i) {
+/* Table row of token i's id, or -1 for the padding id, -2 for an id outside the table. The lookup
+ * counts tokens in 64 bits, the gradient (up to 2^31 - 1 of them) in 32. */
+template <typename I>
+static __device__ __forceinline__ long long ga__em_row(const ga__em_layout &L, const char *ids, I i) {
   const GA_EM_I_T raw =
       *reinterpret_cast<const GA_EM_I_T *>(ids + ga__lm_offset<GA_EM_ND>(i, L.dims, L.i_str));
   long long r = (long long)raw;

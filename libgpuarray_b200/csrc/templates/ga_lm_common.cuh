@@ -122,23 +122,29 @@ static __device__ __forceinline__ void ga__lm_put(ga__lm_vec<T, N> &q, const F x
 
 #define GA_LM_MAXD 4
 
-/* Byte offset of leading index i: the dimensions left after collapsing, last one fastest. */
+/* Byte offset of leading index i: the dimensions left after collapsing, last one fastest. Quotients
+ * of 32-bit numbers are several times cheaper; an index of 32 bits is below 2^32 - 1, which stands for
+ * any longer dimension. */
+template <int ND>
+static __device__ __forceinline__ long long ga__lm_offset(unsigned int i, const unsigned long long *dims,
+                                                          const long long *strs) {
+  long long p = 0;
+#pragma unroll
+  for (int d = ND - 1; d > 0; d--) {
+    const unsigned int n = dims[d] > 0xffffffffULL ? 0xffffffffu : (unsigned int)dims[d];
+    const unsigned int q = i / n;
+    p += (long long)(i - q * n) * strs[d];
+    i = q;
+  }
+  return p + (long long)i * strs[0];
+}
 template <int ND>
 static __device__ __forceinline__ long long ga__lm_offset(unsigned long long i,
                                                           const unsigned long long *dims,
                                                           const long long *strs) {
   if (ND <= 1) return (long long)i * strs[0];
+  if (i < 0xffffffffULL) return ga__lm_offset<ND>((unsigned int)i, dims, strs);
   long long p = 0;
-  if (i <= 0xffffffffULL) { /* quotients of 32-bit numbers are several times cheaper */
-    unsigned int r = (unsigned int)i;
-#pragma unroll
-    for (int d = ND - 1; d > 0; d--) {
-      const unsigned int n = (unsigned int)dims[d], q = dims[d] > 0xffffffffULL ? 0 : r / n;
-      p += (long long)(r - q * n) * strs[d];
-      r = q;
-    }
-    return p + (long long)r * strs[0];
-  }
 #pragma unroll
   for (int d = ND - 1; d > 0; d--) {
     const unsigned long long q = i / dims[d];

@@ -15,6 +15,14 @@ TEMPLATES = os.path.join(ROOT, "libgpuarray_b200", "csrc", "templates")
 SOURCE = """
 #include "ga_lm_common.cuh"
 extern "C" long long offset(int nd, unsigned long long i, const unsigned long long *dims, const long long *strs) {
+  if (i < 0x80000000ULL) { /* an index of 32 bits */
+    const unsigned int j = (unsigned int)i;
+    const long long p = nd == 1 ? ga__lm_offset<1>(j, dims, strs) : nd == 2 ? ga__lm_offset<2>(j, dims, strs)
+                      : nd == 3 ? ga__lm_offset<3>(j, dims, strs) : ga__lm_offset<4>(j, dims, strs);
+    const long long q = nd == 1 ? ga__lm_offset<1>(i, dims, strs) : nd == 2 ? ga__lm_offset<2>(i, dims, strs)
+                      : nd == 3 ? ga__lm_offset<3>(i, dims, strs) : ga__lm_offset<4>(i, dims, strs);
+    return p == q ? p : -1;
+  }
   return nd == 1 ? ga__lm_offset<1>(i, dims, strs) : nd == 2 ? ga__lm_offset<2>(i, dims, strs)
        : nd == 3 ? ga__lm_offset<3>(i, dims, strs) : ga__lm_offset<4>(i, dims, strs);
 }
