@@ -14,10 +14,13 @@
  *    or in double where an array is GA_DOUBLE, and rounded once when written.
  *    scale is finite as a float.
  *  - Offsets and strides of all arrays are honoured (adjacent row elements on
- *    16- or 32-byte boundaries are fastest). A destination must not overlap the other
+ *    16- or 32-byte boundaries are fastest). Dimensions of ids that lie one
+ *    behind the other in both arrays count as one; more than four that do not
+ *    are GA_UNSUPPORTED_ERROR. A destination must not overlap the other
  *    arrays, nor may two of its elements share a place.
  *  - GA_EMBED_PAD: tokens whose id equals `pad` (compared before the rule for
- *    negative ids) give a row of zeros and add nothing to the gradient.
+ *    negative ids; a GA_ULONG id of 2^63 and more by its bits) give a row of
+ *    zeros and add nothing to the gradient.
  *  - An id outside the table leaves its row of `out` as it was and adds nothing
  *    to the gradient. With GA_EMBED_CHECK the call waits for the result and
  *    returns GA_VALUE_ERROR for it; without, it is not reported and nothing

@@ -19,15 +19,18 @@
  *    and at most 2.358e38, so that scale * log2 e is a float (GA_VALUE_ERROR).
  *    Differences of logits are taken before it: where two finite logits are
  *    further apart than the largest float, the lower one has probability 0.
- *  - Offsets and strides are honoured; inputs of the gradient may have strides
+ *  - Offsets and strides are honoured (rows' dimensions that lie one behind the
+ *    other in all arrays count as one; more than four that do not are
+ *    GA_UNSUPPORTED_ERROR); inputs of the gradient may have strides
  *    of 0 (one dlogp for all rows). Adjacent logits are fastest; rows may start
  *    at any element. dlogits may be the logits themselves; other overlaps of a
  *    destination are not allowed.
  *  - A row without a logit above -inf: logp and the alternatives' values are
  *    -inf, entropy 0, stats (-inf, -inf), gradient 0. A row that holds a NaN or
  *    +inf: NaN in all of them (the indices stay those of the largest numbers).
- *  - GA_LOGPROBS_IGNORE: rows whose target equals `ignore` have logp 0, which has
- *    no gradient: the dlogp term is dropped whatever the row holds.
+ *  - GA_LOGPROBS_IGNORE: rows whose target equals `ignore` (a GA_ULONG of 2^63
+ *    and more by its bits) have logp 0, which has no gradient: the dlogp term is
+ *    dropped whatever the row holds.
  *  - Any other target outside [0, V) gives a logp and a gradient row of NaN,
  *    whatever the row holds; with GA_LOGPROBS_CHECK the call also waits for the
  *    result and returns GA_VALUE_ERROR (not while a CUDA graph is captured:

@@ -457,6 +457,32 @@ def test_logprobs(api, ctx, rng, dtype, kind, rows, V):
 
 
 @pytest.mark.parametrize("dtype", ["f2", "f4"])
+@pytest.mark.parametrize("kind", ["plain", "masked", "ties"])
+@pytest.mark.parametrize("V", [2, 61, 250])
+def test_logprobs_of_short_rows_within_their_few_roundings(api, ctx, rng, dtype, kind, V):
+    """Rows of at most 64 vectors: a lane has three of them at most. A term e^y has 4 u |y| and the
+    instruction's 4 u as in lp_tols, along with what rescaling adds to its exponent; a lane adds at most
+    13 numbers, five additions join the lanes; two rescalings in a lane, that of the lanes' join and the
+    one that takes back a folded product have 6 u each: 46 u. The logarithm is off by 2 u of its size,
+    the difference to the target by 3 u of its own, the result by u."""
+    u = 2.0 ** -24
+    z = rows_of_logits(rng, 37, V, dtype, kind)
+    targets = rng.integers(0, V, 37).astype(np.int64)
+    lp, st = api.GpuArray.empty(ctx, (37,), "f4"), api.GpuArray.empty(ctx, (37, 2), "f4")
+    op = api.GpuLogProbs(ctx, dtype, np.int64)
+    for g in (put(api, ctx, z), at_offset(api, ctx, z, 1)):
+        op(g, put(api, ctx, targets), logp=lp, stats=st, scale=1.0)
+        want, _, _, p, empty = lp_formula(z, targets, 1.0)
+        gap = lp_tols(z, 1.0, p)[2]
+        with np.errstate(invalid="ignore", divide="ignore"):
+            ls = np.log(np.exp(z.astype(np.float64) - np.where(empty, 0, z.max(-1).astype(np.float64))[:, None]).sum(-1))
+        tol = 1.01 * u * (4 * (gap * p).sum(-1) + 46 + 2 * np.where(empty, 0, ls))
+        close(st.to_numpy()[:, 1], np.where(empty, -INF, ls), tol, "log of the sum")
+        t_gap = np.take_along_axis(gap, targets[:, None], -1)[:, 0]
+        close(lp.to_numpy(), want, tol + 1.01 * u * (3 * t_gap + np.where(np.isfinite(want), np.abs(want), 0)), "logp")
+
+
+@pytest.mark.parametrize("dtype", ["f2", "f4"])
 def test_logprobs_rows_that_hide_their_largest_in_few_threads(api, ctx, rng, dtype):
     """values that rise with period 2048 (or 1024) vectors put the largest in the same threads; a
     row of one value; a row of NaNs and infinities"""
@@ -991,6 +1017,41 @@ def test_embed_refusals(api, ctx):
     L = api.lib()
     assert L.GpuArray_embed(out.at, table.at, ids.at, 1.0, 0, 64) == api.GA_INVALID_ERROR
     assert L.GpuArray_embed(None, table.at, ids.at, 1.0, 0, 0) == api.GA_INVALID_ERROR
+
+
+def test_pad_and_ignore_of_unsigned_ids_are_compared_by_their_bits(api, ctx):
+    """-1 names the id 2^64 - 1, and no id of 32 bits"""
+    f, e = np.float32, api.GpuArray.empty
+    table, z = put(api, ctx, np.ones((3, 4), f)), put(api, ctx, np.zeros((2, 4), f))
+    for t, padded in ((np.uint64, True), (np.uint32, False)):
+        ids = put(api, ctx, np.array([2, np.iinfo(t).max], t))
+        out, lp = put(api, ctx, np.full((2, 4), 5, f)), e(ctx, (2,), f)
+        api.embed(out, table, ids, pad=-1)
+        assert (out.to_numpy() == [[1] * 4, [0 if padded else 5] * 4]).all()
+        api.GpuLogProbs(ctx, f, t)(z, ids, logp=lp, ignore=-1)
+        assert lp.to_numpy()[1] == 0 if padded else np.isnan(lp.to_numpy()[1])
+
+
+def test_embed_and_logprobs_refuse_more_than_four_dimensions_apart(api, ctx):
+    """dimensions that lie one behind the other in all arrays count as one: four may be left"""
+    e, f = api.GpuArray.empty, np.float32
+    U = api.GA_UNSUPPORTED_ERROR
+    for nd in (4, 5):
+        shape = (2,) * nd
+        inner = tuple(slice(0, 2) for _ in shape)
+        for gaps in (False, True):
+            ids = put(api, ctx, np.ones((3,) * nd, np.int32))[inner] if gaps else put(api, ctx, np.ones(shape, np.int32))
+            rows, table = e(ctx, shape + (4,), f), put(api, ctx, np.ones((3, 4), f))
+            lp = e(ctx, shape, f)
+            for call in (lambda: api.embed(rows, table, ids), lambda: api.GpuLogProbs(ctx, f, np.int32)(rows, ids, logp=lp),
+                         lambda: api.GpuEmbedGrad(ctx)(table, rows, ids)):
+                if nd == 5 and gaps:
+                    refused(api, U, call)
+                else:
+                    call()
+            if not (nd == 5 and gaps):
+                assert (rows.to_numpy() == 1).all() and (np.abs(lp.to_numpy() + np.log(4)) < 1e-6).all()
+                assert (table.to_numpy() == np.array([[0], [2 ** nd], [0]])).all()
 
 
 def test_logprobs_refusals(api, ctx):
