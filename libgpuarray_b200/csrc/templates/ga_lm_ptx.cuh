@@ -27,12 +27,6 @@ static __device__ __forceinline__ void ga__unpack_h2(unsigned int w, float &lo, 
       : "=f"(lo), "=f"(hi)
       : "r"(w));
 }
-/* both halves plus c, each with one rounding */
-static __device__ __forceinline__ void ga__add_h2_f32(unsigned int w, float c, float &lo, float &hi) {
-  asm("{.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tadd.rn.f32.f16 %0, l, %3;\n\tadd.rn.f32.f16 %1, h, %3;}"
-      : "=f"(lo), "=f"(hi)
-      : "r"(w), "f"(c));
-}
 static __device__ __forceinline__ unsigned int ga__pack_h2(float lo, float hi) {
   unsigned int w;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(hi), "f"(lo));

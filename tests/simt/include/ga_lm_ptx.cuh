@@ -35,15 +35,6 @@ static inline unsigned int __ballot_sync(unsigned, int pred) {
   simt::warp_barrier(w, n);
   return r;
 }
-static inline unsigned int __match_any_sync(unsigned, unsigned int v) {
-  const unsigned w = simt::cur->linear / 32, lane = simt::cur->linear % 32, n = simt::warp_lanes(w);
-  simt::warp_slot[w][lane] = v;
-  simt::warp_barrier(w, n);
-  unsigned int r = 0;
-  for (unsigned l = 0; l < n; l++) r |= (unsigned int)(simt::warp_slot[w][l] == v) << l;
-  simt::warp_barrier(w, n);
-  return r;
-}
 static inline float __fmul_rn(float a, float b) { return a * b; }
 static inline int __popc(unsigned int v) { return __builtin_popcount(v); }
 static inline int __ffs(unsigned int v) { return __builtin_ffs((int)v); }
@@ -66,11 +57,6 @@ static inline void ga__unpack_h2(unsigned int w, float &lo, float &hi) {
   h.data = (ga_ushort)(w >> 16);
   lo = ga_half2float(l);
   hi = ga_half2float(h);
-}
-static inline void ga__add_h2_f32(unsigned int w, float c, float &lo, float &hi) {
-  ga__unpack_h2(w, lo, hi);
-  lo += c;
-  hi += c;
 }
 static inline unsigned int ga__pack_h2(float lo, float hi) {
   return (unsigned int)ga_float2half(lo).data | (unsigned int)ga_float2half(hi).data << 16;
